@@ -1,4 +1,5 @@
-"""ctypes binding of ``libaie_conv.so`` (the C ABI in ``include/aie_conv.h``).
+"""ctypes binding of ``libaie_conv.so`` (the C ABI in ``include/aie_conv.h`` and
+``include/aie_seq.h``).
 
 The product path has no CPU fallback: importing this module on a machine
 without the built library raises, and every ABI call that returns a
@@ -8,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libaie_conv.so")
@@ -98,6 +100,30 @@ SIGNATURES = {
     "aie_conv_run_parts": (C.c_int, [_vp, C.POINTER(TView), _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
+# The argument structs of include/aie_seq.h, packed in one go: pointers and
+# strides (q), sizes (I), flags (i) and floats (f) in the header's order.
+QK_ROPE = struct.Struct("@15q5q2I5q6I2ifI")   # q k v q_out k_out, pages, weights cos_sin positions slots, ...
+PROMPT = struct.Struct("@12qq5I2if")          # q k v out, cu, ...
+PREFIX = struct.Struct("@6q5q2I3qqQ7IifI")    # q out, pages, prefix table lens, workspace, ...
+PAGES = struct.Struct("@6qQ6I")               # kv refs lens table status workspace, page_bytes, ...
+DT_F32, DT_F16, DT_BF16 = 0, 1, 2             # aie_dtype
+PAGES_FULL, PAGES_BAD_ROW = 1, 2              # aie_pages_status
+
+# Every symbol include/aie_seq.h declares; a packed struct goes in as bytes.
+_bp = C.c_char_p
+SEQ_SIGNATURES = {
+    "aie_qk_norm_rope": (C.c_int, [_bp, _vp]),
+    "aie_prompt_attn": (C.c_int, [_bp, _vp]),
+    "aie_prefix_attn": (C.c_int, [_bp, _vp]),
+    "aie_prefix_attn_workspace": (C.c_uint64, [_bp]),
+    "aie_pages_workspace": (C.c_uint64, [C.c_uint32, C.c_uint32]),
+    "aie_pages_grow": (C.c_int, [_bp, _vp, _vp, C.c_uint32, _vp, C.c_uint32, _vp]),
+    "aie_pages_fork": (C.c_int, [_bp, _vp, _vp, C.c_uint32, _vp]),
+    "aie_pages_copy": (C.c_int, [_bp, _vp, _vp, C.c_uint32, _vp]),
+    "aie_pages_free": (C.c_int, [_bp, _vp, C.c_uint32, _vp]),
+    "aie_pages_compact": (C.c_int, [_bp, _vp, _vp]),
+}
+
 _LIB = None
 
 
@@ -110,7 +136,7 @@ def load(path: str = LIB_PATH):
         raise ImportError(f"{path} is missing: build it with `python -m ai_engine_b200.build` "
                           "(the conv path has no CPU fallback)")
     lib = C.CDLL(path)
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in (*SIGNATURES.items(), *SEQ_SIGNATURES.items()):
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args

@@ -1,7 +1,8 @@
 """In-tree build of the CUDA library ``ai_engine_b200/libaie_conv.so``.
 
-One translation unit (``csrc/aie_conv.cu`` includes the kernel headers),
-compiled for sm_100a only.  The CUDA runtime is linked statically, so the
+Two translation units, compiled for sm_100a only and side by side: the conv
+path (``csrc/aie_conv.cu``, which includes the ``k_*.cuh`` kernels) and the
+sequence operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels).  The CUDA runtime is linked statically, so the
 library depends on nothing but the driver; the tensor-map encoder is fetched
 from the driver at run time.
 """
@@ -17,12 +18,13 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaie_conv.so")
-MAIN = os.path.join(CSRC, "aie_conv.cu")
+UNITS = ("aie_conv", "aie_seq")
+OBJ = os.path.join(HERE, "_build")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
+    "-Xcompiler", "-fPIC,-fvisibility=hidden",
     "-cudart", "static",
     "--expt-relaxed-constexpr",
     "-Xptxas", "-warn-spills",
@@ -36,28 +38,48 @@ def nvcc() -> str:
     raise RuntimeError("nvcc not found")
 
 
-def sources():
-    return [MAIN, *glob.glob(os.path.join(CSRC, "*.cuh")), os.path.join(ROOT, "include", "aie_conv.h")]
+def sources(unit=None):
+    """The files a translation unit is made from (None: all of them)."""
+    if unit is None:
+        return sorted({f for u in UNITS for f in sources(u)})
+    headers = [f for f in glob.glob(os.path.join(CSRC, "*.cuh"))
+               if not os.path.basename(f).startswith("seq_" if unit == "aie_conv" else "k_")]
+    api = ["aie_conv.h"] if unit == "aie_conv" else ["aie_conv.h", "aie_seq.h"]
+    return [os.path.join(CSRC, unit + ".cu"), *headers, *(os.path.join(ROOT, "include", h) for h in api)]
+
+
+def _older(path, files) -> bool:
+    return not os.path.exists(path) or any(os.path.getmtime(f) > os.path.getmtime(path) for f in files)
 
 
 def stale() -> bool:
-    if not os.path.exists(LIB):
-        return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(s) > t for s in sources())
+    return _older(LIB, sources())
 
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> str:
     if not force and not stale():
         return LIB
-    cmd = [nvcc(), *NVCC_FLAGS, *extra, MAIN, "-o", LIB + ".tmp"]
-    if verbose:
-        print(" ".join(cmd))
-    subprocess.run(cmd, check=True)
-    os.replace(LIB + ".tmp", LIB)
+    os.makedirs(OBJ, exist_ok=True)
+    objs, jobs, tmp = [], [], f".tmp{os.getpid()}"
+    for u in UNITS:
+        obj = os.path.join(OBJ, u + ".o")
+        objs.append(obj)
+        if force or _older(obj, sources(u)):
+            cmd = [nvcc(), *NVCC_FLAGS, *extra, "-c", os.path.join(CSRC, u + ".cu"), "-o", obj + tmp]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            jobs.append((obj, cmd, subprocess.Popen(cmd)))
+    for obj, cmd, p in jobs:
+        if p.wait() == 0:
+            os.replace(obj + tmp, obj)
+    for _, cmd, p in jobs:
+        if p.returncode:
+            raise subprocess.CalledProcessError(p.returncode, cmd)
+    subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", *objs, "-o", LIB + tmp], check=True)
+    os.replace(LIB + tmp, LIB)
     return LIB
 
 
 if __name__ == "__main__":
     extra = ["-Xptxas", "-v"] if "-v" in sys.argv else []
-    print(build(force=True, verbose=True, extra=extra))
+    print(build(force="--changed" not in sys.argv, verbose=True, extra=extra))

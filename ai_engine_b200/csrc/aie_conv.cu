@@ -3,13 +3,13 @@
 // Host side: descriptor validation, kernel/math choice (the Conv arm of
 // ai-gpu-runtime's lower_op, crates/ai-gpu-runtime/src/lowering.rs:99-187),
 // weight packing, and launch dispatch.  Device side: the kernels in the
-// included .cuh files.  Built as one translation unit for sm_100a.
+// included .cuh files.  The sequence operators (include/aie_seq.h) are a
+// translation unit of their own, aie_seq.cu.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
 #include <atomic>
-#include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
@@ -19,6 +19,7 @@
 
 #include "../../include/aie_conv.h"
 #include "common.cuh"
+#include "host.cuh"
 #include "k_simt.cuh"
 #include "k_tc.cuh"
 #include "k_stem_tc.cuh"
@@ -27,30 +28,6 @@
 #include "k_elem.cuh"
 
 using namespace aie;
-
-// ------------------------------------------------------------ errors ---
-
-static thread_local char t_err[512];
-
-static int fail(int status, const char *fmt, ...)
-{
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(t_err, sizeof t_err, fmt, ap);
-    va_end(ap);
-    return status;
-}
-
-static int cuda_fail(cudaError_t e, const char *what)
-{
-    return fail(AIE_E_CUDA, "%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
-}
-
-#define CUDA_TRY(call)                                  \
-    do {                                                \
-        cudaError_t e_ = (call);                        \
-        if (e_ != cudaSuccess) return cuda_fail(e_, #call); \
-    } while (0)
 
 // -------------------------------------------------------------- plan ---
 
@@ -1366,6 +1343,9 @@ extern "C" int aie_device_status(void *stream, uint32_t *code_out)
     uint32_t v = 0, zero = 0;
     CUDA_TRY(cudaMemcpyFromSymbol(&v, g_aie_error, sizeof v));
     if (v) CUDA_TRY(cudaMemcpyToSymbol(g_aie_error, &zero, sizeof zero));
+    uint32_t vs = 0;
+    CUDA_TRY(seq_take_device_error(&vs));
+    if (!v) v = vs;
     if (code_out) *code_out = v;
     if (v) return fail(AIE_E_DEVICE_TIMEOUT, "device wait gave up, code 0x%08x", v);
     return AIE_OK;

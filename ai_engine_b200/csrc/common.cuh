@@ -356,8 +356,8 @@ __device__ __forceinline__ void tma_load_4d(void *dst, const CUtensorMap *tm, ui
 
 // Device error word set by bounded waits that give up (read and cleared by
 // aie_device_status).  Bit layout: [31:24] kernel id, [23:0] site code.
-// The library is one translation unit, so the definition lives here.
-__device__ uint32_t g_aie_error = 0;
+// Each translation unit has its own word; aie_device_status reads them all.
+static __device__ uint32_t g_aie_error = 0;
 
 __device__ __forceinline__ void report_error(uint32_t code) { atomicCAS(&g_aie_error, 0u, code); }
 

@@ -1,0 +1,63 @@
+// Types and small device helpers of the sequence operators.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/aie_seq.h"
+#include "common.cuh"
+
+namespace aie {
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x)
+{
+    if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(x);
+    else return x;
+}
+
+// [tokens][heads][dim] of type T (aie_heads)
+template <typename T>
+struct HeadsOf {
+    T *p;
+    long long ts, hs;
+    __device__ __forceinline__ T *at(long long t, int h) const { return p + t * ts + h * hs; }
+};
+
+template <typename T>
+static inline HeadsOf<T> heads_of(const aie_heads &h)
+{
+    return HeadsOf<T>{(T *)h.data, (long long)h.token_stride, (long long)h.head_stride};
+}
+
+// One page's places of one head (aie_kv_pages)
+struct PagesGeom {
+    long long ps, ts, hs;
+    int pages, size;
+};
+
+static inline PagesGeom pages_geom(const aie_kv_pages &p)
+{
+    return PagesGeom{(long long)p.page_stride, (long long)p.token_stride, (long long)p.head_stride, (int)p.pages,
+                     (int)p.page_size};
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+__device__ __forceinline__ float warp_max(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+}  // namespace aie

@@ -11,6 +11,7 @@
 #include "host.cuh"
 #include "tc_ptx.cuh"
 #include "seq_common.cuh"
+#include "seq_attn.cuh"
 #include "seq_pages.cuh"
 #include "seq_rope.cuh"
 #include "seq_rows.cuh"
@@ -142,6 +143,49 @@ static int prompt_rows(const aie_prompt &p, cudaStream_t s)
     return launched(cudaGetLastError(), "prompt attention");
 }
 
+// Whether the tensor cores take these heads: 16-bit operands, a head of at
+// most 128 elements in whole 16-byte pieces, a group of query heads that fits
+// a tile, and a scale under which the largest product has the largest weight.
+static bool attn_heads_ok(int32_t dtype, uint32_t hq, uint32_t hk, uint32_t d, float scale)
+{
+    return dtype != AIE_DT_F32 && d % 8 == 0 && d <= 128 && hq / hk <= kAtTile && scale >= 1e-30f && scale <= 1e30f;
+}
+
+template <typename T>
+static cudaError_t attn_prompt_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
+                                      unsigned grid, cudaStream_t s)
+{
+    return a.d <= 64 ? attn_launch<T, 1, false>(q, k, v, a, grid, s) : attn_launch<T, 2, false>(q, k, v, a, grid, s);
+}
+
+static int prompt_tc(const aie_prompt &p, cudaStream_t s)
+{
+    AttnArgs a = {};
+    a.cu = p.cu;
+    a.out = p.out.data;
+    a.out_ts = p.out.token_stride; a.out_hs = p.out.head_stride;
+    a.tokens = (int)p.tokens; a.seqs = (int)p.seqs;
+    a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
+    a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
+    a.causal = p.causal != 0;
+    a.vec_out = (uintptr_t)p.out.data % 16 == 0 && p.out.token_stride % 8 == 0 && p.out.head_stride % 8 == 0;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    const bool bf16 = p.dtype == AIE_DT_BF16;
+    CUtensorMap q, k, v;
+    if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.tokens, p.q.token_stride, 0, 0, a.group,
+                  a.tokens_per_tile) ||
+        !attn_map(&k, bf16, p.k.data, p.head_dim, p.kv_heads, p.k.head_stride, p.tokens, p.k.token_stride, 0, 0, 1, kAtTile) ||
+        !attn_map(&v, bf16, p.v.data, p.head_dim, p.kv_heads, p.v.head_stride, p.tokens, p.v.token_stride, 0, 0, 1, kAtTile))
+        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
+    // no more pairs of tiles than whole ones, and one that is not whole per sequence
+    const uint64_t pairs = p.tokens / (2 * a.tokens_per_tile) + std::min(p.seqs, p.tokens);
+    const uint64_t grid = pairs * p.kv_heads;
+    if (grid > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "too many tiles");
+    return launched(bf16 ? attn_prompt_launch<__nv_bfloat16>(q, k, v, a, (unsigned)grid, s)
+                         : attn_prompt_launch<__half>(q, k, v, a, (unsigned)grid, s),
+                    "prompt attention");
+}
+
 extern "C" int aie_prompt_attn(const aie_prompt *p, void *stream)
 {
     if (!p) return fail(AIE_E_INVALID, "null arguments");
@@ -157,6 +201,11 @@ extern "C" int aie_prompt_attn(const aie_prompt *p, void *stream)
     TRY(check_heads(p->out, p->dtype, "out"));
     if ((uint64_t)p->tokens * p->q_heads > 0x1ffffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^33 query rows");
     cudaStream_t s = (cudaStream_t)stream;
+    if (attn_heads_ok(p->dtype, p->q_heads, p->kv_heads, p->head_dim, p->scale) &&
+        attn_addressable(p->q.data, p->q.token_stride, p->q.head_stride, p->tokens, p->q_heads) &&
+        attn_addressable(p->k.data, p->k.token_stride, p->k.head_stride, p->tokens, p->kv_heads) &&
+        attn_addressable(p->v.data, p->v.token_stride, p->v.head_stride, p->tokens, p->kv_heads))
+        return prompt_tc(*p, s);
     if (p->dtype == AIE_DT_F32) return prompt_rows<float>(*p, s);
     return p->dtype == AIE_DT_F16 ? prompt_rows<__half>(*p, s) : prompt_rows<__nv_bfloat16>(*p, s);
 }
@@ -174,21 +223,92 @@ static int check_prefix(const aie_prefix *p)
     return AIE_OK;
 }
 
+// How the shared part is computed: over key tiles in `splits` pieces on the
+// tensor cores, or (0) with the streams' own part, row by row.
+struct PrefixPlan {
+    int splits, tiles_per_split, row_pairs;
+    uint64_t part_o, bytes;  // the partial results' place in the workspace, and its size
+};
+
+static PrefixPlan prefix_plan(const aie_prefix &p)
+{
+    PrefixPlan w = {};
+    const uint32_t keys = std::min(p.prefix_len, p.max_len), size = p.pages.page_size;
+    const bool pages_ok = size >= 8 && (size <= kAtTile ? kAtTile % size == 0 : size % kAtTile == 0);
+    if (keys && p.batch && pages_ok && attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) &&
+        attn_addressable(p.q.data, p.q.token_stride, p.q.head_stride, p.batch, p.q_heads) &&
+        attn_addressable(p.pages.k, p.pages.token_stride, p.pages.head_stride, size, p.kv_heads) &&
+        attn_addressable(p.pages.v, p.pages.page_stride, 8, p.pages.pages, 1)) {
+        const int tiles = (int)((keys + kAtTile - 1) / kAtTile);
+        const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads);
+        w.row_pairs = ((int)p.batch + 2 * tpt - 1) / (2 * tpt);
+        // one block per SM; pieces of whole tiles
+        const int units = w.row_pairs * (int)p.kv_heads;
+        w.splits = std::min(tiles, std::max(1, tc_sm_count() / units));
+        w.tiles_per_split = (tiles + w.splits - 1) / w.splits;
+        w.splits = (tiles + w.tiles_per_split - 1) / w.tiles_per_split;
+    }
+    const uint64_t rows = (uint64_t)p.batch * p.q_heads;
+    w.part_o = (w.splits * rows * 4 + 15) / 16 * 16;
+    w.bytes = w.part_o + w.splits * rows * p.head_dim * 4 + 16;
+    return w;
+}
+
 extern "C" uint64_t aie_prefix_attn_workspace(const aie_prefix *p)
 {
-    return check_prefix(p) ? 0 : 16;
+    return check_prefix(p) ? 0 : prefix_plan(*p).bytes;
 }
 
 template <typename T>
-static int prefix_rows(const aie_prefix &p, cudaStream_t s)
+static cudaError_t attn_prefix_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
+                                      unsigned grid, cudaStream_t s)
+{
+    return a.d <= 64 ? attn_launch<T, 1, true>(q, k, v, a, grid, s) : attn_launch<T, 2, true>(q, k, v, a, grid, s);
+}
+
+static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
+{
+    AttnArgs a = {};
+    a.prefix = p.prefix; a.lens = p.lens;
+    a.part_lse = (float *)p.workspace;
+    a.part_o = (float *)((char *)p.workspace + w.part_o);
+    a.tokens = (int)p.batch;
+    a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
+    a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
+    a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len;
+    a.page_size = (int)p.pages.page_size; a.pages = (int)p.pages.pages;
+    a.splits = w.splits; a.tiles_per_split = w.tiles_per_split;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    const bool bf16 = p.dtype == AIE_DT_BF16;
+    const aie_kv_pages &g = p.pages;
+    const uint32_t rows = std::min(g.page_size, (uint32_t)kAtTile);
+    CUtensorMap q, k, v;
+    if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.batch, p.q.token_stride, 0, 0, a.group,
+                  a.tokens_per_tile) ||
+        !attn_map(&k, bf16, g.k, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  rows) ||
+        !attn_map(&v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  rows))
+        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
+    const uint64_t grid = (uint64_t)w.row_pairs * p.kv_heads * w.splits;
+    if (grid > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "too many tiles");
+    return launched(bf16 ? attn_prefix_launch<__nv_bfloat16>(q, k, v, a, (unsigned)grid, s)
+                         : attn_prefix_launch<__half>(q, k, v, a, (unsigned)grid, s),
+                    "prefix attention");
+}
+
+template <typename T>
+static int prefix_rows(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
 {
     PrefixRows<T> a;
     a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
     a.k = (const T *)p.pages.k; a.v = (const T *)p.pages.v;
     a.g = pages_geom(p.pages);
     a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
+    a.part_lse = (const float *)p.workspace;
+    a.part_o = (const float *)((const char *)p.workspace + w.part_o);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
-    a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
+    a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
     a.scale = p.scale;
     const long long rows = (long long)p.batch * p.q_heads;
     prefix_rows_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
@@ -211,12 +331,13 @@ extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
             return fail(AIE_E_INVALID, "rows of %u pages of %u do not hold max_len %u", p->table_stride,
                         p->pages.page_size, p->max_len);
     }
-    if (p->workspace_bytes < aie_prefix_attn_workspace(p) || !p->workspace || (uintptr_t)p->workspace % 16)
-        return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed",
-                    (unsigned long long)aie_prefix_attn_workspace(p));
+    const PrefixPlan w = prefix_plan(*p);
+    if (p->workspace_bytes < w.bytes || !p->workspace || (uintptr_t)p->workspace % 16)
+        return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)w.bytes);
     cudaStream_t s = (cudaStream_t)stream;
-    if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, s);
-    return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, s) : prefix_rows<__nv_bfloat16>(*p, s);
+    if (w.splits) TRY(prefix_tc(*p, w, s));
+    if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, w, s);
+    return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, w, s) : prefix_rows<__nv_bfloat16>(*p, w, s);
 }
 
 // --------------------------------------------------------------- pages ---

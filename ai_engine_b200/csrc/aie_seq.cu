@@ -15,6 +15,7 @@
 #include "seq_pages.cuh"
 #include "seq_rope.cuh"
 #include "seq_rows.cuh"
+#include "seq_step.cuh"
 
 using namespace aie;
 
@@ -223,10 +224,11 @@ static int check_prefix(const aie_prefix *p)
     return AIE_OK;
 }
 
-// How the shared part is computed: over key tiles in `splits` pieces on the
-// tensor cores, or (0) with the streams' own part, row by row.
+// How a call is computed.  The shared part: over key tiles in `splits` pieces
+// on the tensor cores, or (0) with the streams' own part.  That: `pieces`
+// blocks per stream and key head, or (0) row by row.
 struct PrefixPlan {
-    int splits, tiles_per_split, row_pairs;
+    int splits, tiles_per_split, row_pairs, pieces;
     uint64_t part_o, bytes;  // the partial results' place in the workspace, and its size
 };
 
@@ -234,11 +236,12 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
 {
     PrefixPlan w = {};
     const uint32_t keys = std::min(p.prefix_len, p.max_len), size = p.pages.page_size;
+    const bool heads_ok = attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) &&
+                          attn_addressable(p.pages.k, p.pages.token_stride, p.pages.head_stride, size, p.kv_heads) &&
+                          attn_addressable(p.pages.v, p.pages.page_stride, 8, p.pages.pages, 1);
     const bool pages_ok = size >= 8 && (size <= kAtTile ? kAtTile % size == 0 : size % kAtTile == 0);
-    if (keys && p.batch && pages_ok && attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) &&
-        attn_addressable(p.q.data, p.q.token_stride, p.q.head_stride, p.batch, p.q_heads) &&
-        attn_addressable(p.pages.k, p.pages.token_stride, p.pages.head_stride, size, p.kv_heads) &&
-        attn_addressable(p.pages.v, p.pages.page_stride, 8, p.pages.pages, 1)) {
+    if (keys && p.batch && pages_ok && heads_ok &&
+        attn_addressable(p.q.data, p.q.token_stride, p.q.head_stride, p.batch, p.q_heads)) {
         const int tiles = (int)((keys + kAtTile - 1) / kAtTile);
         const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads);
         w.row_pairs = ((int)p.batch + 2 * tpt - 1) / (2 * tpt);
@@ -247,6 +250,13 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
         w.splits = std::min(tiles, std::max(1, tc_sm_count() / units));
         w.tiles_per_split = (tiles + w.splits - 1) / w.splits;
         w.splits = (tiles + w.tiles_per_split - 1) / w.tiles_per_split;
+    }
+    if (heads_ok && p.kv_heads <= 65535) {
+        // two blocks per SM, each with four tiles of places or more
+        const int places = (int)(p.max_len - (w.splits ? keys : 0));
+        const uint64_t units = (uint64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16);
+        w.pieces = 1;
+        while (w.pieces < kStMostPieces && w.pieces * units < 2ull * tc_sm_count() && w.pieces * 4 * kStKeys < places) w.pieces *= 2;
     }
     const uint64_t rows = (uint64_t)p.batch * p.q_heads;
     w.part_o = (w.splits * rows * 4 + 15) / 16 * 16;
@@ -315,6 +325,26 @@ static int prefix_rows(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     return launched(cudaGetLastError(), "prefix attention");
 }
 
+template <typename T>
+static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
+{
+    StepArgs<T> a;
+    a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
+    a.k = (const T *)p.pages.k; a.v = (const T *)p.pages.v;
+    a.g = pages_geom(p.pages);
+    a.size = make_fastdiv((int)p.pages.page_size);
+    a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
+    a.part_lse = (const float *)p.workspace;
+    a.part_o = (const float *)((const char *)p.workspace + w.part_o);
+    a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.hk = (int)p.kv_heads; a.group = (int)(p.q_heads / p.kv_heads);
+    a.d = (int)p.head_dim;
+    a.shared = (int)p.prefix_len; a.from = w.splits ? a.shared : 0;
+    a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    return launched(a.d <= 64 ? step_launch<T, 64>(a, w.pieces, w.splits > 0, s) : step_launch<T, 128>(a, w.pieces, w.splits > 0, s),
+                    "prefix attention");
+}
+
 extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
 {
     TRY(check_prefix(p));
@@ -336,6 +366,7 @@ extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
         return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)w.bytes);
     cudaStream_t s = (cudaStream_t)stream;
     if (w.splits) TRY(prefix_tc(*p, w, s));
+    if (w.pieces) return p->dtype == AIE_DT_F16 ? prefix_step<__half>(*p, w, s) : prefix_step<__nv_bfloat16>(*p, w, s);
     if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, w, s);
     return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, w, s) : prefix_rows<__nv_bfloat16>(*p, w, s);
 }

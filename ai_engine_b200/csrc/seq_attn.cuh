@@ -279,6 +279,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         for (int t = 0; t < 2; t++) steps[t] = max(min(steps[t], step0 + a.tiles_per_split), step0);
     }
     const int n = max(steps[0], steps[1]);
+    // the streams' own part (prefix_step_kernel) may start beside this one
+    if constexpr (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));

@@ -245,11 +245,19 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
         const int tiles = (int)((keys + kAtTile - 1) / kAtTile);
         const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads);
         w.row_pairs = ((int)p.batch + 2 * tpt - 1) / (2 * tpt);
-        // one block per SM; pieces of whole tiles
-        const int units = w.row_pairs * (int)p.kv_heads;
-        w.splits = std::min(tiles, std::max(1, tc_sm_count() / units));
-        w.tiles_per_split = (tiles + w.splits - 1) / w.splits;
-        w.splits = (tiles + w.tiles_per_split - 1) / w.tiles_per_split;
+        // one block per SM at a time: the pieces (of whole tiles) that give the
+        // shortest run, a block costing about three tiles besides its own
+        const long long units = (long long)w.row_pairs * p.kv_heads, sms = tc_sm_count();
+        long long best = 0;
+        for (int want = 1; want <= std::min(tiles, kAtMostSplits); want++) {
+            const int per = (tiles + want - 1) / want, splits = (tiles + per - 1) / per;
+            const long long cost = (units * splits + sms - 1) / sms * (per + 3);
+            if (!best || cost < best) {
+                best = cost;
+                w.splits = splits;
+                w.tiles_per_split = per;
+            }
+        }
     }
     if (heads_ok && p.kv_heads <= 65535) {
         // two blocks per SM, each with four tiles of places or more
@@ -341,6 +349,7 @@ static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.shared = (int)p.prefix_len; a.from = w.splits ? a.shared : 0;
     a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
     a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.q_pairs = (uintptr_t)p.q.data % 4 == 0 && p.q.token_stride % 2 == 0 && p.q.head_stride % 2 == 0;
     return launched(a.d <= 64 ? step_launch<T, 64>(a, w.pieces, w.splits > 0, s) : step_launch<T, 128>(a, w.pieces, w.splits > 0, s),
                     "prefix attention");
 }

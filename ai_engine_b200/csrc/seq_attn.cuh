@@ -38,6 +38,7 @@ constexpr int kAtThreads = 384;
 constexpr int kAtRowRegs = 216, kAtIssueRegs = 72;
 constexpr int kAtTile = 128;      // query rows of a tile, keys of a step
 constexpr uint32_t kAtBlockBytes = kAtTile * 128;  // 128 rows of 64 16-bit elements
+constexpr int kAtMostSplits = 64; // pieces of the shared prefix
 constexpr uint32_t kAtErr = 0x41000000u;
 
 // --------------------------------------------------------------- PTX ---

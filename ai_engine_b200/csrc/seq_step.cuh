@@ -37,6 +37,7 @@ struct StepArgs {
     const int32_t *prefix, *table, *lens;
     const float *part_o, *part_lse;  // the shared part's results, `splits` of them
     int batch, hq, hk, group, d, from, shared, max_len, table_stride, splits;
+    int q_pairs;  // two elements of q are 4-byte aligned
     float scale_log2;
 };
 
@@ -77,6 +78,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
                      "{%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void add_scaled(float4 &x, float f, const float4 &y)
+{
+    x.x = fmaf(f, y.x, x.x);
+    x.y = fmaf(f, y.y, x.y);
+    x.z = fmaf(f, y.z, x.z);
+    x.w = fmaf(f, y.w, x.w);
 }
 
 template <int DK>
@@ -123,7 +132,8 @@ prefix_step_kernel(const StepArgs<T> a)
                 uint32_t x = 0;
                 if (row < heads && col < a.d) {  // d is even
                     const T *p = a.q.at(b, kvh * a.group + row0 + row) + col;
-                    x = (uint32_t)*(const unsigned short *)p | (uint32_t)*(const unsigned short *)(p + 1) << 16;
+                    x = a.q_pairs ? *(const uint32_t *)p
+                                  : (uint32_t)*(const unsigned short *)p | (uint32_t)*(const unsigned short *)(p + 1) << 16;
                 }
                 qa[k][i] = x;
             }
@@ -248,17 +258,18 @@ prefix_step_kernel(const StepArgs<T> a)
         }
     }
     __syncthreads();
-    for (int e = tid; e < heads * DK; e += kStThreads) {
-        const int r = e / DK, c = e % DK;
+    for (int e = tid; e < heads * (DK / 4); e += kStThreads) {
+        const int r = e / (DK / 4), c = e % (DK / 4);
         const float top = fmaxf(fmaxf(warp_m[0][r], warp_m[1][r]), fmaxf(warp_m[2][r], warp_m[3][r]));
-        float x = 0.f, sum = 0.f;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; w++) {
             const float f = warp_m[w][r] == -INFINITY && warp_l[w][r] == 0.f ? 0.f : ex2(warp_m[w][r] - top);
-            x = fmaf(f, ((const float *)(smem + w * Sm::kO))[r * DK + c], x);
+            add_scaled(x, f, ((const float4 *)(smem + w * Sm::kO))[r * (DK / 4) + c]);
             sum = fmaf(f, warp_l[w][r], sum);
         }
-        block_o[r * DK + c] = x;
+        ((float4 *)block_o)[r * (DK / 4) + c] = x;
         if (c == 0) {
             block_m[r] = top;
             block_l[r] = sum;
@@ -266,31 +277,54 @@ prefix_step_kernel(const StepArgs<T> a)
     }
     // the shared part's launch may still run: its results from here on
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    cluster.sync();
-    // ---- all partial results of a row; the cluster's blocks take turns at the elements
-    const long long rows = (long long)a.batch * a.hq;
-    for (int e = rank * kStThreads + tid; e < heads * a.d; e += ranks * kStThreads) {
-        const int r = e / a.d, c = e % a.d, h = kvh * a.group + row0 + r;
-        const long long prow = (long long)b * a.hq + h;
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    // ---- a row's partial results: the cluster's blocks, then the shared
+    // part's pieces.  Their weights first, a warp per row.
+    const long long rows = (long long)a.batch * a.hq, prow0 = (long long)b * a.hq + kvh * a.group + row0;
+    const int parts = ranks + a.splits;
+    float *const weight = (float *)smem;  // [row][part], over the ring
+    for (int r = warp; r < heads; r += 4) {
         float top = -INFINITY;
-        for (int i = 0; i < ranks; i++) top = fmaxf(top, *cluster.map_shared_rank(&block_m[r], i));
-        for (int i = 0; i < a.splits; i++) top = fmaxf(top, a.part_lse[i * rows + prow]);
-        float x = 0.f, sum = 0.f;
-        for (int i = 0; i < ranks; i++) {
-            const float bm = *cluster.map_shared_rank(&block_m[r], i), bl = *cluster.map_shared_rank(&block_l[r], i);
-            const float f = bm == -INFINITY && bl == 0.f ? 0.f : ex2(bm - top);
-            x = fmaf(f, *cluster.map_shared_rank(&block_o[r * DK + c], i), x);
-            sum = fmaf(f, bl, sum);
+        for (int i = lane; i < parts; i += 32) {
+            float w;
+            if (i < ranks) {
+                w = *cluster.map_shared_rank(&block_m[r], i);
+                if (w == -INFINITY && *cluster.map_shared_rank(&block_l[r], i) != 0.f) w = __int_as_float(0x7fffffff);
+            } else w = a.part_lse[(i - ranks) * rows + prow0 + r];
+            weight[r * parts + i] = w;
+            top = fmaxf(top, w);
         }
-        for (int i = 0; i < a.splits; i++) {
-            const float lse = a.part_lse[i * rows + prow];
-            const float f = lse == -INFINITY ? 0.f : ex2(lse - top);
-            x = fmaf(f, a.part_o[(i * rows + prow) * a.d + c], x);
-            sum += f;
+        top = warp_max(top);
+        float sum = 0.f;
+        for (int i = lane; i < parts; i += 32) {
+            // nothing seen: no weight
+            const float w = weight[r * parts + i], f = w == -INFINITY ? 0.f : ex2(w - top);
+            weight[r * parts + i] = f;
+            sum += i < ranks ? f * *cluster.map_shared_rank(&block_l[r], i) : f;
         }
-        a.o.at(b, h)[c] = from_f32<T>(len > 0 ? x / sum : 0.f);
+        sum = warp_sum(sum);
+        if (lane == 0) warp_l[0][r] = len > 0 ? 1.f / sum : 0.f;
     }
-    cluster.sync();  // a block's results stay until the others have read them
+    __syncthreads();
+    // the cluster's blocks take turns at the elements
+    const int quads = a.d / 4;
+    for (int e = rank * kStThreads + tid; e < heads * quads; e += ranks * kStThreads) {
+        const int r = e / quads, c = e % quads;
+        const float *w = weight + r * parts;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < ranks; i++) add_scaled(x, w[i], ((const float4 *)cluster.map_shared_rank(block_o, i))[r * (DK / 4) + c]);
+        const float4 *o = (const float4 *)(a.part_o + (prow0 + r) * a.d) + c;
+#pragma unroll 8
+        for (int i = 0; i < a.splits; i++) add_scaled(x, w[ranks + i], o[i * rows * quads]);
+        const float f = warp_l[0][r];
+        T *dst = a.o.at(b, kvh * a.group + row0 + r) + 4 * c;
+        dst[0] = from_f32<T>(len > 0 ? x.x * f : 0.f);
+        dst[1] = from_f32<T>(len > 0 ? x.y * f : 0.f);
+        dst[2] = from_f32<T>(len > 0 ? x.z * f : 0.f);
+        dst[3] = from_f32<T>(len > 0 ? x.w * f : 0.f);
+    }
+    if (ranks > 1) cluster.sync();  // a block's results stay until the others have read them
 }
 
 // Largest number of blocks that share one stream's places.

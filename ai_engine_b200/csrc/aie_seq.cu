@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <numeric>
 #include <utility>
 #include <vector>
 
@@ -236,11 +237,11 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
 {
     PrefixPlan w = {};
     const uint32_t keys = std::min(p.prefix_len, p.max_len), size = p.pages.page_size;
-    const bool heads_ok = attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) &&
+    // pages of whole swizzle atoms: 8 places
+    const bool heads_ok = attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) && size % 8 == 0 &&
                           attn_addressable(p.pages.k, p.pages.token_stride, p.pages.head_stride, size, p.kv_heads) &&
                           attn_addressable(p.pages.v, p.pages.page_stride, 8, p.pages.pages, 1);
-    const bool pages_ok = size >= 8 && (size <= kAtTile ? kAtTile % size == 0 : size % kAtTile == 0);
-    if (keys && p.batch && pages_ok && heads_ok &&
+    if (keys && p.batch && heads_ok &&
         attn_addressable(p.q.data, p.q.token_stride, p.q.head_stride, p.batch, p.q_heads)) {
         const int tiles = (int)((keys + kAtTile - 1) / kAtTile);
         const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads);
@@ -259,12 +260,12 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
             }
         }
     }
-    if (heads_ok && p.kv_heads <= 65535) {
-        // two blocks per SM, each with four tiles of places or more
-        const int places = (int)(p.max_len - (w.splits ? keys : 0));
-        const uint64_t units = (uint64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16);
+    const uint64_t units = (uint64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16);
+    if (heads_ok && (w.splits || !keys) && units <= 0x3fffffffu) {
+        // up to two blocks per SM, each with four tiles of places or more
+        const int places = (int)(p.max_len - keys);
         w.pieces = 1;
-        while (w.pieces < kStMostPieces && w.pieces * units < 2ull * tc_sm_count() && w.pieces * 4 * kStKeys < places) w.pieces *= 2;
+        while (w.pieces < kStMostPieces && 2 * w.pieces * units <= 2ull * tc_sm_count() && w.pieces * 4 * kStKeys < places) w.pieces *= 2;
     }
     const uint64_t rows = (uint64_t)p.batch * p.q_heads;
     w.part_o = (w.splits * rows * 4 + 15) / 16 * 16;
@@ -299,7 +300,8 @@ static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.scale_log2 = p.scale * 1.4426950408889634f;
     const bool bf16 = p.dtype == AIE_DT_BF16;
     const aie_kv_pages &g = p.pages;
-    const uint32_t rows = std::min(g.page_size, (uint32_t)kAtTile);
+    const uint32_t rows = std::gcd(g.page_size, (uint32_t)kAtTile);  // of a box: inside one page, whole boxes a tile
+    a.box_rows = (int)rows;
     CUtensorMap q, k, v;
     if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.batch, p.q.token_stride, 0, 0, a.group,
                   a.tokens_per_tile) ||
@@ -336,21 +338,30 @@ static int prefix_rows(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
 template <typename T>
 static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
 {
-    StepArgs<T> a;
+    const aie_kv_pages &g = p.pages;
+    StepArgs<T> a = {};
     a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
-    a.k = (const T *)p.pages.k; a.v = (const T *)p.pages.v;
-    a.g = pages_geom(p.pages);
-    a.size = make_fastdiv((int)p.pages.page_size);
-    a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
+    a.size = make_fastdiv((int)g.page_size);
+    a.table = p.table; a.lens = p.lens;
     a.part_lse = (const float *)p.workspace;
     a.part_o = (const float *)((const char *)p.workspace + w.part_o);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.hk = (int)p.kv_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim;
-    a.shared = (int)p.prefix_len; a.from = w.splits ? a.shared : 0;
+    a.from = (int)p.prefix_len;
     a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
-    a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.pages = (int)g.pages; a.page_size = (int)g.page_size; a.box_rows = std::gcd((int)g.page_size, kStKeys);
+    a.zs = (a.group + 15) / 16; a.units = a.batch * a.hk * a.zs; a.rows = std::min(a.group, 16);
     a.q_pairs = (uintptr_t)p.q.data % 4 == 0 && p.q.token_stride % 2 == 0 && p.q.head_stride % 2 == 0;
-    return launched(a.d <= 64 ? step_launch<T, 64>(a, w.pieces, w.splits > 0, s) : step_launch<T, 128>(a, w.pieces, w.splits > 0, s),
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    const bool bf16 = p.dtype == AIE_DT_BF16;
+    CUtensorMap k, v;
+    if (!attn_map(&k, bf16, g.k, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  a.box_rows) ||
+        !attn_map(&v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  a.box_rows))
+        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
+    const bool behind = w.splits > 0;
+    return launched(a.d <= 64 ? step_launch<T, 64>(k, v, a, w.pieces, behind, s) : step_launch<T, 128>(k, v, a, w.pieces, behind, s),
                     "prefix attention");
 }
 

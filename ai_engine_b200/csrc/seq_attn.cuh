@@ -161,7 +161,7 @@ struct AttnArgs {
     int tokens, seqs;         // prompts: packed tokens; shared prefix: streams
     int kv_heads, q_heads, group, d, tokens_per_tile;
     int causal, vec_out;
-    int shared, max_len, page_size, pages, splits, tiles_per_split;
+    int shared, max_len, page_size, pages, box_rows, splits, tiles_per_split;
     float scale_log2;
 };
 
@@ -440,7 +440,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                         w.first + tok0 + t * tpt);
                 }
                 // paged: each lane copies one page's part of a tile
-                const int rows = PAGED ? min(a.page_size, kAtTile) : kAtTile;
+                const int rows = PAGED ? a.box_rows : kAtTile;
                 auto page_of = [&](int step) {
                     const int place = step * kAtTile + lane * rows;
                     // past the prefix: a page that does not exist, read as zeros

@@ -6,13 +6,13 @@
 //   has weight 2^(m_i - m):  out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i
 //
 // Each place is read once and used for a group of query heads: memory-bound.
-// A block takes a piece of one stream's places for one key/value head, 64 at
-// a time through a ring of shared memory filled by asynchronous copies; each
-// of its four warps multiplies 16 of the 64 (m16n8k16, the group padded to
-// 16 rows) and carries its own m, l and O.  Where streams are few, the pieces
-// of one stream are a cluster of up to 8 blocks, whose results meet in
-// distributed shared memory.  Fixed order throughout: results repeat bit for
-// bit.
+// A block goes through (stream, key/value head) pairs.  One warp copies tiles
+// of 64 places into a ring of shared memory (TMA, a box per page or part of
+// one) and runs ahead into the next pair; four warps multiply 16 of the 64
+// places each (m16n8k16, the group padded to 16 rows) and carry their own m, l
+// and O.  Where streams are few, the places of one stream are split over a
+// cluster of up to 8 blocks, whose results meet in distributed shared memory.
+// Fixed order throughout: results repeat bit for bit.
 //
 // Rounding to fewer bits: the weights to the operands' type for the product
 // with V (l sums them unrounded), and the result.
@@ -23,32 +23,25 @@
 
 namespace aie {
 
-constexpr int kStKeys = 64;      // places of one ring stage
-constexpr int kStStages = 3;
-constexpr int kStThreads = 128;
-constexpr int kStList = 1024;    // page numbers held at a time
+constexpr int kStKeys = 64;        // places of one ring stage
+constexpr int kStThreads = 160;    // four warps that multiply, one that copies
+constexpr int kStMostPieces = 8;   // largest number of blocks that share one stream's places
+constexpr int kStMostStages = 3;
+constexpr uint32_t kStErr = 0x42000000u;
 
 template <typename T>
 struct StepArgs {
     HeadsOf<T> q, o;
-    const T *k, *v;
-    PagesGeom g;
     FastDiv size;
-    const int32_t *prefix, *table, *lens;
+    const int32_t *table, *lens;
     const float *part_o, *part_lse;  // the shared part's results, `splits` of them
-    int batch, hq, hk, group, d, from, shared, max_len, table_stride, splits;
-    int q_pairs;  // two elements of q are 4-byte aligned
+    int batch, hq, hk, group, d, from, max_len, table_stride, splits;
+    int pages, page_size, box_rows;  // places of one box: the greatest common divisor of a page's and a tile's
+    int units, zs, rows;             // (stream, key head, 16 heads of the group) triples; rows kept: min(group, 16)
+    int stages;
+    int q_pairs;                     // two elements of q are 4-byte aligned
     float scale_log2;
 };
-
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool real)
-{
-    const int n = real ? 16 : 0;  // 0: zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4])
 {
@@ -90,256 +83,329 @@ __device__ __forceinline__ void add_scaled(float4 &x, float f, const float4 &y)
 
 template <int DK>
 struct StepSmem {
-    static constexpr uint32_t kTile = kStKeys * DK * 2;          // K or V of a stage
-    static constexpr uint32_t kRing = kStStages * 2 * kTile;     // reused for the warps' O at the end
-    static constexpr uint32_t kO = 16 * DK * 4;                  // one result of 16 rows
-    static constexpr uint32_t kBytes = kRing + kO;               // ring, the block's result
-    static_assert(4 * kO <= kRing, "the warps' results fit the ring");
+    static constexpr uint32_t kBlock = kStKeys * 128;             // 64 places of 64 elements
+    static constexpr uint32_t kTile = DK / 64 * kBlock;           // K or V of a stage
+    static constexpr uint32_t kStage = 2 * kTile;
+    // the warps' results, then the weights of `parts` partial results per row
+    static uint32_t bytes(int stages, int rows, int parts) { return stages * kStage + 4 * rows * DK * 4 + rows * parts * 4 + 1024; }
 };
+
+struct StepShared {
+    uint64_t full[kStMostStages], empty[kStMostStages];
+    float warp_m[4][16], warp_l[4][16], block_m[16], block_l[16], inv[16];
+    uint32_t abort;
+};
+
+__device__ __forceinline__ void step_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }  // the four multiplying warps
 
 template <typename T, int DK>
 __global__ void __launch_bounds__(kStThreads)
-prefix_step_kernel(const StepArgs<T> a)
+prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const StepArgs<T> a)
 {
     namespace cg = cooperative_groups;
     using Sm = StepSmem<DK>;
-    constexpr int kChunks = DK / 8;  // 16-byte pieces of a head
-    extern __shared__ __align__(128) char smem[];
-    __shared__ int32_t list[kStList];
-    __shared__ float warp_m[4][16], warp_l[4][16], block_m[16], block_l[16];
+    extern __shared__ char smem_raw[];
+    __shared__ StepShared sh;
+    char *const smem = (char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    float *const result = (float *)(smem + a.stages * Sm::kStage);  // [warp][row][DK]; the first becomes the block's
+    float *const weight = result + 4 * a.rows * DK;                 // [row][part]
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int kvh = blockIdx.y, row0 = blockIdx.z * 16;
-    const int b = blockIdx.x / ranks;
-    const int heads = min(a.group - row0, 16);
-    float *const block_o = (float *)(smem + Sm::kRing);
 
-    // this block's places [lo, hi): whole tiles of 64
-    const int len = min(max(a.lens[b], 0), a.max_len);
-    const int tiles = (max(len - a.from, 0) + kStKeys - 1) / kStKeys, per = (tiles + ranks - 1) / ranks;
-    const int lo = a.from + min(rank * per, tiles) * kStKeys, hi = min(a.from + min((rank + 1) * per, tiles) * kStKeys, len);
-
-    // the group's queries, padded to 16 rows, as the A operand
-    uint32_t qa[DK / 16][4];
-    {
-        const int r = lane >> 2, c = (lane & 3) * 2;
-#pragma unroll
-        for (int k = 0; k < DK / 16; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int row = r + (i & 1) * 8, col = k * 16 + c + (i >> 1) * 8;
-                uint32_t x = 0;
-                if (row < heads && col < a.d) {  // d is even
-                    const T *p = a.q.at(b, kvh * a.group + row0 + row) + col;
-                    x = a.q_pairs ? *(const uint32_t *)p
-                                  : (uint32_t)*(const unsigned short *)p | (uint32_t)*(const unsigned short *)(p + 1) << 16;
-                }
-                qa[k][i] = x;
-            }
+    if (tid == 0) {
+        for (int i = 0; i < a.stages; i++) {
+            mbar_init(&sh.full[i], 1);
+            mbar_init(&sh.empty[i], 4);
+        }
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    float o[DK / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < DK / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    __syncthreads();
+    volatile uint32_t *abort = &sh.abort;
+    auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t site) {
+        if (mbar_wait(bar, parity)) return true;
+        report_error(kStErr | site);
+        *abort = 1;
+        return false;
+    };
+    // a unit's tiles of 64 places, this block's part of them
+    auto tiles_of = [&](int b, int &len, int &lo, int &hi) {
+        len = min(max(a.lens[b], 0), a.max_len);
+        const int first = a.from / kStKeys, end = len > a.from ? (len - 1) / kStKeys + 1 : first;
+        const int per = (end - first + ranks - 1) / ranks;
+        lo = min(first + rank * per, end);
+        hi = min(lo + per, end);
+    };
+    int ring = 0;  // tiles so far, over all units
+    bool ok = true;
 
-    const int32_t *row = a.table + (long long)b * a.table_stride;
-    const int edge = fdiv(a.shared, a.size);  // the page in which the shared part ends, if inside
-    const int edge_page = a.shared > edge * a.g.size && a.from < a.shared ? a.prefix[edge] : -1;
+    if (warp == 4) {
+        // ---- copies; each lane one box of a tile
+        const int boxes = kStKeys / a.box_rows;
+        for (int u = blockIdx.x / ranks; u < a.units; u += gridDim.x / ranks) {
+            const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk;
+            int len, lo, hi;
+            tiles_of(b, len, lo, hi);
+            const int32_t *row = a.table + (long long)b * a.table_stride;
+            auto page_of = [&](int tile) {
+                const int place = tile * kStKeys + lane * a.box_rows;
+                // outside the stream's places, or no page of the cache: one that does not exist, read as zeros
+                const int page = lane < boxes && place < len && place + a.box_rows > a.from ? row[fdiv(place, a.size)] : a.pages;
+                return page < 0 || page > a.pages ? a.pages : page;
+            };
+            int next = lo < hi ? page_of(lo) : 0;
+            for (int tile = lo; tile < hi && ok; tile++, ring++) {
+                const int page = next, st = ring % a.stages, round = ring / a.stages;
+                if (tile + 1 < hi) next = page_of(tile + 1);
+                int go = 1;
+                if (lane == 0) {
+                    go = !*abort && (!round || wait(&sh.empty[st], (round - 1) & 1, 1));
+                    if (go) mbar_expect_tx(&sh.full[st], Sm::kStage);
+                }
+                ok = __shfl_sync(0xffffffffu, go, 0);
+                if (ok && lane < boxes) {
+                    const int place = tile * kStKeys + lane * a.box_rows, at = place - fdiv(place, a.size) * a.page_size;
+                    char *dst = smem + st * Sm::kStage + lane * a.box_rows * 128;
+#pragma unroll
+                    for (int i = 0; i < DK / 64; i++) {
+                        tma_load_4d(dst + i * Sm::kBlock, &tm_k, &sh.full[st], i * 64, kvh, at, page);
+                        tma_load_4d(dst + Sm::kTile + i * Sm::kBlock, &tm_v, &sh.full[st], i * 64, kvh, at, page);
+                    }
+                }
+            }
+            if (ranks > 1) {
+                cluster.sync();
+                cluster.sync();
+            }
+        }
+        // nothing may still be written to this block's memory when it ends
+        if (!ok && lane == 0)
+            for (int i = max(ring - a.stages, 0); i < ring; i++) mbar_wait(&sh.full[i % a.stages], (i / a.stages) & 1);
+        __syncwarp();
+        return;
+    }
+
+    // ---- products
     const float sl = a.scale_log2;
-    // as many places at a time as the list of page numbers covers
-    const int most = (kStList - 1) * a.g.size / kStKeys * kStKeys;
-    for (int s0 = lo; s0 < hi; s0 += most) {
-        const int s1 = min(hi, s0 + most), page0 = fdiv(s0, a.size), pages = fdiv(s1 - 1, a.size) + 1 - page0;
-        __syncthreads();
-        // pages of shared places alone come from the prefix; a table row is
-        // only there if places behind the shared ones are wanted
-        for (int i = tid; i < pages; i += kStThreads)
-            list[i] = page0 + i < edge && a.from < a.shared ? a.prefix[page0 + i] : s1 > a.shared ? row[page0 + i] : -1;
-        __syncthreads();
-        const int n = (s1 - s0 + kStKeys - 1) / kStKeys;
-        auto load = [&](int tile) {
-            char *dst = smem + (tile % kStStages) * 2 * Sm::kTile;
-            const int c = tid % kChunks;
+    bool first_unit = true;
+    for (int u = blockIdx.x / ranks; u < a.units; u += gridDim.x / ranks) {
+        const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk, row0 = u % a.zs * 16, heads = min(a.group - row0, 16);
+        int len, lo, hi;
+        tiles_of(b, len, lo, hi);
+        // the group's queries, padded to 16 rows, as the A operand
+        uint32_t qa[DK / 16][4];
+        {
+            const int r = lane >> 2, c = (lane & 3) * 2;
 #pragma unroll
-            for (int r = tid / kChunks; r < kStKeys; r += kStThreads / kChunks) {
-                const int place = s0 + tile * kStKeys + r;
-                bool real = place < s1 && c * 8 < a.d;
-                long long at = 0;
-                if (real) {
-                    const int i = fdiv(place, a.size);
-                    const int page = i == edge && place < a.shared && a.from < a.shared ? edge_page : list[i - page0];
-                    real = page >= 0 && page < a.g.pages;
-                    if (real) at = page * a.g.ps + (place - i * a.g.size) * a.g.ts + kvh * a.g.hs + c * 8;
+            for (int k = 0; k < DK / 16; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int row = r + (i & 1) * 8, col = k * 16 + c + (i >> 1) * 8;
+                    uint32_t x = 0;
+                    if (row < heads && col < a.d) {  // d is even
+                        const T *p = a.q.at(b, kvh * a.group + row0 + row) + col;
+                        x = a.q_pairs ? *(const uint32_t *)p
+                                      : (uint32_t)*(const unsigned short *)p | (uint32_t)*(const unsigned short *)(p + 1) << 16;
+                    }
+                    qa[k][i] = x;
                 }
-                const uint32_t to = smem_u32(dst) + r * DK * 2 + ((c ^ (r & 7)) << 4);
-                cp_async16(to, a.k + at, real);
-                cp_async16(to + Sm::kTile, a.v + at, real);
-            }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < kStStages - 1; i++) {
-            if (i < n) load(i);
-            else cp_async_commit();
         }
-        for (int tile = 0; tile < n; tile++) {
-            cp_async_wait<kStStages - 2>();
-            __syncthreads();
-            if (tile + kStStages - 1 < n) load(tile + kStStages - 1);
-            else cp_async_commit();
-            const uint32_t kt = smem_u32(smem + (tile % kStStages) * 2 * Sm::kTile), vt = kt + Sm::kTile;
-            const int key0 = warp * 16;
-            float s[2][4] = {};
+        float o[DK / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
-            for (int k = 0; k < DK / 16; k++) {
-                uint32_t kb[4];
-                const int r = key0 + (lane & 7) + (lane >> 4) * 8, c = k * 2 + (lane >> 3 & 1);
-                ldmatrix4(kt + r * DK * 2 + ((c ^ (r & 7)) << 4), kb);
-                mma16816<T>(s[0], qa[k], kb[0], kb[1]);
-                mma16816<T>(s[1], qa[k], kb[2], kb[3]);
-            }
-            // places behind the last one carry no weight
-            const int here = s1 - (s0 + tile * kStKeys + key0);
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (i * 8 + (lane & 3) * 2 + (j & 1) >= here) s[i][j] = -INFINITY;
-            uint32_t p[4];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {  // rows lane / 4 and lane / 4 + 8
-                float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                top = fmaxf(top, m[h]);
-                const float f = top == m[h] ? 1.f : ex2((m[h] - top) * sl);
-                m[h] = top;
-                const float off = top == -INFINITY ? 0.f : -top * sl;
-                float e[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) e[i] = ex2(fmaf(s[i >> 1][2 * h + (i & 1)], sl, off));
-                l[h] = fmaf(l[h], f, (e[0] + e[1]) + (e[2] + e[3]));
-                p[h] = pack2<T>(e[0], e[1]);
-                p[h + 2] = pack2<T>(e[2], e[3]);
-#pragma unroll
-                for (int i = 0; i < DK / 8; i++) {
-                    o[i][2 * h] *= f;
-                    o[i][2 * h + 1] *= f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < DK / 16; i++) {
-                uint32_t vb[4];
-                const int r = key0 + (lane & 7) + (lane >> 3 & 1) * 8, c = i * 2 + (lane >> 4);
-                ldmatrix4_t(vt + r * DK * 2 + ((c ^ (r & 7)) << 4), vb);
-                mma16816<T>(o[2 * i], p, vb[0], vb[1]);
-                mma16816<T>(o[2 * i + 1], p, vb[2], vb[3]);
-            }
-        }
-        cp_async_wait<0>();
-    }
+        for (int i = 0; i < DK / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-    // ---- the four warps' results become the block's, in log2 units
-    __syncthreads();
-    {
-        float *wo = (float *)(smem + warp * Sm::kO);
-        const int r = lane >> 2, c = (lane & 3) * 2;
+        for (int tile = lo; tile < hi; tile++, ring++) {
+            const int st = ring % a.stages;
+            ok = ok && __all_sync(0xffffffffu, wait(&sh.full[st], (ring / a.stages) & 1, 2));
+            if (!ok) continue;
+            const uint32_t kt = smem_u32(smem + st * Sm::kStage), vt = kt + Sm::kTile;
+            const int key0 = warp * 16, place0 = tile * kStKeys + key0;
+            const int skip = a.from - place0, here = len - place0;  // of this warp's 16 places: skip .. here - 1 count
+            if (skip < 16 && here > 0) {
+                const bool edge = skip > 0 || here < 16;
+                if (edge) {
+                    // values of other places may be anything, and 0 times them NaN: zeros
+                    for (int i = lane; i < 16 * 8; i += 32)
+                        if (i / 8 < skip || i / 8 >= here)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-            l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-            if ((lane & 3) == 0) {
-                warp_m[warp][r + 8 * h] = m[h] * sl;
-                warp_l[warp][r + 8 * h] = l[h];
+                            for (int k = 0; k < DK / 64; k++)
+                                *(uint4 *)(smem + st * Sm::kStage + Sm::kTile + k * Sm::kBlock + (key0 * 8 + i) * 16) =
+                                    make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+                float s[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < DK / 16; k++) {
+                    uint32_t kb[4];
+                    const int r = key0 + (lane & 7) + (lane >> 4) * 8, c = (k & 3) * 2 + (lane >> 3 & 1);
+                    ldmatrix4(kt + (k >> 2) * Sm::kBlock + r * 128 + ((c ^ (r & 7)) << 4), kb);
+                    mma16816<T>(s[0], qa[k], kb[0], kb[1]);
+                    mma16816<T>(s[1], qa[k], kb[2], kb[3]);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const int key = i * 8 + (lane & 3) * 2 + (j & 1);
+                            if (key < skip || key >= here) s[i][j] = -INFINITY;
+                        }
+                }
+                uint32_t p[4];
+                float top[2];
+                bool grow = false;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {  // rows lane / 4 and lane / 4 + 8
+                    float x = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+                    top[h] = fmaxf(x, m[h]);
+                    grow |= (top[h] - m[h]) * sl > 8.f;  // as in attn_tc_kernel: smaller steps leave m
+                }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float f = top[h] == m[h] ? 1.f : ex2((m[h] - top[h]) * sl);
+                        m[h] = top[h];
+                        l[h] *= f;
+#pragma unroll
+                        for (int i = 0; i < DK / 8; i++) {
+                            o[i][2 * h] *= f;
+                            o[i][2 * h + 1] *= f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const float off = m[h] == -INFINITY ? 0.f : -m[h] * sl;
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) e[i] = ex2(fmaf(s[i >> 1][2 * h + (i & 1)], sl, off));
+                    l[h] += (e[0] + e[1]) + (e[2] + e[3]);
+                    p[h] = pack2<T>(e[0], e[1]);
+                    p[h + 2] = pack2<T>(e[2], e[3]);
+                }
+#pragma unroll
+                for (int i = 0; i < DK / 16; i++) {
+                    uint32_t vb[4];
+                    const int r = key0 + (lane & 7) + (lane >> 3 & 1) * 8, c = (i & 3) * 2 + (lane >> 4);
+                    ldmatrix4_t(vt + (i >> 2) * Sm::kBlock + r * 128 + ((c ^ (r & 7)) << 4), vb);
+                    mma16816<T>(o[2 * i], p, vb[0], vb[1]);
+                    mma16816<T>(o[2 * i + 1], p, vb[2], vb[3]);
+                }
+                if (edge) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the zeros before the next copy
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.empty[st]);
+        }
+
+        // ---- the four warps' results become the block's, in log2 units
+        step_sync();  // the last unit's are read
+        {
+            float *wo = result + warp * a.rows * DK;
+            const int r = lane >> 2, c = (lane & 3) * 2;
 #pragma unroll
-            for (int i = 0; i < DK / 8; i++)
-                *(float2 *)(wo + (r + 8 * h) * DK + i * 8 + c) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
-        }
-    }
-    __syncthreads();
-    for (int e = tid; e < heads * (DK / 4); e += kStThreads) {
-        const int r = e / (DK / 4), c = e % (DK / 4);
-        const float top = fmaxf(fmaxf(warp_m[0][r], warp_m[1][r]), fmaxf(warp_m[2][r], warp_m[3][r]));
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
+            for (int h = 0; h < 2; h++) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+                if (r + 8 * h < heads) {
+                    if ((lane & 3) == 0) {
+                        sh.warp_m[warp][r + 8 * h] = m[h] * sl;
+                        sh.warp_l[warp][r + 8 * h] = l[h];
+                    }
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
-            const float f = warp_m[w][r] == -INFINITY && warp_l[w][r] == 0.f ? 0.f : ex2(warp_m[w][r] - top);
-            add_scaled(x, f, ((const float4 *)(smem + w * Sm::kO))[r * (DK / 4) + c]);
-            sum = fmaf(f, warp_l[w][r], sum);
+                    for (int i = 0; i < DK / 8; i++)
+                        *(float2 *)(wo + (r + 8 * h) * DK + i * 8 + c) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+                }
+            }
         }
-        ((float4 *)block_o)[r * (DK / 4) + c] = x;
-        if (c == 0) {
-            block_m[r] = top;
-            block_l[r] = sum;
+        step_sync();
+        for (int e = tid; e < heads * (DK / 4); e += 128) {
+            const int r = e / (DK / 4);
+            const float top = fmaxf(fmaxf(sh.warp_m[0][r], sh.warp_m[1][r]), fmaxf(sh.warp_m[2][r], sh.warp_m[3][r]));
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float f = sh.warp_m[w][r] == -INFINITY && sh.warp_l[w][r] == 0.f ? 0.f : ex2(sh.warp_m[w][r] - top);
+                add_scaled(x, f, ((const float4 *)(result + w * a.rows * DK))[e]);
+                sum = fmaf(f, sh.warp_l[w][r], sum);
+            }
+            ((float4 *)result)[e] = x;
+            if (e % (DK / 4) == 0) {
+                sh.block_m[r] = top;
+                sh.block_l[r] = sum;
+            }
         }
-    }
-    // the shared part's launch may still run: its results from here on
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (ranks > 1) cluster.sync();
-    else __syncthreads();
-    // ---- a row's partial results: the cluster's blocks, then the shared
-    // part's pieces.  Their weights first, a warp per row.
-    const long long rows = (long long)a.batch * a.hq, prow0 = (long long)b * a.hq + kvh * a.group + row0;
-    const int parts = ranks + a.splits;
-    float *const weight = (float *)smem;  // [row][part], over the ring
-    for (int r = warp; r < heads; r += 4) {
-        float top = -INFINITY;
-        for (int i = lane; i < parts; i += 32) {
-            float w;
-            if (i < ranks) {
-                w = *cluster.map_shared_rank(&block_m[r], i);
-                if (w == -INFINITY && *cluster.map_shared_rank(&block_l[r], i) != 0.f) w = __int_as_float(0x7fffffff);
-            } else w = a.part_lse[(i - ranks) * rows + prow0 + r];
-            weight[r * parts + i] = w;
-            top = fmaxf(top, w);
+        // the shared part's launch may still run: its results from here on
+        if (first_unit) asm volatile("griddepcontrol.wait;" ::: "memory");
+        first_unit = false;
+        if (ranks > 1) cluster.sync();
+        else step_sync();
+        // ---- a row's partial results: the cluster's blocks, then the shared
+        // part's pieces.  Their weights first, a warp per row.
+        const long long rows = (long long)a.batch * a.hq, prow0 = (long long)b * a.hq + kvh * a.group + row0;
+        const int parts = ranks + a.splits;
+        for (int r = warp; r < heads; r += 4) {
+            float top = -INFINITY;
+            for (int i = lane; i < parts; i += 32) {
+                float w;
+                if (i < ranks) {
+                    w = *cluster.map_shared_rank(&sh.block_m[r], i);
+                    if (w == -INFINITY && *cluster.map_shared_rank(&sh.block_l[r], i) != 0.f) w = __int_as_float(0x7fffffff);
+                } else w = a.part_lse[(i - ranks) * rows + prow0 + r];
+                weight[r * parts + i] = w;
+                top = fmaxf(top, w);
+            }
+            top = warp_max(top);
+            float sum = 0.f;
+            for (int i = lane; i < parts; i += 32) {
+                // nothing seen: no weight
+                const float w = weight[r * parts + i], f = w == -INFINITY ? 0.f : ex2(w - top);
+                weight[r * parts + i] = f;
+                sum += i < ranks ? f * *cluster.map_shared_rank(&sh.block_l[r], i) : f;
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) sh.inv[r] = 1.f / sum;
         }
-        top = warp_max(top);
-        float sum = 0.f;
-        for (int i = lane; i < parts; i += 32) {
-            // nothing seen: no weight
-            const float w = weight[r * parts + i], f = w == -INFINITY ? 0.f : ex2(w - top);
-            weight[r * parts + i] = f;
-            sum += i < ranks ? f * *cluster.map_shared_rank(&block_l[r], i) : f;
-        }
-        sum = warp_sum(sum);
-        if (lane == 0) warp_l[0][r] = len > 0 ? 1.f / sum : 0.f;
-    }
-    __syncthreads();
-    // the cluster's blocks take turns at the elements
-    const int quads = a.d / 4;
-    for (int e = rank * kStThreads + tid; e < heads * quads; e += ranks * kStThreads) {
-        const int r = e / quads, c = e % quads;
-        const float *w = weight + r * parts;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < ranks; i++) add_scaled(x, w[i], ((const float4 *)cluster.map_shared_rank(block_o, i))[r * (DK / 4) + c]);
-        const float4 *o = (const float4 *)(a.part_o + (prow0 + r) * a.d) + c;
+        step_sync();
+        // the cluster's blocks take turns at the elements
+        const int quads = a.d / 4;
+        for (int e = rank * 128 + tid; e < heads * quads; e += ranks * 128) {
+            const int r = e / quads, c = e % quads;
+            const float *w = weight + r * parts;
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < ranks; i++) add_scaled(x, w[i], ((const float4 *)cluster.map_shared_rank(result, i))[r * (DK / 4) + c]);
+            const float4 *po = (const float4 *)(a.part_o + (prow0 + r) * a.d) + c;
 #pragma unroll 8
-        for (int i = 0; i < a.splits; i++) add_scaled(x, w[ranks + i], o[i * rows * quads]);
-        const float f = warp_l[0][r];
-        T *dst = a.o.at(b, kvh * a.group + row0 + r) + 4 * c;
-        dst[0] = from_f32<T>(len > 0 ? x.x * f : 0.f);
-        dst[1] = from_f32<T>(len > 0 ? x.y * f : 0.f);
-        dst[2] = from_f32<T>(len > 0 ? x.z * f : 0.f);
-        dst[3] = from_f32<T>(len > 0 ? x.w * f : 0.f);
+            for (int i = 0; i < a.splits; i++) add_scaled(x, w[ranks + i], po[i * rows * quads]);
+            const float f = sh.inv[r];
+            T *dst = a.o.at(b, kvh * a.group + row0 + r) + 4 * c;
+            dst[0] = from_f32<T>(len > 0 ? x.x * f : 0.f);
+            dst[1] = from_f32<T>(len > 0 ? x.y * f : 0.f);
+            dst[2] = from_f32<T>(len > 0 ? x.z * f : 0.f);
+            dst[3] = from_f32<T>(len > 0 ? x.w * f : 0.f);
+        }
+        if (ranks > 1) cluster.sync();  // a block's results stay until the others have read them
     }
-    if (ranks > 1) cluster.sync();  // a block's results stay until the others have read them
 }
 
-// Largest number of blocks that share one stream's places.
-constexpr int kStMostPieces = 8;
-
 template <typename T, int DK>
-static cudaError_t step_launch(const StepArgs<T> &a, int pieces, bool behind_shared, cudaStream_t s)
+static cudaError_t step_launch(const CUtensorMap &k, const CUtensorMap &v, StepArgs<T> a, int pieces, bool behind_shared,
+                               cudaStream_t s)
 {
     auto *fn = &prefix_step_kernel<T, DK>;
-    cudaError_t e = ensure_smem_attr((const void *)fn, StepSmem<DK>::kBytes);
+    // the deepest ring with which two blocks fit an SM
+    const int parts = pieces + a.splits;
+    a.stages = kStMostStages;
+    while (a.stages > 2 && StepSmem<DK>::bytes(a.stages, a.rows, parts) + sizeof(StepShared) + 1024 > 228 * 1024 / 2) a.stages--;
+    cudaError_t e = ensure_smem_attr((const void *)fn, StepSmem<DK>::bytes(kStMostStages, 16, kStMostPieces + kAtMostSplits));
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.batch * pieces), (unsigned)a.hk, (unsigned)((a.group + 15) / 16));
+    cfg.gridDim = dim3((unsigned)(std::min(a.units, std::max(1, 2 * tc_sm_count() / pieces)) * pieces));
     cfg.blockDim = dim3(kStThreads);
-    cfg.dynamicSmemBytes = StepSmem<DK>::kBytes;
+    cfg.dynamicSmemBytes = StepSmem<DK>::bytes(a.stages, a.rows, parts);
     cfg.stream = s;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -350,7 +416,7 @@ static cudaError_t step_launch(const StepArgs<T> &a, int pieces, bool behind_sha
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
     cfg.numAttrs = behind_shared ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, fn, a);
+    return cudaLaunchKernelEx(&cfg, fn, k, v, a);
 }
 
 }  // namespace aie

@@ -153,3 +153,20 @@ def last_error() -> str:
 def check(status: int, where: str):
     if status != AIE_OK:
         raise AieError(status, where, last_error())
+
+
+_SEQCALL = None
+
+
+def seqcall():
+    """The sequence operators' binding on torch tensors (csrc/seq_bind.cpp)."""
+    global _SEQCALL
+    if _SEQCALL is None:
+        import torch  # noqa: F401  (the binding links against its libraries)
+        load()
+        try:
+            from . import _seqcall
+        except ImportError as e:
+            raise ImportError(f"{e}: build it with `python -m ai_engine_b200.build`") from e
+        _SEQCALL = _seqcall
+    return _SEQCALL

@@ -2,7 +2,9 @@
 
 Two translation units, compiled for sm_100a only and side by side: the conv
 path (``csrc/aie_conv.cu``, which includes the ``k_*.cuh`` kernels) and the
-sequence operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels).  The CUDA runtime is linked statically, so the
+sequence operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels).  Beside
+it ``_seqcall.so``, the sequence operators' binding on torch tensors
+(``csrc/seq_bind.cpp``), which is linked against it.  The CUDA runtime is linked statically, so the
 library depends on nothing but the driver; the tensor-map encoder is fetched
 from the driver at run time.
 """
@@ -20,6 +22,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaie_conv.so")
 UNITS = ("aie_conv", "aie_seq")
 OBJ = os.path.join(HERE, "_build")
+BIND = os.path.join(HERE, "_seqcall.so")
+BIND_SRC = os.path.join(CSRC, "seq_bind.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -53,7 +57,24 @@ def _older(path, files) -> bool:
 
 
 def stale() -> bool:
-    return _older(LIB, sources())
+    return _older(LIB, sources()) or _older(BIND, _bind_sources())
+
+
+def _bind_sources():
+    return [BIND_SRC, *(os.path.join(ROOT, "include", h) for h in ("aie_conv.h", "aie_seq.h"))]
+
+
+def _bind_command(out: str):
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    inc = [f for d in (sysconfig.get_paths()["include"], *cpp_extension.include_paths("cuda")) for f in ("-isystem", d)]
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, BIND_SRC, "-o", out,
+            "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-L", HERE, "-l:libaie_conv.so",
+            "-Wl,-rpath,$ORIGIN"]
 
 
 def build(force: bool = False, verbose: bool = False, extra=()) -> str:
@@ -75,8 +96,12 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> str:
     for _, cmd, p in jobs:
         if p.returncode:
             raise subprocess.CalledProcessError(p.returncode, cmd)
-    subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", *objs, "-o", LIB + tmp], check=True)
-    os.replace(LIB + tmp, LIB)
+    if jobs or _older(LIB, objs):
+        subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", *objs, "-o", LIB + tmp], check=True)
+        os.replace(LIB + tmp, LIB)
+    if force or _older(BIND, _bind_sources()):
+        subprocess.run(_bind_command(BIND + tmp), check=True)
+        os.replace(BIND + tmp, BIND)
     return LIB
 
 

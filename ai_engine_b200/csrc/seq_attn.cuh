@@ -145,15 +145,6 @@ __device__ __forceinline__ float max3(float a, float b, float c)
     return y;
 }
 
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi)
-{
-    uint32_t y;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-    return y;
-}
-
 // ------------------------------------------------------------- kernel ---
 
 struct AttnArgs {

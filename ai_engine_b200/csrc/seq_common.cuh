@@ -20,6 +20,16 @@ __device__ __forceinline__ T from_f32(float x)
     else return x;
 }
 
+// Two values rounded to a pair of 16-bit ones.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    uint32_t y;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+
 // [tokens][heads][dim] of type T (aie_heads)
 template <typename T>
 struct HeadsOf {

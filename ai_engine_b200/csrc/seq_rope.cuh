@@ -107,7 +107,10 @@ __device__ __forceinline__ Vec8<T> load8(const T *p)
 {
     Vec8<T> v;
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; i++) v.u[i] = ((const uint4 *)p)[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; i++)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.u[i].x), "=r"(v.u[i].y), "=r"(v.u[i].z), "=r"(v.u[i].w)
+                     : "l"((const uint4 *)p + i));
     return v;
 }
 
@@ -121,18 +124,36 @@ __device__ __forceinline__ void store8(T *p, const Vec8<T> &v)
 template <typename T>
 __device__ __forceinline__ void unpack8(const Vec8<T> &v, float *f)
 {
-    const T *e = (const T *)&v;
+    const uint32_t *u = (const uint32_t *)&v;
 #pragma unroll
-    for (int i = 0; i < 8; i++) f[i] = to_f32(e[i]);
+    for (int i = 0; i < 4; i++) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // a bf16 is the upper half of an f32
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 y = __half22float2(*(const __half2 *)&u[i]);
+            f[2 * i] = y.x;
+            f[2 * i + 1] = y.y;
+        } else {
+            f[2 * i] = __uint_as_float(u[2 * i]);
+            f[2 * i + 1] = __uint_as_float(u[2 * i + 1]);
+        }
+    }
 }
 
 template <typename T>
 __device__ __forceinline__ Vec8<T> pack8(const float *f)
 {
     Vec8<T> v;
-    T *e = (T *)&v;
+    uint32_t *u = (uint32_t *)&v;
 #pragma unroll
-    for (int i = 0; i < 8; i++) e[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 2) u[i] = pack2<T>(f[2 * i], f[2 * i + 1]);
+        else {
+            u[2 * i] = __float_as_uint(f[2 * i]);
+            u[2 * i + 1] = __float_as_uint(f[2 * i + 1]);
+        }
+    }
     return v;
 }
 
@@ -149,131 +170,160 @@ __device__ __forceinline__ void load8f(const float *p, float *f)
 // halves, elements i and i + rot / 2; interleaved or not rotated, neighbours.
 // A lane keeps its pieces' weights and its token's angles in registers for
 // HPT heads of the token, whose loads are all in flight at once.
+//
+// Bound by memory: 16384 tokens of 32 + 8 heads of 128 with keys and values
+// filed take 86 us, 444 MB at 5.2 TB/s.  Measured there: 5 blocks an SM (96
+// registers) 86 us, 4 89, 6 (80 registers, some spilled) 93; 2 heads a lane
+// 101; blocks of 256 threads 99.
+constexpr int kRopeThreads = 128, kRopeBlocks = 5;
 struct RopeVec {
-    int units_per_token, q_units, k_units;  // groups of HPT heads of q, k, v
-    unsigned units;
-    int slots32;  // the cache's places fit 32 bits
+    unsigned q_units, k_units;  // groups of HPT heads of a token
+    unsigned q_end, k_end, end; // units: all of q, then of k, then of v
+    int slots32;                // the cache's places fit 32 bits
+    float inv_d;
 };
 
 template <typename T, int LPR, int HPT, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) rope_vec_kernel(const RopeArgs<T> a, const RopeVec g)
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(const RopeArgs<T> a, const RopeVec g)
 {
-    const unsigned unit = (unsigned)(((unsigned long long)blockIdx.x * blockDim.x + threadIdx.x) / LPR);
+    unsigned unit = (unsigned)(((unsigned long long)blockIdx.x * blockDim.x + threadIdx.x) / LPR);
     const int lane = threadIdx.x % LPR;
-    if (unit >= g.units) return;  // whole groups of LPR lanes
+    if (unit >= g.end) return;  // whole groups of LPR lanes
     const unsigned mask = LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (threadIdx.x % 32 / LPR * LPR);
-    const int t = (int)(unit / (unsigned)g.units_per_token);
-    int u = (int)(unit - (unsigned)t * g.units_per_token);
-    const int kind = u < g.q_units ? 0 : u < g.q_units + g.k_units ? 1 : 2;
-    u -= kind == 0 ? 0 : kind == 1 ? g.q_units : g.q_units + g.k_units;
-    const int heads = kind == 0 ? a.hq : a.hk, h0 = u * HPT;
+    // q, k and v one after the other: few warps hold more than one of them
+    const bool key = unit >= g.q_end, value = unit >= g.k_end;
+    unit -= value ? g.k_end : key ? g.q_end : 0;
+    const unsigned per = key ? g.k_units : g.q_units;
+    const int t = (int)(unit / per), h0 = (int)(unit - (unsigned)t * per) * HPT;
+    const int n = min(HPT, (key ? a.hk : a.hq) - h0);
     const bool on = lane * 16 < a.d;
-    // the lane's pieces
+    // the lane's pieces: elements e0 and e0 + gap on
     const int half = a.rot >> 1;
-    const bool turn = kind < 2 && lane * 16 < a.rot;
-    const int e0 = !INTERLEAVED && turn ? lane * 8 : lane * 16, e1 = !INTERLEAVED && turn ? e0 + half : e0 + 8;
+    const bool turn = !value && lane * 16 < a.rot;
+    const int e0 = !INTERLEAVED && turn ? lane * 8 : lane * 16, gap = !INTERLEAVED && turn ? half : 8;
 
-    const HeadsOf<T> &src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
+    const HeadsOf<T> &src = value ? a.v : key ? a.k : a.q;
     Vec8<T> x[HPT][2];
-#pragma unroll
-    for (int i = 0; i < HPT; i++)
-        if (on && h0 + i < heads) {
-            const T *p = src.at(t, h0 + i);
-            x[i][0] = load8(p + e0);
-            x[i][1] = load8(p + e1);
-        }
-    // the token's place in the cache
-    T *pages = kind == 0 ? nullptr : kind == 1 ? a.kp : a.vp;
-    if (pages) {
-        const long long s = a.slots[t];
-        if (s < 0 || s >= (long long)a.pg.pages * a.pg.size) pages = nullptr;
-        else if (g.slots32) {
-            const unsigned page = (unsigned)s / (unsigned)a.pg.size;
-            pages += page * a.pg.ps + ((unsigned)s - page * (unsigned)a.pg.size) * a.pg.ts;
-        } else pages += s / a.pg.size * a.pg.ps + s % a.pg.size * a.pg.ts;
-    }
-    if (kind == 2) {
+    if (on) {
+        const T *p = src.at(t, h0) + e0;
 #pragma unroll
         for (int i = 0; i < HPT; i++)
-            if (on && pages && h0 + i < heads) {
-                T *p = pages + (h0 + i) * a.pg.hs;
-                store8(p + e0, x[i][0]);
-                store8(p + e1, x[i][1]);
+            if (i < n) {
+                x[i][0] = load8(p);
+                x[i][1] = load8(p + gap);
+                p += src.hs;
+            }
+    }
+    // the token's place in the cache
+    T *page = !key ? nullptr : value ? a.vp : a.kp;
+    if (page) {
+        const long long s = a.slots[t];
+        if (s < 0 || s >= (long long)a.pg.pages * a.pg.size) page = nullptr;
+        else {
+            if (g.slots32) {
+                const unsigned number = (unsigned)s / (unsigned)a.pg.size;
+                page += number * a.pg.ps + ((unsigned)s - number * (unsigned)a.pg.size) * a.pg.ts;
+            } else page += s / a.pg.size * a.pg.ps + s % a.pg.size * a.pg.ts;
+            page += h0 * a.pg.hs + e0;
+        }
+    }
+    if (value) {
+#pragma unroll
+        for (int i = 0; i < HPT; i++)
+            if (on && page && i < n) {
+                store8(page, x[i][0]);
+                store8(page + gap, x[i][1]);
+                page += a.pg.hs;
             }
         return;
     }
-    float c[8], sn[8], w0[8], w1[8];
-    if (on && turn) {
-        const int pos = a.pos[t];
-        if (pos >= 0 && pos < a.max_pos) {
-            // angles: e0 .. e0 + 7 of the halves, or of the eight neighbouring pairs
-            const float *cs = a.cs + (long long)pos * a.rot + lane * 8;
-            load8f(cs, c);
-            load8f(cs + half, sn);
-        } else {
+    // y0 = r (x0 a0 + x1 b0), y1 = r (x1 a1 + x0 b1): weight and angle in one
+    // factor, the same for all heads of the token.  Two elements to a register pair.
+    const float *w = key ? a.wk : a.wq;
+    float2 a0[4], a1[4], b0[4], b1[4];
+    if (on) {
+        float c[8], sn[8], w0[8], w1[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) c[i] = sn[i] = __int_as_float(0x7fffffff);
+        for (int k = 0; k < 8; k++) {
+            c[k] = w0[k] = w1[k] = 1.f;
+            sn[k] = 0.f;
         }
-    }
-    const float *w = kind == 0 ? a.wq : a.wk;
-    if (on && w) {
-        load8f(w + e0, w0);
-        load8f(w + e1, w1);
-    }
-    const HeadsOf<T> &dst = kind == 0 ? a.qo : a.ko;
-#pragma unroll
-    for (int i = 0; i < HPT; i++) {
-        if (h0 + i >= heads) break;
-        float f0[8], f1[8];
-        float sum = 0.f;
-        if (on) {
-            unpack8(x[i][0], f0);
-            unpack8(x[i][1], f1);
-#pragma unroll
-            for (int k = 0; k < 8; k++) sum = fmaf(f0[k], f0[k], fmaf(f1[k], f1[k], sum));
-        }
-        if (w) {
-#pragma unroll
-            for (int o = LPR / 2; o; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-            if (on) {
-                const float r = 1.0f / sqrtf(sum / (float)a.d + a.eps);
-#pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    f0[k] = f0[k] * r * w0[k];
-                    f1[k] = f1[k] * r * w1[k];
-                }
-            }
-        }
-        if (!on) continue;
         if (turn) {
-            if constexpr (INTERLEAVED) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float p = f0[2 * k], q = f0[2 * k + 1], v = f1[2 * k], z = f1[2 * k + 1];
-                    f0[2 * k] = p * c[k] - q * sn[k];
-                    f0[2 * k + 1] = q * c[k] + p * sn[k];
-                    f1[2 * k] = v * c[k + 4] - z * sn[k + 4];
-                    f1[2 * k + 1] = z * c[k + 4] + v * sn[k + 4];
-                }
+            const int pos = a.pos[t];
+            if (pos >= 0 && pos < a.max_pos) {
+                // angles: e0 .. e0 + 7 of the halves, or of the eight neighbouring pairs
+                const float *cs = a.cs + (long long)pos * a.rot + lane * 8;
+                load8f(cs, c);
+                load8f(cs + half, sn);
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
-                    const float p = f0[k], q = f1[k];
-                    f0[k] = p * c[k] - q * sn[k];
-                    f1[k] = q * c[k] + p * sn[k];
-                }
+                for (int k = 0; k < 8; k++) c[k] = sn[k] = __int_as_float(0x7fffffff);
             }
         }
-        const Vec8<T> y0 = pack8<T>(f0), y1 = pack8<T>(f1);
-        if (dst.p) {
-            T *p = dst.at(t, h0 + i);
-            store8(p + e0, y0);
-            store8(p + e1, y1);
+        if (w) {
+            load8f(w + e0, w0);
+            load8f(w + e0 + gap, w1);
         }
-        if (pages) {
-            T *p = pages + (h0 + i) * a.pg.hs;
-            store8(p + e0, y0);
-            store8(p + e1, y1);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int i = 2 * k, j = i + 1;
+            if (INTERLEAVED && turn) {  // pairs (i, j) of either piece; b goes with the pair swapped
+                a0[k] = make_float2(w0[i] * c[k], w0[j] * c[k]);
+                b0[k] = make_float2(-w0[j] * sn[k], w0[i] * sn[k]);
+                a1[k] = make_float2(w1[i] * c[k + 4], w1[j] * c[k + 4]);
+                b1[k] = make_float2(-w1[j] * sn[k + 4], w1[i] * sn[k + 4]);
+            } else {
+                a0[k] = make_float2(w0[i] * c[i], w0[j] * c[j]);
+                b0[k] = make_float2(-w1[i] * sn[i], -w1[j] * sn[j]);
+                a1[k] = make_float2(w1[i] * c[i], w1[j] * c[j]);
+                b1[k] = make_float2(w0[i] * sn[i], w0[j] * sn[j]);
+            }
+        }
+    }
+    const HeadsOf<T> &dst = key ? a.ko : a.qo;
+    T *out = dst.p ? dst.at(t, h0) + e0 : nullptr;
+#pragma unroll
+    for (int i = 0; i < HPT; i++) {
+        if (i >= n) break;
+        float2 f0[4], f1[4];
+        float r = 1.f;
+        if (on) {
+            unpack8(x[i][0], (float *)f0);
+            unpack8(x[i][1], (float *)f1);
+        }
+        if (w) {
+            float2 sum = make_float2(0.f, 0.f);
+            if (on)
+#pragma unroll
+                for (int k = 0; k < 4; k++) sum = __ffma2_rn(f0[k], f0[k], __ffma2_rn(f1[k], f1[k], sum));
+            float total = sum.x + sum.y;
+#pragma unroll
+            for (int o = LPR / 2; o; o >>= 1) total += __shfl_xor_sync(mask, total, o);
+            r = rsqrtf(fmaf(total, g.inv_d, a.eps));
+        }
+        if (!on) continue;
+        const float2 r2 = make_float2(r, r);
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 p = f0[k], q = f1[k];
+            float2 y0 = __fmul2_rn(p, a0[k]), y1 = __fmul2_rn(q, a1[k]);
+            if (turn) {
+                y0 = __ffma2_rn(INTERLEAVED ? make_float2(p.y, p.x) : q, b0[k], y0);
+                y1 = __ffma2_rn(INTERLEAVED ? make_float2(q.y, q.x) : p, b1[k], y1);
+            }
+            f0[k] = __fmul2_rn(y0, r2);
+            f1[k] = __fmul2_rn(y1, r2);
+        }
+        const Vec8<T> y0 = pack8<T>((const float *)f0), y1 = pack8<T>((const float *)f1);
+        if (out) {
+            store8(out, y0);
+            store8(out + gap, y1);
+            out += dst.hs;
+        }
+        if (page) {
+            store8(page, y0);
+            store8(page + gap, y1);
+            page += a.pg.hs;
         }
     }
 }
@@ -292,23 +342,28 @@ template <typename T, int LPR, int HPT>
 static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
 {
     RopeVec g;
-    g.q_units = (a.hq + HPT - 1) / HPT;
-    g.k_units = (a.hk + HPT - 1) / HPT;
-    g.units_per_token = g.q_units + g.k_units * (a.vp ? 2 : 1);
-    g.units = (unsigned)a.tokens * g.units_per_token;  // under 2^32: rope_vec_ok
+    g.q_units = (unsigned)(a.hq + HPT - 1) / HPT;
+    g.k_units = (unsigned)(a.hk + HPT - 1) / HPT;
+    g.q_end = a.tokens * g.q_units;  // all under 2^32: rope_vec_ok
+    g.k_end = g.q_end + a.tokens * g.k_units;
+    g.end = g.k_end + (a.vp ? a.tokens * g.k_units : 0);
     g.slots32 = (unsigned long long)a.pg.pages * a.pg.size <= 0xffffffffull;
-    const unsigned grid = (unsigned)(((unsigned long long)g.units * LPR + 255) / 256);
-    if (a.interleaved) rope_vec_kernel<T, LPR, HPT, true><<<grid, 256, 0, s>>>(a, g);
-    else rope_vec_kernel<T, LPR, HPT, false><<<grid, 256, 0, s>>>(a, g);
+    g.inv_d = 1.0f / (float)a.d;
+    const unsigned grid = (unsigned)(((unsigned long long)g.end * LPR + kRopeThreads - 1) / kRopeThreads);
+    if (a.interleaved) rope_vec_kernel<T, LPR, HPT, true><<<grid, kRopeThreads, 0, s>>>(a, g);
+    else rope_vec_kernel<T, LPR, HPT, false><<<grid, kRopeThreads, 0, s>>>(a, g);
     return cudaGetLastError();
 }
 
-// Few heads: one at a time, over as many SMs as they reach.
+// So few heads that one at a time they are all resident at once: one at a time
+// (8 tokens of 24 heads of 64: 2.6 us against 3.8 us four at a time; 1237 tokens
+// of 25 heads of 96, beyond that: 5.6 us four at a time against 6.6 us).
 template <typename T, int LPR>
 static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
 {
     const long long threads = (long long)a.tokens * (a.hq + 2 * a.hk) * LPR;
-    return threads < 4ll * 2048 * tc_sm_count() ? rope_vec_launch<T, LPR, 1>(a, s) : rope_vec_launch<T, LPR, 4>(a, s);
+    return threads <= (long long)kRopeThreads * kRopeBlocks * tc_sm_count() ? rope_vec_launch<T, LPR, 1>(a, s)
+                                                                            : rope_vec_launch<T, LPR, 4>(a, s);
 }
 
 template <typename T>

@@ -170,7 +170,8 @@ static int prompt_tc(const aie_prompt &p, cudaStream_t s)
     a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
     a.causal = p.causal != 0;
-    a.vec_out = (uintptr_t)p.out.data % 16 == 0 && p.out.token_stride % 8 == 0 && p.out.head_stride % 8 == 0;
+    const uint64_t bits = (uintptr_t)p.out.data | 2 * p.out.token_stride | 2 * p.out.head_stride;
+    a.out_bytes = bits % 32 == 0 && p.head_dim % 16 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
     a.scale_log2 = p.scale * 1.4426950408889634f;
     const bool bf16 = p.dtype == AIE_DT_BF16;
     CUtensorMap q, k, v;
@@ -230,7 +231,7 @@ static int check_prefix(const aie_prefix *p)
 // blocks per stream and key head, or (0) row by row.
 struct PrefixPlan {
     int splits, tiles_per_split, row_pairs, pieces;
-    uint64_t part_o, bytes;  // the partial results' place in the workspace, and its size
+    uint64_t bytes;  // of the workspace
 };
 
 static PrefixPlan prefix_plan(const aie_prefix &p)
@@ -268,9 +269,15 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
         while (w.pieces < kStMostPieces && 2 * w.pieces * units <= 2ull * tc_sm_count() && w.pieces * 4 * kStKeys < places) w.pieces *= 2;
     }
     const uint64_t rows = (uint64_t)p.batch * p.q_heads;
-    w.part_o = (w.splits * rows * 4 + 15) / 16 * 16;
-    w.bytes = w.part_o + w.splits * rows * p.head_dim * 4 + 16;
+    w.bytes = w.splits * rows * (4 + 4 * (uint64_t)p.head_dim) + 64;
     return w;
+}
+
+// The partial results: their weights' sums at the front, then whole sectors.
+static float *part_o(const aie_prefix &p, const PrefixPlan &w)
+{
+    const uintptr_t at = (uintptr_t)p.workspace + (uint64_t)w.splits * p.batch * p.q_heads * 4;
+    return (float *)((at + 31) / 32 * 32);
 }
 
 extern "C" uint64_t aie_prefix_attn_workspace(const aie_prefix *p)
@@ -290,7 +297,7 @@ static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     AttnArgs a = {};
     a.prefix = p.prefix; a.lens = p.lens;
     a.part_lse = (float *)p.workspace;
-    a.part_o = (float *)((char *)p.workspace + w.part_o);
+    a.part_o = part_o(p, w);
     a.tokens = (int)p.batch;
     a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
@@ -326,7 +333,7 @@ static int prefix_rows(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.g = pages_geom(p.pages);
     a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
     a.part_lse = (const float *)p.workspace;
-    a.part_o = (const float *)((const char *)p.workspace + w.part_o);
+    a.part_o = part_o(p, w);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
     a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
     a.scale = p.scale;
@@ -344,7 +351,7 @@ static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.size = make_fastdiv((int)g.page_size);
     a.table = p.table; a.lens = p.lens;
     a.part_lse = (const float *)p.workspace;
-    a.part_o = (const float *)((const char *)p.workspace + w.part_o);
+    a.part_o = part_o(p, w);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.hk = (int)p.kv_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim;
     a.from = (int)p.prefix_len;

@@ -131,6 +131,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t *r)
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void store32(void *p, const uint32_t *v)
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
+                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+
 __device__ __forceinline__ float ex2(float x)
 {
     float y;
@@ -156,7 +163,8 @@ struct AttnArgs {
     float *part_o, *part_lse; // shared prefix: [split][row][d] and [split][row], row = stream * q_heads + head
     int tokens, seqs;         // prompts: packed tokens; shared prefix: streams
     int kv_heads, q_heads, group, d, tokens_per_tile;
-    int causal, vec_out;
+    int causal;
+    int out_bytes;            // what `out` is aligned to, in every row: 32, 16 or less
     int shared, max_len, page_size, pages, box_rows, splits, tiles_per_split;
     float scale_log2;
 };
@@ -384,38 +392,46 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const bool none = nt <= step0 || seen <= step0 * kAtTile;  // of this split's keys
             const float r = none ? 0.f : 1.f / l;
             const long long prow = PAGED ? ((long long)w.split * a.tokens + tok) * a.q_heads + head : 0;
-            float o[64 * DB];
-            if (nt > step0) {
-#pragma unroll
-                for (int c = 0; c < 2 * DB; c++) tmem_ld32(to + 32 * c, o + 32 * c);
-#pragma unroll
-                for (int c = 0; c < 2 * DB; c++) tmem_wait_ld32(o + 32 * c);
+            // 32 columns at a time out of tensor memory: a thread holds a row and
+            // writes whole 32-byte sectors of it (16-byte pieces: 2 us a tile, so: 1)
+            const long long at = PAGED ? prow * a.d : (w.first + tok) * a.out_ts + head * a.out_hs;
+            if constexpr (PAGED) {
+                // log2 of the weights' sum; -inf where nothing was seen
+                if (real) a.part_lse[prow] = none ? -INFINITY : fmaf(m, sl, log2f(l));
             }
-            if (real) {
+#pragma unroll 1
+            for (int c = 0; c < 2 * DB; c++) {
+                float o[32];
+                if (nt > step0) {
+                    tmem_ld32(to + 32 * c, o);
+                    tmem_wait_ld32(o);
+                }
 #pragma unroll
-                for (int i = 0; i < 64 * DB; i++) o[i] = none ? 0.f : o[i] * r;
-                if constexpr (PAGED) {
-                    // log2 of the weights' sum; -inf where nothing was seen
-                    a.part_lse[prow] = none ? -INFINITY : fmaf(m, sl, log2f(l));
-                    float4 *dst = (float4 *)(a.part_o + prow * a.d);
+                for (int i = 0; i < 32; i++) o[i] = none ? 0.f : o[i] * r;
+                if (real) {
 #pragma unroll
-                    for (int i = 0; i < 16 * DB; i++)
-                        if (4 * i < a.d) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
-                } else {
-                    T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs;
-                    if (a.vec_out) {
+                    for (int i = 0; i < 32; i += PAGED ? 8 : 16) {
+                        if (32 * c + i >= a.d) break;
+                        if constexpr (PAGED) {
+                            store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
+                        } else {
+                            T *dst = (T *)a.out + at + 32 * c + i;
+                            uint32_t v[8];
 #pragma unroll
-                        for (int i = 0; i < 8 * DB; i++)
-                            if (8 * i < a.d)
-                                ((uint4 *)dst)[i] =
-                                    make_uint4(pack2<T>(o[8 * i], o[8 * i + 1]), pack2<T>(o[8 * i + 2], o[8 * i + 3]),
-                                               pack2<T>(o[8 * i + 4], o[8 * i + 5]), pack2<T>(o[8 * i + 6], o[8 * i + 7]));
-                    } else {
+                            for (int e = 0; e < 8; e++) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
+                            if (a.out_bytes == 32) store32(dst, v);
+                            else if (a.out_bytes == 16) {
+                                ((uint4 *)dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                                if (32 * c + i + 8 < a.d) ((uint4 *)dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                            } else {
 #pragma unroll
-                        for (int i = 0; i < 64 * DB; i++)
-                            if (i < a.d) dst[i] = from_f32<T>(o[i]);
+                                for (int e = 0; e < 16; e++)
+                                    if (32 * c + i + e < a.d) dst[e] = from_f32<T>(o[i + e]);
+                            }
+                        }
                     }
                 }
+                __syncwarp();
             }
         }
     } else {

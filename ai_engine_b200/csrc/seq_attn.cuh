@@ -245,7 +245,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             if (!found && lane == 0) sh.seq_len = 0;
         }
     }
-    if (threadIdx.x == 0) {
+    // beside that, by other warps: tensor memory, barriers, the maps' descriptors
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (threadIdx.x == 32 * 8) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+    }
+    if (threadIdx.x == 32 * 10) {
         mbar_init(&sh.q_full, 1);
         for (int i = 0; i < Sm::kStages; i++) {
             mbar_init(&sh.kv_full[i], 1);
@@ -261,12 +271,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         sh.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
     if constexpr (!PAGED) {
         w.first = sh.seq_first;
         w.len = sh.seq_len;
         w.pair = sh.pair;
-        if (w.len == 0) return;  // a block past the last pair
+        if (w.len == 0) {  // a block past the last pair
+            if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+            return;
+        }
     }
     // keys seen by a tile's last token; `keys` also bounds the values that exist
     const int tok0 = w.pair * 2 * tpt;
@@ -283,14 +299,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // the streams' own part (prefix_step_kernel) may start beside this one
     if constexpr (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = sh.tmem;
     volatile uint32_t *abort = &sh.abort;
     auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t site) {
         if (mbar_wait(bar, parity)) return true;

@@ -192,6 +192,26 @@ pages_fork_plan_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int 
     }
 }
 
+// One block copies 16-byte pieces, 4 a thread in flight at a time.  Memory-bound:
+// 790 MB of moving pages of 32 KB take 131 us, 6.0 TB/s (one at a time 157 us; 8
+// at a time 130 us, but 22 us against 18 for 96 forks' pages of 16 KB).
+__device__ __forceinline__ void copy_chunk(const char *src, char *dst, long long vecs)
+{
+    constexpr int kAhead = 4;
+    const uint4 *from = (const uint4 *)src;
+    uint4 *to = (uint4 *)dst;
+    for (long long i0 = threadIdx.x; i0 < vecs; i0 += kAhead * blockDim.x) {
+        uint4 v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+            if (i0 + k * blockDim.x < vecs)
+                v[k] = from[i0 + k * blockDim.x];
+#pragma unroll
+        for (int k = 0; k < kAhead; k++)
+            if (i0 + k * blockDim.x < vecs) to[i0 + k * blockDim.x] = v[k];
+    }
+}
+
 // Copies the listed pages in every layer, K and V: one block per chunk at a time.
 __device__ __forceinline__ void copy_pages(const PagesArgs &a, const int2 *pairs, int n, int block, int blocks)
 {
@@ -201,9 +221,7 @@ __device__ __forceinline__ void copy_pages(const PagesArgs &a, const int2 *pairs
         const int2 p = pairs[u / chunks];
         if (p.x < 0 || p.y < 0 || p.x >= a.pages || p.y >= a.pages) continue;
         const long long c = u % chunks * a.pages;
-        const uint4 *from = (const uint4 *)(a.kv + (c + p.x) * a.page_bytes);
-        uint4 *to = (uint4 *)(a.kv + (c + p.y) * a.page_bytes);
-        for (long long i = threadIdx.x; i < vecs; i += blockDim.x) to[i] = from[i];
+        copy_chunk(a.kv + (c + p.x) * a.page_bytes, a.kv + (c + p.y) * a.page_bytes, vecs);
     }
 }
 
@@ -240,9 +258,7 @@ pages_copy_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
         const int x = src[u / chunks], y = dst[u / chunks];
         if (x < 0 || y < 0 || x >= a.pages || y >= a.pages) continue;
         const long long c = u % chunks * a.pages;
-        const uint4 *from = (const uint4 *)(a.kv + (c + x) * a.page_bytes);
-        uint4 *to = (uint4 *)(a.kv + (c + y) * a.page_bytes);
-        for (long long i = threadIdx.x; i < vecs; i += blockDim.x) to[i] = from[i];
+        copy_chunk(a.kv + (c + x) * a.page_bytes, a.kv + (c + y) * a.page_bytes, vecs);
     }
 }
 

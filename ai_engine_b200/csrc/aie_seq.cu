@@ -477,8 +477,7 @@ extern "C" int aie_pages_fork(const aie_pages *p, const int32_t *src, const int3
     cudaStream_t s = (cudaStream_t)stream;
     pages_fork_plan_kernel<<<1, kPagesThreads, (p->rows + 31) / 32 * 4, s>>>(a, src, dst, (int)n);
     TRY(launched(cudaGetLastError(), "fork"));
-    pages_fork_kernel<<<copy_grid(2ll * p->layers * n), 256, 0, s>>>(a, src, dst, (int)n);
-    return launched(cudaGetLastError(), "fork");
+    return launched(launch_second(pages_fork_kernel, copy_grid(2ll * p->layers * n), s, a, src, dst, (int)n), "fork");
 }
 
 extern "C" int aie_pages_copy(const aie_pages *p, const int32_t *src, const int32_t *dst, uint32_t n, void *stream)
@@ -511,6 +510,6 @@ extern "C" int aie_pages_compact(const aie_pages *p, int32_t *remap, void *strea
     cudaStream_t s = (cudaStream_t)stream;
     pages_compact_plan_kernel<<<1, kPagesThreads, 0, s>>>(a, remap);
     TRY(launched(cudaGetLastError(), "compact"));
-    pages_compact_kernel<<<copy_grid(2ll * p->layers * p->pages), 256, 0, s>>>(a, remap);
-    return launched(cudaGetLastError(), "compact");
+    return launched(launch_second(pages_compact_kernel, copy_grid(2ll * p->layers * p->pages), s, a, (const int32_t *)remap),
+                    "compact");
 }

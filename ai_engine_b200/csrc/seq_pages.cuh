@@ -153,6 +153,7 @@ pages_grow_kernel(PagesArgs a, const int32_t *rows, const int32_t *counts, int n
 __global__ void __launch_bounds__(kPagesThreads)
 pages_fork_plan_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ unsigned map[];
     __shared__ int smem[32];
     bool ok = rows_ok(dst, n, a, true, map);
@@ -229,6 +230,7 @@ __device__ __forceinline__ void copy_pages(const PagesArgs &a, const int2 *pairs
 __global__ void __launch_bounds__(256)
 pages_fork_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the first part's decisions
     if (!a.ws[1]) return;
     const int2 *pairs = (const int2 *)(a.ws + 2);
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
@@ -279,6 +281,7 @@ __global__ void __launch_bounds__(256) pages_free_kernel(PagesArgs a, const int3
 // Compact, first part: new numbers, the pages to move, the counts in their new places.
 __global__ void __launch_bounds__(kPagesThreads) pages_compact_plan_kernel(PagesArgs a, int32_t *remap)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     __shared__ int smem[32];
     int live = 0;
     for (int p = threadIdx.x; p < a.pages; p += blockDim.x) live += a.refs[p] > 0;
@@ -312,12 +315,29 @@ __global__ void __launch_bounds__(kPagesThreads) pages_compact_plan_kernel(Pages
 // Compact, second part: the moves, and the rows' new page numbers.
 __global__ void __launch_bounds__(256) pages_compact_kernel(PagesArgs a, const int32_t *remap)
 {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the first part's decisions
     const long long all = (long long)a.rows * a.width;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long long)gridDim.x * blockDim.x) {
         const int page = a.table[i];
         if (page >= 0) a.table[i] = page < a.pages ? remap[page] : -1;
     }
     copy_pages(a, (const int2 *)(a.ws + 2), a.ws[0], blockIdx.x, gridDim.x);
+}
+
+// The second part of a call: its blocks are set up while the first part runs.
+template <typename... P, typename... A>
+static cudaError_t launch_second(void (*fn)(P...), unsigned grid, cudaStream_t s, A... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
 }  // namespace aie

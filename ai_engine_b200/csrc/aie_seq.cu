@@ -238,8 +238,9 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
 {
     PrefixPlan w = {};
     const uint32_t keys = std::min(p.prefix_len, p.max_len), size = p.pages.page_size;
+    const uint64_t units = (uint64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16);
     // pages of whole swizzle atoms: 8 places
-    const bool heads_ok = attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) && size % 8 == 0 &&
+    const bool heads_ok = units <= 0x3fffffffu && attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) && size % 8 == 0 &&
                           attn_addressable(p.pages.k, p.pages.token_stride, p.pages.head_stride, size, p.kv_heads) &&
                           attn_addressable(p.pages.v, p.pages.page_stride, 8, p.pages.pages, 1);
     if (keys && p.batch && heads_ok &&
@@ -249,11 +250,11 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
         w.row_pairs = ((int)p.batch + 2 * tpt - 1) / (2 * tpt);
         // one block per SM at a time: the pieces (of whole tiles) that give the
         // shortest run, a block costing about three tiles besides its own
-        const long long units = (long long)w.row_pairs * p.kv_heads, sms = tc_sm_count();
+        const long long blocks = (long long)w.row_pairs * p.kv_heads, sms = tc_sm_count();
         long long best = 0;
         for (int want = 1; want <= std::min(tiles, kAtMostSplits); want++) {
             const int per = (tiles + want - 1) / want, splits = (tiles + per - 1) / per;
-            const long long cost = (units * splits + sms - 1) / sms * (per + 3);
+            const long long cost = (blocks * splits + sms - 1) / sms * (per + 3);
             if (!best || cost < best) {
                 best = cost;
                 w.splits = splits;
@@ -261,8 +262,7 @@ static PrefixPlan prefix_plan(const aie_prefix &p)
             }
         }
     }
-    const uint64_t units = (uint64_t)p.batch * p.kv_heads * ((p.q_heads / p.kv_heads + 15) / 16);
-    if (heads_ok && (w.splits || !keys) && units <= 0x3fffffffu) {
+    if (heads_ok && (w.splits || !keys)) {
         // up to two blocks per SM, each with four tiles of places or more
         const int places = (int)(p.max_len - keys);
         w.pieces = 1;
@@ -325,17 +325,15 @@ static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
 }
 
 template <typename T>
-static int prefix_rows(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
+static int prefix_rows(const aie_prefix &p, cudaStream_t s)
 {
     PrefixRows<T> a;
     a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
     a.k = (const T *)p.pages.k; a.v = (const T *)p.pages.v;
     a.g = pages_geom(p.pages);
     a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
-    a.part_lse = (const float *)p.workspace;
-    a.part_o = part_o(p, w);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
-    a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
+    a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
     a.scale = p.scale;
     const long long rows = (long long)p.batch * p.q_heads;
     prefix_rows_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
@@ -394,8 +392,8 @@ extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
     cudaStream_t s = (cudaStream_t)stream;
     if (w.splits) TRY(prefix_tc(*p, w, s));
     if (w.pieces) return p->dtype == AIE_DT_F16 ? prefix_step<__half>(*p, w, s) : prefix_step<__nv_bfloat16>(*p, w, s);
-    if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, w, s);
-    return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, w, s) : prefix_rows<__nv_bfloat16>(*p, w, s);
+    if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, s);
+    return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, s) : prefix_rows<__nv_bfloat16>(*p, s);
 }
 
 // --------------------------------------------------------------- pages ---

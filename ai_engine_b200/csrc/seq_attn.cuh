@@ -213,34 +213,42 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     } else {
         w.split = 0;
         if (warp == 0) {
-            // unit -> (sequence, pair of tiles): 32 sequences at a time
+            // unit -> (sequence, pair of tiles): 128 sequences at a time, 4 a lane
             int at = 0;
             bool found = false;
-            for (int s0 = 0; s0 < a.seqs && !found; s0 += 32) {
-                const int s = s0 + lane;
-                int first = 0, n = 0;
-                if (s < a.seqs) {
-                    first = min(max(a.cu[s], 0), a.tokens);
-                    n = max(min(a.cu[s + 1], a.tokens) - first, 0);
+            for (int s0 = 0; s0 < a.seqs && !found; s0 += 128) {
+                int start[5], pairs[4], sum = 0;
+#pragma unroll
+                for (int i = 0; i < 5; i++) start[i] = min(max(a.cu[min(s0 + 4 * lane + i, a.seqs)], 0), a.tokens);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    pairs[i] = (max(start[i + 1] - start[i], 0) + 2 * tpt - 1) / (2 * tpt);
+                    sum += pairs[i];
                 }
-                const int pairs = (n + 2 * tpt - 1) / (2 * tpt);
-                int sum = pairs;
+                int upto = sum;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, sum, o);
-                    if (lane >= o) sum += y;
+                    const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += y;
                 }
-                const unsigned hit = __ballot_sync(0xffffffffu, unit < at + sum);
+                const unsigned hit = __ballot_sync(0xffffffffu, unit < at + upto);
                 if (hit) {
                     found = true;
                     if (lane == __ffs(hit) - 1) {
-                        sh.seq_first = first;
-                        sh.seq_len = n;
-                        // a causal sequence's last tiles see the most keys: first
-                        sh.pair = pairs - 1 - (unit - (at + sum - pairs));
+                        int left = unit - (at + upto - sum);  // among this lane's pairs
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            if (left >= 0 && left < pairs[i]) {
+                                sh.seq_first = start[i];
+                                sh.seq_len = start[i + 1] - start[i];
+                                // a causal sequence's last tiles see the most keys: first
+                                sh.pair = pairs[i] - 1 - left;
+                            }
+                            left -= pairs[i];
+                        }
                     }
                 }
-                at += __shfl_sync(0xffffffffu, sum, 31);
+                at += __shfl_sync(0xffffffffu, upto, 31);
             }
             if (!found && lane == 0) sh.seq_len = 0;
         }

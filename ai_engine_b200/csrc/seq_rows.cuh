@@ -4,7 +4,10 @@
 //   s_j = scale q . k_j,  m = max s,  l = sum e^(s_j - m),
 //   out = sum e^(s_j - m) v_j / l
 //
-// with m, l and the sum carried along 32 keys at a time.
+// with m, l and the sum carried along 32 keys at a time.  For the calls that the
+// tensor cores do not take (seq_attn.cuh); bound by the dot products, a key a
+// lane, at a few TFLOP/s: 826 ms for two prompts of 8192 and 6001 tokens, 32
+// heads of 128, that take 0.8 ms there.
 #pragma once
 #include "seq_common.cuh"
 
@@ -45,29 +48,15 @@ struct PagedKeys {
     }
 };
 
-// A row's result over some of its keys: weights relative to e^m, their sum l,
-// and this lane's elements (lane + 32 i) of the weighted sum of values.
-struct RowSum {
-    float m, l, acc[kRowsMaxDim / 32];
-};
-
-__device__ __forceinline__ void row_sum_init(RowSum &r)
-{
-    r.m = -INFINITY;
-    r.l = 0.f;
-#pragma unroll
-    for (int i = 0; i < kRowsMaxDim / 32; i++) r.acc[i] = 0.f;
-}
-
-// The row's keys from..n added to r, and the result written.  qs: this
-// warp's scaled query in shared memory.
+// One row over its first n keys.  qs: this warp's scaled query in shared memory.
 template <typename T, typename Keys>
-__device__ __forceinline__ void attend_row(const float *qs, const Keys &keys, RowSum &r, int from, int n, int d, T *out,
-                                           int lane)
+__device__ __forceinline__ void attend_row(const float *qs, const Keys &keys, int n, int d, T *out, int lane)
 {
-    float (&acc)[kRowsMaxDim / 32] = r.acc;
-    float m = r.m, l = r.l;
-    for (int j0 = from; j0 < n; j0 += 32) {
+    float acc[kRowsMaxDim / 32];
+#pragma unroll
+    for (int i = 0; i < kRowsMaxDim / 32; i++) acc[i] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 32) {
         const int j = j0 + lane;
         const T *kj = nullptr, *vj = nullptr;
         const bool real = j < n && keys.find(j, kj, vj);
@@ -137,9 +126,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(PromptRows<T> a)
     for (int i = lane; i < a.d; i += 32) qs[warp][i] = to_f32(q[i]) * a.scale;
     __syncwarp();
     const PackedKeys<T> keys{a.k, a.v, first, h / a.group};
-    RowSum r;
-    row_sum_init(r);
-    attend_row<T>(qs[warp], keys, r, 0, (a.causal ? t + 1 : end) - first, a.d, a.o.at(t, h), lane);
+    attend_row<T>(qs[warp], keys, (a.causal ? t + 1 : end) - first, a.d, a.o.at(t, h), lane);
 }
 
 template <typename T>
@@ -148,8 +135,7 @@ struct PrefixRows {
     const T *k, *v;
     PagesGeom g;
     const int32_t *prefix, *table, *lens;
-    const float *part_o, *part_lse;  // the shared part's results (attn_tc_kernel), or NULL
-    int batch, hq, group, d, shared, max_len, table_stride, splits;
+    int batch, hq, group, d, shared, max_len, table_stride;
     float scale;
 };
 
@@ -159,29 +145,13 @@ __global__ void __launch_bounds__(128) prefix_rows_kernel(PrefixRows<T> a)
     __shared__ float qs[4][kRowsMaxDim];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * 4 + warp;
-    const long long rows = (long long)a.batch * a.hq;
-    if (row >= rows) return;
+    if (row >= (long long)a.batch * a.hq) return;
     const int b = (int)(row / a.hq), h = (int)(row % a.hq);
     const T *q = a.q.at(b, h);
     for (int i = lane; i < a.d; i += 32) qs[warp][i] = to_f32(q[i]) * a.scale;
     __syncwarp();
     const PagedKeys<T> keys{a.k, a.v, a.g, a.prefix, a.table + (long long)b * a.table_stride, a.shared, h / a.group};
-    RowSum r;
-    row_sum_init(r);
-    float top = -INFINITY;
-    for (int i = 0; i < a.splits; i++) top = fmaxf(top, a.part_lse[i * rows + row]);
-    if (top > -INFINITY) {
-        r.m = top * 0.69314718055994531f;  // from log2
-        for (int i = 0; i < a.splits; i++) {
-            const float w = exp2f(a.part_lse[i * rows + row] - top);
-            r.l += w;
-            const float *o = a.part_o + (i * rows + row) * a.d;
-#pragma unroll
-            for (int k = 0; k < kRowsMaxDim / 32; k++)
-                if (lane + 32 * k < a.d) r.acc[k] = fmaf(w, o[lane + 32 * k], r.acc[k]);
-        }
-    }
-    attend_row<T>(qs[warp], keys, r, a.splits ? a.shared : 0, min(a.lens[b], a.max_len), a.d, a.o.at(b, h), lane);
+    attend_row<T>(qs[warp], keys, min(a.lens[b], a.max_len), a.d, a.o.at(b, h), lane);
 }
 
 }  // namespace aie

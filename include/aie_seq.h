@@ -133,7 +133,7 @@ typedef enum aie_pages_status {
 /* Bytes of scratch for a call with n list entries. */
 AIE_API uint64_t aie_pages_workspace(uint32_t pages, uint32_t n);
 
-/* Row rows[i] gets counts[i] more tokens, and pages for them: the lowest
+/* Row rows[i] gets counts[i] (0 if negative) more tokens, and pages for them: the lowest
  * free pages, in the order of the list.  slots (tokens of them, the list's
  * order, nullable when tokens is 0) receives where each new token stands:
  * page * page_size + place; entries past the counts' sum become -1. */

@@ -166,6 +166,26 @@ def test_prompt(cuda_ok, lens, hq, hk, d, dt, causal):
     _seq.check(got, *_prompt_want(q, k, v, lens, causal, d ** -0.5))
 
 
+@pytest.mark.parametrize("n, hq, hk, d", [(31, 4, 2, 64), (128, 2, 1, 64), (129, 4, 4, 128), (300, 8, 2, 64)])
+def test_prompt_many_sequences(cuda_ok, n, hq, hk, d):
+    lens = [(i * 37) % 90 if i % 5 else 0 for i in range(n)]
+    x = _rand((sum(lens), hq + 2 * hk, d), F16, n)
+    q, k, v = x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:]
+    _seq.check(attention.prompt_attention(q, k, v, _cu(lens)), *_prompt_want(q, k, v, lens, True, d ** -0.5))
+
+
+def test_prompt_broadcast_values_and_starts_out_of_range(cuda_ok):
+    """Values expanded over heads (stride 0); entries of cu outside the tokens are cut to them."""
+    t, d = 90, 64
+    q, k = _rand((t, 4, d), F16, 1), _rand((t, 4, d), F16, 2)
+    v = _rand((t, 1, d), F16, 3).expand(t, 4, d)
+    _seq.check(attention.prompt_attention(q, k, v, _cu([t])), *_prompt_want(q, k, v, [t], True, d ** -0.5))
+    out = torch.full_like(q, 5.0)
+    cu = torch.tensor([-7, 40, 2000], dtype=torch.int32, device="cuda")
+    attention.prompt_attention(q, k, k, cu, out=out)
+    _seq.check(out, *_prompt_want(q, k, k, [40, 50], True, d ** -0.5))
+
+
 @pytest.mark.parametrize("lens, hq, hk, d", [([70, 3], 4, 2, 64), ([33], 3, 1, 24), ([9, 9], 2, 2, 256)])
 def test_prompt_f32(cuda_ok, lens, hq, hk, d):
     t = sum(lens)

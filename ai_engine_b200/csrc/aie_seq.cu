@@ -141,8 +141,7 @@ static int prompt_rows(const aie_prompt &p, cudaStream_t s)
     a.d = (int)p.head_dim; a.causal = p.causal != 0;
     a.scale = p.scale;
     const long long rows = (long long)p.tokens * p.q_heads;
-    prompt_rows_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
-    return launched(cudaGetLastError(), "prompt attention");
+    return launched(launch_behind(prompt_rows_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "prompt attention");
 }
 
 // Whether the tensor cores take these heads: 16-bit operands, a head of at
@@ -336,8 +335,7 @@ static int prefix_rows(const aie_prefix &p, cudaStream_t s)
     a.shared = (int)p.prefix_len; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
     a.scale = p.scale;
     const long long rows = (long long)p.batch * p.q_heads;
-    prefix_rows_kernel<T><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
-    return launched(cudaGetLastError(), "prefix attention");
+    return launched(launch_behind(prefix_rows_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "prefix attention");
 }
 
 template <typename T>
@@ -365,8 +363,7 @@ static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
         !attn_map(&v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
                   a.box_rows))
         return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
-    const bool behind = w.splits > 0;
-    return launched(a.d <= 64 ? step_launch<T, 64>(k, v, a, w.pieces, behind, s) : step_launch<T, 128>(k, v, a, w.pieces, behind, s),
+    return launched(a.d <= 64 ? step_launch<T, 64>(k, v, a, w.pieces, s) : step_launch<T, 128>(k, v, a, w.pieces, s),
                     "prefix attention");
 }
 
@@ -459,9 +456,9 @@ extern "C" int aie_pages_grow(const aie_pages *p, const int32_t *rows, const int
         TRY(check_list(rows, "rows", n));
         TRY(check_list(counts, "counts", n));
     }
-    pages_grow_kernel<<<1, kPagesThreads, (p->rows + 31) / 32 * 4, (cudaStream_t)stream>>>(a, rows, counts, (int)n, slots,
-                                                                                           (int)tokens);
-    return launched(cudaGetLastError(), "grow");
+    return launched(launch_behind(pages_grow_kernel, 1, kPagesThreads, (p->rows + 31) / 32 * 4, (cudaStream_t)stream, a, rows, counts,
+                                  (int)n, slots, (int)tokens),
+                    "grow");
 }
 
 extern "C" int aie_pages_fork(const aie_pages *p, const int32_t *src, const int32_t *dst, uint32_t n, void *stream)
@@ -473,9 +470,8 @@ extern "C" int aie_pages_fork(const aie_pages *p, const int32_t *src, const int3
     TRY(check_list(src, "src", n));
     TRY(check_list(dst, "dst", n));
     cudaStream_t s = (cudaStream_t)stream;
-    pages_fork_plan_kernel<<<1, kPagesThreads, (p->rows + 31) / 32 * 4, s>>>(a, src, dst, (int)n);
-    TRY(launched(cudaGetLastError(), "fork"));
-    return launched(launch_second(pages_fork_kernel, copy_grid(2ll * p->layers * n), s, a, src, dst, (int)n), "fork");
+    TRY(launched(launch_behind(pages_fork_plan_kernel, 1, kPagesThreads, (p->rows + 31) / 32 * 4, s, a, src, dst, (int)n), "fork"));
+    return launched(launch_behind(pages_fork_kernel, copy_grid(2ll * p->layers * n), 256, 0, s, a, src, dst, (int)n), "fork");
 }
 
 extern "C" int aie_pages_copy(const aie_pages *p, const int32_t *src, const int32_t *dst, uint32_t n, void *stream)
@@ -485,8 +481,8 @@ extern "C" int aie_pages_copy(const aie_pages *p, const int32_t *src, const int3
     if (!n) return AIE_OK;
     TRY(check_list(src, "src", n));
     TRY(check_list(dst, "dst", n));
-    pages_copy_kernel<<<copy_grid(2ll * p->layers * n), 256, 0, (cudaStream_t)stream>>>(a, src, dst, (int)n);
-    return launched(cudaGetLastError(), "copy");
+    return launched(launch_behind(pages_copy_kernel, copy_grid(2ll * p->layers * n), 256, 0, (cudaStream_t)stream, a, src, dst, (int)n),
+                    "copy");
 }
 
 extern "C" int aie_pages_free(const aie_pages *p, const int32_t *rows, uint32_t n, void *stream)
@@ -495,8 +491,7 @@ extern "C" int aie_pages_free(const aie_pages *p, const int32_t *rows, uint32_t 
     TRY(pages_args(p, true, false, false, &a));
     if (!n) return AIE_OK;
     TRY(check_list(rows, "rows", n));
-    pages_free_kernel<<<n, 256, 0, (cudaStream_t)stream>>>(a, rows);
-    return launched(cudaGetLastError(), "free");
+    return launched(launch_behind(pages_free_kernel, n, 256, 0, (cudaStream_t)stream, a, rows), "free");
 }
 
 extern "C" int aie_pages_compact(const aie_pages *p, int32_t *remap, void *stream)
@@ -506,8 +501,7 @@ extern "C" int aie_pages_compact(const aie_pages *p, int32_t *remap, void *strea
     TRY(check_ws(p));
     if (!remap) return fail(AIE_E_INVALID, "remap is NULL");
     cudaStream_t s = (cudaStream_t)stream;
-    pages_compact_plan_kernel<<<1, kPagesThreads, 0, s>>>(a, remap);
-    TRY(launched(cudaGetLastError(), "compact"));
-    return launched(launch_second(pages_compact_kernel, copy_grid(2ll * p->layers * p->pages), s, a, (const int32_t *)remap),
+    TRY(launched(launch_behind(pages_compact_plan_kernel, 1, kPagesThreads, 0, s, a, remap), "compact"));
+    return launched(launch_behind(pages_compact_kernel, copy_grid(2ll * p->layers * p->pages), 256, 0, s, a, (const int32_t *)remap),
                     "compact");
 }

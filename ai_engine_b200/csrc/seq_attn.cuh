@@ -201,6 +201,36 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tpt = a.tokens_per_tile;
 
+    // tensor memory, barriers, the maps' descriptors: each by a warp of its own
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (threadIdx.x == 32 * 8) {
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
+    }
+    if (threadIdx.x == 32 * 10) {
+        mbar_init(&sh.q_full, 1);
+        for (int i = 0; i < Sm::kStages; i++) {
+            mbar_init(&sh.kv_full[i], 1);
+            mbar_init(&sh.kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sh.s_full[i], 1);
+            mbar_init(&sh.p_full[i][0], 5);
+            mbar_init(&sh.p_full[i][1], 4);
+            mbar_init(&sh.o_full[i], 1);
+        }
+        mbar_init(&sh.drain, 1);
+        sh.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // also for the streams' own part (prefix_step_kernel), which may then start
+    // beside this one
+    behind_last_launch();
+
     // ---- which tokens, which keys
     AttnWork w;
     w.kvh = blockIdx.x % a.kv_heads;
@@ -253,32 +283,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             if (!found && lane == 0) sh.seq_len = 0;
         }
     }
-    // beside that, by other warps: tensor memory, barriers, the maps' descriptors
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512));
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-    }
-    if (threadIdx.x == 32 * 8) {
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_q)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_k)) : "memory");
-        asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_v)) : "memory");
-    }
-    if (threadIdx.x == 32 * 10) {
-        mbar_init(&sh.q_full, 1);
-        for (int i = 0; i < Sm::kStages; i++) {
-            mbar_init(&sh.kv_full[i], 1);
-            mbar_init(&sh.kv_empty[i], 1);
-        }
-        for (int i = 0; i < 2; i++) {
-            mbar_init(&sh.s_full[i], 1);
-            mbar_init(&sh.p_full[i][0], 5);
-            mbar_init(&sh.p_full[i][1], 4);
-            mbar_init(&sh.o_full[i], 1);
-        }
-        mbar_init(&sh.drain, 1);
-        sh.abort = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -304,9 +308,6 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     };
     const int n0 = steps_of(0), n1 = steps_of(1), n = max(n0, n1);
     auto n_of = [&](int t) { return t ? n1 : n0; };
-    // the streams' own part (prefix_step_kernel) may start beside this one
-    if constexpr (PAGED) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-
     volatile uint32_t *abort = &sh.abort;
     auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t site) {
         if (mbar_wait(bar, parity)) return true;
@@ -649,8 +650,7 @@ static cudaError_t attn_launch(const CUtensorMap &q, const CUtensorMap &k, const
     auto *fn = &attn_tc_kernel<T, DB, PAGED>;
     cudaError_t e = ensure_smem_attr((const void *)fn, AttnSmem<DB>::kBytes);
     if (e != cudaSuccess) return e;
-    fn<<<grid, kAtThreads, AttnSmem<DB>::kBytes, s>>>(q, k, v, a);
-    return cudaGetLastError();
+    return launch_behind(fn, grid, kAtThreads, AttnSmem<DB>::kBytes, s, q, k, v, a);
 }
 
 }  // namespace aie

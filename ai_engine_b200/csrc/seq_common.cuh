@@ -56,6 +56,33 @@ static inline PagesGeom pages_geom(const aie_kv_pages &p)
                      (int)p.page_size};
 }
 
+// Every launch of these kernels may be set up while the one before it in the
+// stream still runs (programmatic stream serialization): nothing in memory is
+// touched before this, which waits for that one's end, and only then lets the
+// launch behind this one be set up.  Back to back, a frame's prompt took 10.25
+// us a call without, of which the kernel is 8.7 us.
+__device__ __forceinline__ void behind_last_launch()
+{
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+static cudaError_t launch_behind(void (*fn)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const A &...args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll

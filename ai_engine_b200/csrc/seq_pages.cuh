@@ -101,6 +101,7 @@ pages_grow_kernel(PagesArgs a, const int32_t *rows, const int32_t *counts, int n
     int32_t *list = a.ws + 2;           // the pages handed out
     int32_t *need_at = list + a.pages;  // each entry's first page in it, then its first slot
     int32_t *slot_at = need_at + n;
+    behind_last_launch();
     const bool ok = rows_ok(rows, n, a, false, map);
     int need = 0, sum = 0, bad = 0;
     for (int i0 = 0; i0 < n; i0 += blockDim.x) {
@@ -153,7 +154,7 @@ pages_grow_kernel(PagesArgs a, const int32_t *rows, const int32_t *counts, int n
 __global__ void __launch_bounds__(kPagesThreads)
 pages_fork_plan_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    behind_last_launch();
     extern __shared__ unsigned map[];
     __shared__ int smem[32];
     bool ok = rows_ok(dst, n, a, true, map);
@@ -230,7 +231,7 @@ __device__ __forceinline__ void copy_pages(const PagesArgs &a, const int2 *pairs
 __global__ void __launch_bounds__(256)
 pages_fork_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the first part's decisions
+    behind_last_launch();  // the first part's decisions
     if (!a.ws[1]) return;
     const int2 *pairs = (const int2 *)(a.ws + 2);
     for (int i = blockIdx.x; i < n; i += gridDim.x) {
@@ -254,6 +255,7 @@ pages_fork_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 __global__ void __launch_bounds__(256)
 pages_copy_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 {
+    behind_last_launch();
     const long long vecs = a.page_bytes / 16;
     const int chunks = 2 * a.layers;
     for (long long u = blockIdx.x; u < (long long)n * chunks; u += gridDim.x) {
@@ -268,6 +270,7 @@ pages_copy_kernel(PagesArgs a, const int32_t *src, const int32_t *dst, int n)
 // row is taken by one of the blocks.
 __global__ void __launch_bounds__(256) pages_free_kernel(PagesArgs a, const int32_t *rows)
 {
+    behind_last_launch();
     const int r = rows[blockIdx.x];
     if (r < 0 || r >= a.rows) return;
     int32_t *row = a.table + (long long)r * a.width;
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(256) pages_free_kernel(PagesArgs a, const int3
 // Compact, first part: new numbers, the pages to move, the counts in their new places.
 __global__ void __launch_bounds__(kPagesThreads) pages_compact_plan_kernel(PagesArgs a, int32_t *remap)
 {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    behind_last_launch();
     __shared__ int smem[32];
     int live = 0;
     for (int p = threadIdx.x; p < a.pages; p += blockDim.x) live += a.refs[p] > 0;
@@ -315,29 +318,13 @@ __global__ void __launch_bounds__(kPagesThreads) pages_compact_plan_kernel(Pages
 // Compact, second part: the moves, and the rows' new page numbers.
 __global__ void __launch_bounds__(256) pages_compact_kernel(PagesArgs a, const int32_t *remap)
 {
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // for the first part's decisions
+    behind_last_launch();  // the first part's decisions
     const long long all = (long long)a.rows * a.width;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (long long)gridDim.x * blockDim.x) {
         const int page = a.table[i];
         if (page >= 0) a.table[i] = page < a.pages ? remap[page] : -1;
     }
     copy_pages(a, (const int2 *)(a.ws + 2), a.ws[0], blockIdx.x, gridDim.x);
-}
-
-// The second part of a call: its blocks are set up while the first part runs.
-template <typename... P, typename... A>
-static cudaError_t launch_second(void (*fn)(P...), unsigned grid, cudaStream_t s, A... args)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(256);
-    cfg.stream = s;
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
 }  // namespace aie

@@ -43,6 +43,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) rope_row_kernel(RopeArgs<T> a)
 {
     __shared__ float buf[4][kRopeMaxDim];
+    behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rows = a.hq + a.hk + (a.vp ? a.hk : 0);
     const long long unit = (long long)blockIdx.x * 4 + warp;
@@ -186,6 +187,7 @@ struct RopeVec {
 template <typename T, int LPR, int HPT, bool INTERLEAVED>
 __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(const RopeArgs<T> a, const RopeVec g)
 {
+    behind_last_launch();
     unsigned unit = (unsigned)(((unsigned long long)blockIdx.x * blockDim.x + threadIdx.x) / LPR);
     const int lane = threadIdx.x % LPR;
     if (unit >= g.end) return;  // whole groups of LPR lanes
@@ -350,9 +352,8 @@ static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
     g.slots32 = (unsigned long long)a.pg.pages * a.pg.size <= 0xffffffffull;
     g.inv_d = 1.0f / (float)a.d;
     const unsigned grid = (unsigned)(((unsigned long long)g.end * LPR + kRopeThreads - 1) / kRopeThreads);
-    if (a.interleaved) rope_vec_kernel<T, LPR, HPT, true><<<grid, kRopeThreads, 0, s>>>(a, g);
-    else rope_vec_kernel<T, LPR, HPT, false><<<grid, kRopeThreads, 0, s>>>(a, g);
-    return cudaGetLastError();
+    return launch_behind(a.interleaved ? rope_vec_kernel<T, LPR, HPT, true> : rope_vec_kernel<T, LPR, HPT, false>, grid, kRopeThreads,
+                         0, s, a, g);
 }
 
 // So few heads that one at a time they are all resident at once: one at a time
@@ -375,8 +376,7 @@ static cudaError_t rope_launch(const RopeArgs<T> &a, cudaStream_t s)
         return rope_vec_launch<T, 32>(a, s);
     }
     const long long units = (long long)a.tokens * (a.hq + a.hk + (a.vp ? a.hk : 0));
-    rope_row_kernel<T><<<(unsigned)((units + 3) / 4), 128, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_behind(rope_row_kernel<T>, (unsigned)((units + 3) / 4), 128, 0, s, a);
 }
 
 }  // namespace aie

@@ -114,6 +114,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) prompt_rows_kernel(PromptRows<T> a)
 {
     __shared__ float qs[4][kRowsMaxDim];
+    behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= (long long)a.tokens * a.hq) return;
@@ -143,6 +144,7 @@ template <typename T>
 __global__ void __launch_bounds__(128) prefix_rows_kernel(PrefixRows<T> a)
 {
     __shared__ float qs[4][kRowsMaxDim];
+    behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long row = (long long)blockIdx.x * 4 + warp;
     if (row >= (long long)a.batch * a.hq) return;

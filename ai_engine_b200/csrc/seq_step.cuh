@@ -113,6 +113,9 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const int rank = (int)cluster.block_rank(), ranks = (int)cluster.num_blocks();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+    // behind the shared part's launch, which has waited for the inputs, only its
+    // results have to be waited for, below
+    if (!a.splits) behind_last_launch();
     if (tid == 0) {
         for (int i = 0; i < a.stages; i++) {
             mbar_init(&sh.full[i], 1);
@@ -339,7 +342,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             }
         }
         // the shared part's launch may still run: its results from here on
-        if (first_unit) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (first_unit && a.splits) behind_last_launch();
         first_unit = false;
         if (ranks > 1) cluster.sync();
         else step_sync();
@@ -392,8 +395,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
 }
 
 template <typename T, int DK>
-static cudaError_t step_launch(const CUtensorMap &k, const CUtensorMap &v, StepArgs<T> a, int pieces, bool behind_shared,
-                               cudaStream_t s)
+static cudaError_t step_launch(const CUtensorMap &k, const CUtensorMap &v, StepArgs<T> a, int pieces, cudaStream_t s)
 {
     auto *fn = &prefix_step_kernel<T, DK>;
     // the deepest ring with which two blocks fit an SM
@@ -411,11 +413,11 @@ static cudaError_t step_launch(const CUtensorMap &k, const CUtensorMap &v, StepA
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = (unsigned)pieces;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    // may begin while the shared part's last blocks run (griddepcontrol.wait)
+    // may begin while the last launch's blocks run (behind_last_launch)
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = behind_shared ? 2 : 1;
+    cfg.numAttrs = 2;
     return cudaLaunchKernelEx(&cfg, fn, k, v, a);
 }
 

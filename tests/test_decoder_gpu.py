@@ -93,3 +93,34 @@ def test_command(cuda_ok, capsys):
     from ai_engine_b200 import decoder
     decoder.main(["3", "40", "4"])
     assert "status 0" in capsys.readouterr().out
+
+
+def test_calls_see_what_the_last_one_wrote(cuda_ok):
+    """Launches are set up while the last one runs: chains of calls, each on the
+    last one's results, with and without a wait between them."""
+    from ai_engine_b200 import attention, pages
+    kv = pages.new_cache(2, 40, 16, 2, 64, torch.float16)
+    kv[:, :, 0] = torch.randn(2, 2, 16, 2, 64, device="cuda").half()
+    at = torch.arange(40, dtype=torch.int32, device="cuda")
+    for i in range(39):
+        pages.copy(kv, at[i:i + 1], at[i + 1:i + 2])
+    assert bool((kv == kv[:, :, :1]).all())
+
+    def chain(wait):
+        g = torch.Generator("cuda").manual_seed(1)
+        q = torch.randn(300, 4, 64, generator=g, device="cuda").half()
+        pos, table = torch.arange(300, dtype=torch.int32, device="cuda"), torch.randn(300, 64, generator=g, device="cuda")
+        w, cu = torch.ones(64, device="cuda"), torch.tensor([0, 120, 300], dtype=torch.int32, device="cuda")
+        cache = pages.new_cache(1, 20, 16, 4, 64, torch.float16)
+        rows = torch.arange(19, dtype=torch.int32, device="cuda")[None]
+        for _ in range(12):
+            k = torch.empty_like(q)
+            attention.qk_norm_rope(q, q, pos, table, q_weight=w, k_weight=w, v=q, k_pages=cache[0, 0], v_pages=cache[0, 1],
+                                   slots=torch.arange(300, device="cuda"), q_out=k, k_out=False)
+            q = attention.prompt_attention(k, k, q, cu)
+            one = attention.prefix_attention(q[-1:], cache[0, 0], cache[0, 1], rows[0], 200, rows, pos[-1:])
+            q = torch.cat([q[:-1], one])
+            if wait:
+                torch.cuda.synchronize()
+        return q
+    assert torch.equal(chain(False), chain(True))

@@ -147,6 +147,9 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         // ---- copies; each lane one box of a tile
         const int boxes = kStKeys / a.box_rows;
         for (int u = blockIdx.x / ranks; u < a.units; u += gridDim.x / ranks) {
+            // the multiplying warps hold the first pair's result back until the shared
+            // part is done, however long that takes: no bounded wait runs meanwhile
+            if (u != blockIdx.x / ranks && a.splits) asm volatile("griddepcontrol.wait;" ::: "memory");
             const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk;
             int len, lo, hi;
             tiles_of(b, len, lo, hi);

@@ -291,7 +291,28 @@ static cudaError_t attn_prefix_launch(const CUtensorMap &q, const CUtensorMap &k
     return a.d <= 64 ? attn_launch<T, 1, true>(q, k, v, a, grid, s) : attn_launch<T, 2, true>(q, k, v, a, grid, s);
 }
 
-static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
+// The cache's maps, for both parts: boxes inside one page, whole boxes to both
+// kernels' tiles.
+struct PageMaps {
+    CUtensorMap k, v;
+    int box_rows;
+};
+
+static int page_maps(const aie_prefix &p, PageMaps *m)
+{
+    const aie_kv_pages &g = p.pages;
+    const bool bf16 = p.dtype == AIE_DT_BF16;
+    static_assert(kAtTile % kStKeys == 0, "whole boxes to either tile");
+    m->box_rows = std::gcd((int)g.page_size, kStKeys);
+    if (!attn_map(&m->k, bf16, g.k, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  m->box_rows) ||
+        !attn_map(&m->v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
+                  m->box_rows))
+        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
+    return AIE_OK;
+}
+
+static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, const PageMaps &m, cudaStream_t s)
 {
     AttnArgs a = {};
     a.prefix = p.prefix; a.lens = p.lens;
@@ -304,22 +325,16 @@ static int prefix_tc(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.page_size = (int)p.pages.page_size; a.pages = (int)p.pages.pages;
     a.splits = w.splits; a.tiles_per_split = w.tiles_per_split;
     a.scale_log2 = p.scale * 1.4426950408889634f;
+    a.box_rows = m.box_rows;
     const bool bf16 = p.dtype == AIE_DT_BF16;
-    const aie_kv_pages &g = p.pages;
-    const uint32_t rows = std::gcd(g.page_size, (uint32_t)kAtTile);  // of a box: inside one page, whole boxes a tile
-    a.box_rows = (int)rows;
-    CUtensorMap q, k, v;
+    CUtensorMap q;
     if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.batch, p.q.token_stride, 0, 0, a.group,
-                  a.tokens_per_tile) ||
-        !attn_map(&k, bf16, g.k, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
-                  rows) ||
-        !attn_map(&v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
-                  rows))
+                  a.tokens_per_tile))
         return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
     const uint64_t grid = (uint64_t)w.row_pairs * p.kv_heads * w.splits;
     if (grid > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "too many tiles");
-    return launched(bf16 ? attn_prefix_launch<__nv_bfloat16>(q, k, v, a, (unsigned)grid, s)
-                         : attn_prefix_launch<__half>(q, k, v, a, (unsigned)grid, s),
+    return launched(bf16 ? attn_prefix_launch<__nv_bfloat16>(q, m.k, m.v, a, (unsigned)grid, s)
+                         : attn_prefix_launch<__half>(q, m.k, m.v, a, (unsigned)grid, s),
                     "prefix attention");
 }
 
@@ -339,7 +354,7 @@ static int prefix_rows(const aie_prefix &p, cudaStream_t s)
 }
 
 template <typename T>
-static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
+static int prefix_step(const aie_prefix &p, const PrefixPlan &w, const PageMaps &m, cudaStream_t s)
 {
     const aie_kv_pages &g = p.pages;
     StepArgs<T> a = {};
@@ -352,18 +367,11 @@ static int prefix_step(const aie_prefix &p, const PrefixPlan &w, cudaStream_t s)
     a.d = (int)p.head_dim;
     a.from = (int)p.prefix_len;
     a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
-    a.pages = (int)g.pages; a.page_size = (int)g.page_size; a.box_rows = std::gcd((int)g.page_size, kStKeys);
+    a.pages = (int)g.pages; a.page_size = (int)g.page_size; a.box_rows = m.box_rows;
     a.zs = (a.group + 15) / 16; a.units = a.batch * a.hk * a.zs; a.rows = std::min(a.group, 16);
     a.q_pairs = (uintptr_t)p.q.data % 4 == 0 && p.q.token_stride % 2 == 0 && p.q.head_stride % 2 == 0;
     a.scale_log2 = p.scale * 1.4426950408889634f;
-    const bool bf16 = p.dtype == AIE_DT_BF16;
-    CUtensorMap k, v;
-    if (!attn_map(&k, bf16, g.k, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
-                  a.box_rows) ||
-        !attn_map(&v, bf16, g.v, p.head_dim, p.kv_heads, g.head_stride, g.page_size, g.token_stride, g.pages, g.page_stride, 1,
-                  a.box_rows))
-        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
-    return launched(a.d <= 64 ? step_launch<T, 64>(k, v, a, w.pieces, s) : step_launch<T, 128>(k, v, a, w.pieces, s),
+    return launched(a.d <= 64 ? step_launch<T, 64>(m.k, m.v, a, w.pieces, s) : step_launch<T, 128>(m.k, m.v, a, w.pieces, s),
                     "prefix attention");
 }
 
@@ -387,8 +395,12 @@ extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
     if (p->workspace_bytes < w.bytes || !p->workspace || (uintptr_t)p->workspace % 16)
         return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)w.bytes);
     cudaStream_t s = (cudaStream_t)stream;
-    if (w.splits) TRY(prefix_tc(*p, w, s));
-    if (w.pieces) return p->dtype == AIE_DT_F16 ? prefix_step<__half>(*p, w, s) : prefix_step<__nv_bfloat16>(*p, w, s);
+    if (w.pieces) {
+        PageMaps m;
+        TRY(page_maps(*p, &m));
+        if (w.splits) TRY(prefix_tc(*p, w, m, s));
+        return p->dtype == AIE_DT_F16 ? prefix_step<__half>(*p, w, m, s) : prefix_step<__nv_bfloat16>(*p, w, m, s);
+    }
     if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, s);
     return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, s) : prefix_rows<__nv_bfloat16>(*p, s);
 }

@@ -73,7 +73,7 @@ def _bind_command(out: str):
     libs = os.path.join(os.path.dirname(torch.__file__), "lib")
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, BIND_SRC, "-o", out,
-            "-L", libs, "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-L", HERE, "-l:libaie_conv.so",
+            "-L", libs, "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L", HERE, "-l:libaie_conv.so",
             "-Wl,-rpath,$ORIGIN"]
 
 

@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -165,10 +166,16 @@ private:
     std::optional<c10::cuda::CUDAStreamGuard> on_;
 };
 
-at::Tensor fresh_like(const at::Tensor &t) { return at::empty_like(t, t.options(), at::MemoryFormat::Contiguous); }
+// Contiguous memory straight from torch's allocator (by way of the dispatcher
+// every tensor costs about 0.5 us more).
+at::Tensor fresh_like(const at::Tensor &t)
+{
+    return at::detail::empty_cuda(t.sizes(), t.scalar_type(), t.device(), std::nullopt);
+}
+
 at::Tensor scratch(int64_t n, at::ScalarType type, int device)
 {
-    return at::empty({n}, at::TensorOptions().dtype(type).device(at::kCUDA, (c10::DeviceIndex)device));
+    return at::detail::empty_cuda({n}, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
 }
 
 void arguments(Py_ssize_t got, Py_ssize_t want)

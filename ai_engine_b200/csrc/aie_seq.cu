@@ -412,7 +412,7 @@ constexpr uint32_t kPagesMaxRows = 1u << 18;  // the row bitmap: 32 KB of shared
 static int pages_args(const aie_pages *p, bool rows, bool places, bool kv, PagesArgs *a)
 {
     if (!p) return fail(AIE_E_INVALID, "null arguments");
-    if (!p->pages || p->pages > 0x3fffffffu) return fail(AIE_E_INVALID, "a cache of %u pages", p->pages);
+    if (!p->pages || p->pages >= (uint32_t)kSumCap) return fail(AIE_E_INVALID, "a cache of %u pages", p->pages);
     if (kv) {
         if (!p->kv || !p->layers || !p->page_bytes) return fail(AIE_E_INVALID, "the cache is NULL or empty");
         if ((uintptr_t)p->kv % 16 || p->page_bytes % 16)

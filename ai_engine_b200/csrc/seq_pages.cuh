@@ -19,7 +19,14 @@ struct PagesArgs {
     int layers, pages, page_size, rows, width;
 };
 
-// Exclusive prefix sum over the block's threads; *total for all of them.
+// Sums stop here: more pages than a cache may have, as many tokens as slots can
+// list.  Two of them still fit 32 bits.
+constexpr int kSumCap = 0x3fffffff;
+
+__device__ __forceinline__ int cap_add(int a, int b) { return min(a + b, kSumCap); }
+
+// Exclusive prefix sum over the block's threads; *total for all of them.  Values
+// from 0 to kSumCap; sums stop at kSumCap, so they ascend whatever a list asks for.
 __device__ __forceinline__ int block_scan(int v, int *total, int *smem)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -27,7 +34,7 @@ __device__ __forceinline__ int block_scan(int v, int *total, int *smem)
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        if (lane >= o) x = cap_add(x, y);
     }
     if (lane == 31) smem[warp] = x;
     __syncthreads();
@@ -36,7 +43,7 @@ __device__ __forceinline__ int block_scan(int v, int *total, int *smem)
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
+            if (lane >= o) w = cap_add(w, y);
         }
         smem[lane] = w;
     }
@@ -44,7 +51,8 @@ __device__ __forceinline__ int block_scan(int v, int *total, int *smem)
     const int before = warp ? smem[warp - 1] : 0;
     *total = smem[warps - 1];
     __syncthreads();
-    return before + x - v;
+    const int y = __shfl_up_sync(0xffffffffu, x, 1);
+    return lane ? cap_add(before, y) : before;
 }
 
 // The lowest `need` free pages, in ascending order, to list[0..]; how many there were.
@@ -111,14 +119,16 @@ pages_grow_kernel(PagesArgs a, const int32_t *rows, const int32_t *counts, int n
             const int len = row_len(a, rows[i]);
             count = max(counts[i], 0);
             const long long after = ((long long)len + count + a.page_size - 1) / a.page_size;
-            if (after > a.width) bad = 1;
-            else pages = (int)after - (len + a.page_size - 1) / a.page_size;
+            if (after > a.width) {
+                bad = 1;
+                count = 0;
+            } else pages = (int)after - (len + a.page_size - 1) / a.page_size;
         }
         int total;
-        const int p = need + block_scan(pages, &total, smem);
-        need += total;
-        const int c = sum + block_scan(count, &total, smem);
-        sum += total;
+        const int p = cap_add(need, block_scan(pages, &total, smem));
+        need = cap_add(need, total);
+        const int c = cap_add(sum, block_scan(count, &total, smem));
+        sum = cap_add(sum, total);
         if (i < n) {
             need_at[i] = p;
             slot_at[i] = c;

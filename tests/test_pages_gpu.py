@@ -214,6 +214,19 @@ def test_offsets_beyond_32_bits(cuda_ok):
     assert (kv[:, :, 1] == 3).all() and torch.equal(kv[:, :, 0], kv[:, :, n - 2])
 
 
+@pytest.mark.parametrize("rows, more", [(4096, 0), (4097, 3)])
+def test_growth_beyond_32_bits(cuda_ok, rows, more):
+    """Lists that ask for 2^31 pages and tokens, or some more, find too few."""
+    width = 1 << 19
+    st = pages.new_state(64, rows, width)
+    counts = [width] * 4096 + [more] * (rows - 4096)
+    slots = pages.grow(st, 1, torch.arange(rows, dtype=torch.int32, device="cuda"), _i32(counts), 100)
+    assert (slots == -1).all() and st.status.item() == _lib.PAGES_FULL
+    assert not st.refs.any() and not st.lens.any() and st.table.max() == -1
+    slots = pages.grow(st, 1, _i32([rows - 1, 0]), _i32([5, 2]), 8)
+    assert slots.tolist() == [0, 1, 2, 3, 4, 5, 6, -1]
+
+
 def test_calls_in_a_graph(cuda_ok):
     kv, st, p = _both()
     pages.grow(st, 16, _i32([0]), _i32([37]), 37)

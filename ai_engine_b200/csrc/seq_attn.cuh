@@ -406,7 +406,8 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         if (nt > step0 && ok) ok = __all_sync(0xffffffffu, wait(&sh.o_full[t], 0, 8));
         tc_fence_after();
         if (ok && (nt > step0 || PAGED)) {
-            const bool none = nt <= step0 || seen <= step0 * kAtTile;  // of this split's keys
+            // of this split's keys; scores of -inf alone (l is 0) count as none here
+            const bool none = nt <= step0 || seen <= step0 * kAtTile || (PAGED && l == 0.f);
             const float r = none ? 0.f : 1.f / l;
             const long long prow = PAGED ? ((long long)w.split * a.tokens + tok) * a.q_heads + head : 0;
             // 32 columns at a time out of tensor memory: a thread holds a row and

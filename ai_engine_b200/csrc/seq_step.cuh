@@ -15,7 +15,8 @@
 // Fixed order throughout: results repeat bit for bit.
 //
 // Rounding to fewer bits: the weights to the operands' type for the product
-// with V (l sums them unrounded), and the result.
+// with V (l sums them unrounded; f16 weights 2^7 times as large, as in
+// attn_tc_kernel), and the result.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -284,7 +285,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float off = m[h] == -INFINITY ? 0.f : -m[h] * sl;
+                    const float off = m[h] == -INFINITY ? 0.f : fmaf(-m[h], sl, kWeightShift<T>);
                     float e[4];
 #pragma unroll
                     for (int i = 0; i < 4; i++) e[i] = ex2(fmaf(s[i >> 1][2 * h + (i & 1)], sl, off));
@@ -306,7 +307,8 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (lane == 0) mbar_arrive(&sh.empty[st]);
         }
 
-        // ---- the four warps' results become the block's, in log2 units
+        // ---- the four warps' results become the block's, in log2 units: m less
+        // the weights' shift, so that 2^m l is the sum
         step_sync();  // the last unit's are read
         {
             float *wo = result + warp * a.rows * DK;
@@ -317,7 +319,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
                 l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
                 if (r + 8 * h < heads) {
                     if ((lane & 3) == 0) {
-                        sh.warp_m[warp][r + 8 * h] = m[h] * sl;
+                        sh.warp_m[warp][r + 8 * h] = fmaf(m[h], sl, -kWeightShift<T>);
                         sh.warp_l[warp][r + 8 * h] = l[h];
                     }
 #pragma unroll

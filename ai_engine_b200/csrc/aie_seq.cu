@@ -360,13 +360,14 @@ static int prefix_step(const aie_prefix &p, const PrefixPlan &w, const PageMaps 
     StepArgs<T> a = {};
     a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
     a.size = make_fastdiv((int)g.page_size);
-    a.table = p.table; a.lens = p.lens;
+    a.prefix = p.prefix; a.table = p.table; a.lens = p.lens;
     a.part_lse = (const float *)p.workspace;
     a.part_o = part_o(p, w);
     a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.hk = (int)p.kv_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim;
     a.from = (int)p.prefix_len;
     a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride; a.splits = w.splits;
+    a.ends_in = w.splits ? std::min(a.from, a.max_len) : 0; a.split_places = w.tiles_per_split * kAtTile;
     a.pages = (int)g.pages; a.page_size = (int)g.page_size; a.box_rows = m.box_rows;
     a.zs = (a.group + 15) / 16; a.units = a.batch * a.hk * a.zs; a.rows = std::min(a.group, 16);
     a.q_pairs = (uintptr_t)p.q.data % 4 == 0 && p.q.token_stride % 2 == 0 && p.q.head_stride % 2 == 0;

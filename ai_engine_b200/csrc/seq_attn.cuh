@@ -427,6 +427,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 // log2 of the weights' sum; -inf where nothing was seen
                 if (real) a.part_lse[prow] = none ? -INFINITY : fmaf(m, sl, log2f(l) - kWeightShift<T>);
             }
+            bool nan = false;
 #pragma unroll 1
             for (int c = 0; c < 2 * DB; c++) {
                 float o[32];
@@ -436,6 +437,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 }
 #pragma unroll
                 for (int i = 0; i < 32; i++) o[i] = none ? 0.f : o[i] * r;
+                if (PAGED && seen < keys)
+#pragma unroll
+                    for (int i = 0; i < 32; i++) nan |= o[i] != o[i];
                 if (real) {
 #pragma unroll
                     for (int i = 0; i < 32; i += PAGED ? 8 : 16) {
@@ -461,6 +465,10 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 }
                 __syncwarp();
             }
+            // A stream that ends in the prefix, and a result of NaN: values that it does
+            // not see may have made it so (0 times them).  prefix_step_kernel works
+            // it out anew where this says so.
+            if (nan && real) a.part_lse[prow] = __int_as_float(0x7fffffff);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kAtIssueRegs));

@@ -14,6 +14,11 @@
 // cluster of up to 8 blocks, whose results meet in distributed shared memory.
 // Fixed order throughout: results repeat bit for bit.
 //
+// A stream that ends inside the shared part has no places of its own.  The
+// shared part multiplies its weights of 0 with values that it does not see, and
+// 0 times a value that is not finite is NaN.  Only then its places are gone
+// through here too, and the shared part's results left out.
+//
 // Rounding to fewer bits: the weights to the operands' type for the product
 // with V (l sums them unrounded; f16 weights 2^7 times as large, as in
 // attn_tc_kernel), and the result.
@@ -34,11 +39,12 @@ template <typename T>
 struct StepArgs {
     HeadsOf<T> q, o;
     FastDiv size;
-    const int32_t *table, *lens;
+    const int32_t *prefix, *table, *lens;
     const float *part_o, *part_lse;  // the shared part's results, `splits` of them
     int batch, hq, hk, group, d, from, max_len, table_stride, splits;
     int pages, page_size, box_rows;  // places of one box: the greatest common divisor of a page's and a tile's
     int units, zs, rows;             // (stream, key head, 16 heads of the group) triples; rows kept: min(group, 16)
+    int ends_in, split_places;       // streams shorter than this end in the shared part; places of one of its pieces
     int stages;
     int q_pairs;                     // two elements of q are 4-byte aligned
     float scale_log2;
@@ -133,10 +139,18 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         *abort = 1;
         return false;
     };
-    // a unit's tiles of 64 places, this block's part of them
-    auto tiles_of = [&](int b, int &len, int &lo, int &hi) {
+    // a unit's tiles of 64 places, this block's part of them, and the first place:
+    // a.from, or 0 for a stream whose shared part is worked out anew
+    auto tiles_of = [&](int b, int head0, int heads, int &len, int &from, int &lo, int &hi) {
         len = min(max(a.lens[b], 0), a.max_len);
-        const int first = a.from / kStKeys, end = len > a.from ? (len - 1) / kStKeys + 1 : first;
+        from = a.from;
+        if (__builtin_expect(len > 0 && len < a.ends_in, 0)) {
+            // the shared part's word on the piece that the stream ends in
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            const long long row = ((long long)((len - 1) / a.split_places) * a.batch + b) * a.hq + head0 + lane;
+            if (__any_sync(0xffffffffu, lane < heads && isnan(a.part_lse[row]))) from = 0;
+        }
+        const int first = from / kStKeys, end = len > from ? (len - 1) / kStKeys + 1 : first;
         const int per = (end - first + ranks - 1) / ranks;
         lo = min(first + rank * per, end);
         hi = min(lo + per, end);
@@ -151,14 +165,14 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             // the multiplying warps hold the first pair's result back until the shared
             // part is done, however long that takes: no bounded wait runs meanwhile
             if (u != blockIdx.x / ranks && a.splits) asm volatile("griddepcontrol.wait;" ::: "memory");
-            const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk;
-            int len, lo, hi;
-            tiles_of(b, len, lo, hi);
-            const int32_t *row = a.table + (long long)b * a.table_stride;
+            const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk, row0 = u % a.zs * 16;
+            int len, from, lo, hi;
+            tiles_of(b, kvh * a.group + row0, min(a.group - row0, 16), len, from, lo, hi);
+            const int32_t *row = from < a.from ? a.prefix : a.table + (long long)b * a.table_stride;
             auto page_of = [&](int tile) {
                 const int place = tile * kStKeys + lane * a.box_rows;
                 // outside the stream's places, or no page of the cache: one that does not exist, read as zeros
-                const int page = lane < boxes && place < len && place + a.box_rows > a.from ? row[fdiv(place, a.size)] : a.pages;
+                const int page = lane < boxes && place < len && place + a.box_rows > from ? row[fdiv(place, a.size)] : a.pages;
                 return page < 0 || page > a.pages ? a.pages : page;
             };
             int next = lo < hi ? page_of(lo) : 0;
@@ -198,8 +212,8 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     bool first_unit = true;
     for (int u = blockIdx.x / ranks; u < a.units; u += gridDim.x / ranks) {
         const int b = u / (a.hk * a.zs), kvh = u / a.zs % a.hk, row0 = u % a.zs * 16, heads = min(a.group - row0, 16);
-        int len, lo, hi;
-        tiles_of(b, len, lo, hi);
+        int len, from, lo, hi;
+        tiles_of(b, kvh * a.group + row0, heads, len, from, lo, hi);
         // the group's queries, padded to 16 rows, as the A operand
         uint32_t qa[DK / 16][4];
         {
@@ -228,7 +242,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             if (!ok) continue;
             const uint32_t kt = smem_u32(smem + st * Sm::kStage), vt = kt + Sm::kTile;
             const int key0 = warp * 16, place0 = tile * kStKeys + key0;
-            const int skip = a.from - place0, here = len - place0;  // of this warp's 16 places: skip .. here - 1 count
+            const int skip = from - place0, here = len - place0;  // of this warp's 16 places: skip .. here - 1 count
             if (skip < 16 && here > 0) {
                 const bool edge = skip > 0 || here < 16;
                 if (edge) {
@@ -354,7 +368,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         // ---- a row's partial results: the cluster's blocks, then the shared
         // part's pieces.  Their weights first, a warp per row.
         const long long rows = (long long)a.batch * a.hq, prow0 = (long long)b * a.hq + kvh * a.group + row0;
-        const int parts = ranks + a.splits;
+        const int splits = from < a.from ? 0 : a.splits, parts = ranks + splits;
         for (int r = warp; r < heads; r += 4) {
             float top = -INFINITY;
             for (int i = lane; i < parts; i += 32) {
@@ -387,7 +401,7 @@ prefix_step_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             for (int i = 0; i < ranks; i++) add_scaled(x, w[i], ((const float4 *)cluster.map_shared_rank(result, i))[r * (DK / 4) + c]);
             const float4 *po = (const float4 *)(a.part_o + (prow0 + r) * a.d) + c;
 #pragma unroll 8
-            for (int i = 0; i < a.splits; i++) add_scaled(x, w[ranks + i], po[i * rows * quads]);
+            for (int i = 0; i < splits; i++) add_scaled(x, w[ranks + i], po[i * rows * quads]);
             const float f = sh.inv[r];
             T *dst = a.o.at(b, kvh * a.group + row0 + r) + 4 * c;
             dst[0] = from_f32<T>(len > 0 ? x.x * f : 0.f);

@@ -95,6 +95,8 @@ AIE_API int aie_prompt_attn(const aie_prompt *p, void *stream);
  * with lens[b] <= 0 gives zeros; lens above max_len count as max_len.
  * prefix, table and lens are read on the device.  Page numbers outside the
  * cache are never read from; the stream's result is then unspecified.
+ * Places from lens[b] on, infinities and NaN among them, never reach stream
+ * b's result.
  * workspace: aie_prefix_attn_workspace(p) bytes, 16-byte aligned, its
  * contents unspecified before and after; calls that may overlap need one
  * each. */

@@ -28,12 +28,14 @@ def angles(positions: int, rot_dim: int, base: float = 10000.0, device="cuda") -
 
 class StreamDecoder:
     """Layers of x += attention(x) wo over a paged cache.  Row 0 of the cache
-    holds the prompt, rows 1 .. streams the streams forked from it."""
+    holds the prompt, rows 1 .. streams the streams forked from it.  A row
+    holds up to max_len tokens, rounded up to whole pages."""
 
     def __init__(self, layers: int, dim: int, q_heads: int, kv_heads: int, head_dim: int, *, streams: int, pages_: int,
                  page_size: int = 16, max_len: int = 4096, dtype=torch.bfloat16, device="cuda", seed: int = 0):
         self.dim, self.hq, self.hk, self.d = dim, q_heads, kv_heads, head_dim
-        self.page_size, self.max_len, self.dtype, self.device = page_size, max_len, dtype, torch.device(device)
+        width = -(-max_len // page_size)
+        self.page_size, self.max_len, self.dtype, self.device = page_size, width * page_size, dtype, torch.device(device)
         g = torch.Generator(device).manual_seed(seed)
         heads = (q_heads + 2 * kv_heads) * head_dim
 
@@ -42,9 +44,9 @@ class StreamDecoder:
         self.wqkv = [weight(dim, heads) for _ in range(layers)]
         self.wo = [weight(q_heads * head_dim, dim) for _ in range(layers)]
         self.norms = [1.0 + 0.1 * torch.randn(2, head_dim, generator=g, device=device) for _ in range(layers)]
-        self.table = angles(max_len, head_dim, device=device)
+        self.table = angles(self.max_len, head_dim, device=device)
         self.kv = pages.new_cache(layers, pages_, page_size, kv_heads, head_dim, dtype, device)
-        self.state = pages.new_state(pages_, streams + 1, -(-max_len // page_size), device)
+        self.state = pages.new_state(pages_, streams + 1, width, device)
         self.prompt_len = 0
 
     def _int(self, x) -> torch.Tensor:

@@ -47,7 +47,7 @@ class StreamDecoder:
         self.table = angles(self.max_len, head_dim, device=device)
         self.kv = pages.new_cache(layers, pages_, page_size, kv_heads, head_dim, dtype, device)
         self.state = pages.new_state(pages_, streams + 1, width, device)
-        self.prompt_len = 0
+        self.prompt_len, self.live = 0, set()  # rows that hold tokens
 
     def _int(self, x) -> torch.Tensor:
         return torch.as_tensor(x, dtype=torch.int32, device=self.device)
@@ -65,7 +65,10 @@ class StreamDecoder:
         return x + o.reshape(x.shape[0], -1) @ self.wo[i]
 
     def prompt(self, x: torch.Tensor) -> torch.Tensor:
-        """The prompt's features [tokens, dim] through the layers and into row 0."""
+        """The prompt's features [tokens, dim] through the layers and into row 0,
+        which is empty, as all rows are."""
+        if self.prompt_len or self.live:
+            raise ValueError("rows hold a prompt or streams: end them first")
         t = x.shape[0]
         slots = pages.grow(self.state, self.page_size, self._int([0]), self._int([t]), t)
         positions, cu = torch.arange(t, dtype=torch.int32, device=self.device), self._int([0, t])
@@ -77,10 +80,13 @@ class StreamDecoder:
 
     def fork(self, rows: Sequence[int]) -> None:
         """The rows become streams that have seen the prompt."""
+        if self.prompt_len:
+            self.live.update(rows)
         pages.fork(self.kv, self.state, self._int([0] * len(rows)), self._int(list(rows)))
 
     def step(self, rows: Sequence[int], x: torch.Tensor) -> torch.Tensor:
         """One token for each of the rows [rows, dim]."""
+        self.live.update(rows)
         r = self._int(list(rows))
         at = r.long()
         positions = self.state.lens[at]
@@ -93,7 +99,11 @@ class StreamDecoder:
         return x
 
     def end(self, rows: Sequence[int], compact: bool = True) -> None:
-        """The rows' streams end; the pages in use move to the front of the cache."""
+        """The rows' streams end; the pages in use move to the front of the cache.
+        Streams outlive the prompt's row: from then on each goes by its own."""
+        self.live.difference_update(rows)
+        if 0 in rows:
+            self.prompt_len = 0
         pages.free(self.state, self._int(list(rows)))
         if compact:
             pages.compact(self.kv, self.state)

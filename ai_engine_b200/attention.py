@@ -8,7 +8,8 @@ that share the front of their contexts.  ``pages`` keeps the cache.
 Tensors are CUDA tensors ``[tokens, heads, head_dim]`` in float16, bfloat16 or
 float32 with any strides, so long as a head's elements lie side by side.
 Every call runs on the current (or given) CUDA stream and waits for nothing;
-outputs come from that stream's memory.
+outputs come from that stream's memory.  There is no backward pass: where
+gradients are recorded, a tensor that requires one is refused.
 """
 from __future__ import annotations
 

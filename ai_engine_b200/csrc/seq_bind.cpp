@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -86,6 +87,22 @@ int dtype_id(const at::Tensor &t)
     }
 }
 
+// The operators have no backward pass; dropping a gradient without a word would
+// give wrong ones.
+const at::Tensor &no_grad(const at::Tensor &t, const char *name)
+{
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        refuse(PyExc_ValueError, "%s requires a gradient, which this call does not pass on: detach it, or call under "
+                                 "torch.no_grad()", name);
+    return t;
+}
+
+// To autograd, a tensor that a call has written is another one than it saved.
+void written(const at::Tensor &t)
+{
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // What the other tensors of a call have to match.
 struct Like {
     at::ScalarType type;
@@ -110,7 +127,7 @@ void same_kind(const at::Tensor &t, const char *name, const Like &l, int64_t dim
 
 aie_heads heads(const at::Tensor &t, const char *name, const Like &l)
 {
-    same_kind(t, name, l, 3);
+    same_kind(no_grad(t, name), name, l, 3);
     if (t.stride(2) != 1 && t.size(2) != 1)
         refuse(PyExc_ValueError, "%s's heads must be contiguous (stride 1 in the last dimension)", name);
     return {t.data_ptr(), t.stride(0), t.stride(1)};
@@ -121,7 +138,7 @@ void *vector(const at::Tensor &t, const char *name, at::ScalarType type, int dev
     if (t.scalar_type() != type || !t.is_cuda() || t.get_device() != device || t.dim() != dims || !t.is_contiguous())
         refuse(PyExc_TypeError, "%s must be a contiguous %lld-D %s tensor on cuda:%d", name, (long long)dims,
                                c10::toString(type), device);
-    return t.data_ptr();
+    return no_grad(t, name).data_ptr();
 }
 
 void same_shape(const at::Tensor &t, const char *name, const at::Tensor &want, const char *what)
@@ -131,8 +148,8 @@ void same_shape(const at::Tensor &t, const char *name, const at::Tensor &want, c
 
 aie_kv_pages cache(const at::Tensor &k, const at::Tensor &v, const Like &l, int64_t kv_heads, int64_t dim)
 {
-    same_kind(k, "k_pages", l, 4);
-    same_kind(v, "v_pages", l, 4);
+    same_kind(no_grad(k, "k_pages"), "k_pages", l, 4);
+    same_kind(no_grad(v, "v_pages"), "v_pages", l, 4);
     if (k.sizes() != v.sizes() || k.strides() != v.strides())
         refuse(PyExc_ValueError, "k_pages and v_pages must have the same shape and strides");
     if (k.size(2) != kv_heads || k.size(3) != dim)
@@ -235,6 +252,12 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
     p.interleaved = truth(a[7]);
     p.eps = (float)real(a[6]);
     check(aie_qk_norm_rope(&p, on.get()), "aie_qk_norm_rope");
+    if (qo) written(*qo);
+    if (ko) written(*ko);
+    if (kp) {
+        written(*kp);
+        written(*vp);
+    }
     PyObject *r0 = qo ? Py_NewRef(a[12]) : THPVariable_Wrap(q_out);
     PyObject *r1 = ko ? Py_NewRef(a[13]) : keep_k ? THPVariable_Wrap(k_out) : Py_NewRef(Py_None);
     return Py_BuildValue("(NN)", r0, r1);
@@ -270,6 +293,7 @@ PyObject *prompt_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     p.causal = truth(a[4]);
     p.scale = a[5] == Py_None ? 1.f / std::sqrt((float)q.size(2)) : (float)real(a[5]);
     check(aie_prompt_attn(&p, on.get()), "aie_prompt_attn");
+    if (o) written(*o);
     return o ? Py_NewRef(a[6]) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -318,6 +342,7 @@ PyObject *prefix_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     const at::Tensor ws = scratch((int64_t)p.workspace_bytes, at::kByte, l.device);
     p.workspace = ws.data_ptr();
     check(aie_prefix_attn(&p, on.get()), "aie_prefix_attn");
+    if (o) written(*o);
     return o ? Py_NewRef(a[9]) : THPVariable_Wrap(out);
     END_HANDLE_TH_ERRORS
 }
@@ -327,7 +352,7 @@ PyObject *prefix_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
 // kv into p; its device
 int pack_kv(PyObject *o, aie_pages &p)
 {
-    const at::Tensor &kv = tensor(o, "kv");
+    const at::Tensor &kv = no_grad(tensor(o, "kv"), "kv");
     if (dtype_id(kv) < 0 || !kv.is_cuda() || kv.dim() != 6 || kv.size(1) != 2 || !kv.is_contiguous())
         refuse(PyExc_TypeError, "kv must be a contiguous float16, bfloat16 or float32 CUDA tensor "
                                "[layers, 2, pages, page_size, kv_heads, head_dim]");
@@ -360,6 +385,11 @@ int pack_state(PyObject *o, aie_pages &p)
     return device;
 }
 
+void written_state(PyObject *o)
+{
+    for (int i = 0; i < 4; i++) written(THPVariable_Unpack(PyTuple_GET_ITEM(o, i)));
+}
+
 uint32_t lists(PyObject *a, PyObject *b, const char *what, int device, const int32_t **x, const int32_t **y)
 {
     const at::Tensor &s = tensor(a, what), &t = tensor(b, what);
@@ -389,6 +419,7 @@ PyObject *pages_grow(PyObject *, PyObject *const *a, Py_ssize_t n)
     OnStream on(a[5], device);
     const at::Tensor ws = page_scratch(p, count, device), slots = scratch(tokens, at::kLong, device);
     check(aie_pages_grow(&p, rows, counts, count, (int64_t *)slots.data_ptr(), tokens, on.get()), "aie_pages_grow");
+    written_state(a[0]);
     return THPVariable_Wrap(slots);
     END_HANDLE_TH_ERRORS
 }
@@ -406,6 +437,8 @@ PyObject *pages_fork(PyObject *, PyObject *const *a, Py_ssize_t n)
     OnStream on(a[4], device);
     const at::Tensor ws = page_scratch(p, count, device);
     check(aie_pages_fork(&p, src, dst, count, on.get()), "aie_pages_fork");
+    written(THPVariable_Unpack(a[0]));
+    written_state(a[1]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -421,6 +454,7 @@ PyObject *pages_copy(PyObject *, PyObject *const *a, Py_ssize_t n)
     const uint32_t count = lists(a[1], a[2], "src and dst", device, &src, &dst);
     OnStream on(a[3], device);
     check(aie_pages_copy(&p, src, dst, count, on.get()), "aie_pages_copy");
+    written(THPVariable_Unpack(a[0]));
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -436,6 +470,7 @@ PyObject *pages_free(PyObject *, PyObject *const *a, Py_ssize_t n)
     const int32_t *list = (const int32_t *)vector(rows, "rows", at::kInt, device);
     OnStream on(a[2], device);
     check(aie_pages_free(&p, list, u32(rows.size(0), "rows"), on.get()), "aie_pages_free");
+    written_state(a[0]);
     Py_RETURN_NONE;
     END_HANDLE_TH_ERRORS
 }
@@ -451,6 +486,8 @@ PyObject *pages_compact(PyObject *, PyObject *const *a, Py_ssize_t n)
     OnStream on(a[2], device);
     const at::Tensor ws = page_scratch(p, 0, device), remap = scratch(p.pages, at::kInt, device);
     check(aie_pages_compact(&p, (int32_t *)remap.data_ptr(), on.get()), "aie_pages_compact");
+    written(THPVariable_Unpack(a[0]));
+    written_state(a[1]);
     return THPVariable_Wrap(remap);
     END_HANDLE_TH_ERRORS
 }

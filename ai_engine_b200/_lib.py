@@ -122,6 +122,7 @@ SEQ_SIGNATURES = {
     "aie_pages_copy": (C.c_int, [_bp, _vp, _vp, C.c_uint32, _vp]),
     "aie_pages_free": (C.c_int, [_bp, _vp, C.c_uint32, _vp]),
     "aie_pages_compact": (C.c_int, [_bp, _vp, _vp]),
+    "aie_seq_selftest_wait_timeout": (C.c_int, [C.c_uint32, _vp]),
 }
 
 _LIB = None

@@ -1331,7 +1331,7 @@ extern "C" int aie_concat(uint32_t n, uint32_t px, uint32_t nparts, const aie_tv
 extern "C" int aie_selftest_wait_timeout(uint32_t timeout_us, void *stream)
 {
     if (timeout_us == 0 || timeout_us > 2000000) return fail(AIE_E_INVALID, "timeout must be 1..2000000 us");
-    selftest_wait_kernel<<<1, 32, 0, (cudaStream_t)stream>>>((unsigned long long)timeout_us * 1000ull);
+    selftest_wait_kernel<<<1, 32, 0, (cudaStream_t)stream>>>((unsigned long long)timeout_us * 1000ull, kSelftestCode);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_fail(e, "selftest launch");
     return AIE_OK;
@@ -1343,9 +1343,8 @@ extern "C" int aie_device_status(void *stream, uint32_t *code_out)
     uint32_t v = 0, zero = 0;
     CUDA_TRY(cudaMemcpyFromSymbol(&v, g_aie_error, sizeof v));
     if (v) CUDA_TRY(cudaMemcpyToSymbol(g_aie_error, &zero, sizeof zero));
-    uint32_t vs = 0;
-    CUDA_TRY(seq_take_device_error(&vs));
-    if (!v) v = vs;
+    // one code a call: the other translation unit's stays for the next
+    if (!v) CUDA_TRY(seq_take_device_error(&v));
     if (code_out) *code_out = v;
     if (v) return fail(AIE_E_DEVICE_TIMEOUT, "device wait gave up, code 0x%08x", v);
     return AIE_OK;

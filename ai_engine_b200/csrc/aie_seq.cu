@@ -33,6 +33,14 @@ cudaError_t aie::seq_take_device_error(uint32_t *code)
     return e;
 }
 
+extern "C" int aie_seq_selftest_wait_timeout(uint32_t timeout_us, void *stream)
+{
+    if (timeout_us == 0 || timeout_us > 2000000) return fail(AIE_E_INVALID, "timeout must be 1..2000000 us");
+    selftest_wait_kernel<<<1, 32, 0, (cudaStream_t)stream>>>((unsigned long long)timeout_us * 1000ull, kSeqSelftestCode);
+    cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? AIE_OK : cuda_fail(e, "selftest launch");
+}
+
 // ------------------------------------------------------------- checks ---
 
 static int launched(cudaError_t e, const char *what)

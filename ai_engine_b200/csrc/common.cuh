@@ -361,6 +361,22 @@ static __device__ uint32_t g_aie_error = 0;
 
 __device__ __forceinline__ void report_error(uint32_t code) { atomicCAS(&g_aie_error, 0u, code); }
 
+// Self-test of the bounded-wait path: one thread waits on an mbarrier that
+// nothing ever arrives at.  The wait gives up after `limit_ns`, records `code`
+// in the device error word and the kernel returns normally -- the same path
+// every role of the tensor-core kernels takes when a wait expires.
+constexpr uint32_t kSelftestCode = 0x7F000001u, kSeqSelftestCode = 0x7F000002u;
+
+static __global__ void selftest_wait_kernel(unsigned long long limit_ns, uint32_t code)
+{
+    __shared__ __align__(8) uint64_t bar;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (!mbar_wait_for(&bar, 0, limit_ns)) report_error(code);
+    }
+}
+
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize, and the shared-memory
 // carveout when asked) once per kernel and device: the attributes belong to
 // the function in each device's context

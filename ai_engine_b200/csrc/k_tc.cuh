@@ -171,22 +171,6 @@ __device__ __forceinline__ Up2Patch up2_patch(const ConvArgs &c, int m0)
 
 // --------------------------------------------------------------- PTX ---
 
-// Self-test of the bounded-wait path: one thread waits on an mbarrier that
-// nothing ever arrives at.  The wait gives up after `limit_ns`, records
-// kSelftestCode in the device error word and the kernel returns normally --
-// the same path every role of tc_conv_kernel takes when a wait expires.
-constexpr uint32_t kSelftestCode = 0x7F000001u;
-
-__global__ void selftest_wait_kernel(unsigned long long limit_ns)
-{
-    __shared__ __align__(8) uint64_t bar;
-    if (threadIdx.x == 0) {
-        mbar_init(&bar, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (!mbar_wait_for(&bar, 0, limit_ns)) report_error(kSelftestCode);
-    }
-}
-
 // The same for 16-channel K blocks (64-byte rows, 64-byte swizzle: 8-row
 // groups 512 bytes apart), and the descriptor of a K block of BK channels.
 __device__ __forceinline__ uint64_t smem_desc_sw64(uint32_t saddr)

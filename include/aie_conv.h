@@ -448,7 +448,9 @@ AIE_API int aie_selftest_wait_timeout(uint32_t timeout_us, void *stream);
 
 /* Read and clear the device error word that bounded device-side waits set
  * when they give up (synchronises `stream`).  AIE_OK or
- * AIE_E_DEVICE_TIMEOUT; *code_out (nullable) receives the raw word. */
+ * AIE_E_DEVICE_TIMEOUT; *code_out (nullable) receives the raw word.  The conv
+ * path and the sequence operators (aie_seq.h) have a word each; where both are
+ * set, a call reports the first and the next call the second. */
 AIE_API int aie_device_status(void *stream, uint32_t *code_out);
 
 #ifdef __cplusplus

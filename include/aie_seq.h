@@ -161,6 +161,10 @@ AIE_API int aie_pages_free(const aie_pages *p, const int32_t *rows, uint32_t n, 
  * ([pages]) receives each page's new number, -1 for a free one. */
 AIE_API int aie_pages_compact(const aie_pages *p, int32_t *remap, void *stream);
 
+/* aie_selftest_wait_timeout for these operators: a wait that gives up after
+ * timeout_us (1..2e6) and records its code, which aie_device_status reports. */
+AIE_API int aie_seq_selftest_wait_timeout(uint32_t timeout_us, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -4,17 +4,22 @@ Two translation units, compiled for sm_100a only and side by side: the conv
 path (``csrc/aie_conv.cu``, which includes the ``k_*.cuh`` kernels) and the
 sequence operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels).  Beside
 it ``_seqcall.so``, the sequence operators' binding on torch tensors
-(``csrc/seq_bind.cpp``), which is linked against it.  The CUDA runtime is linked statically, so the
-library depends on nothing but the driver; the tensor-map encoder is fetched
-from the driver at run time.
+(``csrc/seq_bind.cpp``), which is linked against it; where torch or Python's
+headers are missing it is left out, with a message (the C ABI needs neither).
+The CUDA runtime is linked statically, so the library depends on nothing but
+the driver; the tensor-map encoder is fetched from the driver at run time.
+
+    python ai_engine_b200/build.py [-v] [--changed]     # needs nvcc alone
 """
 from __future__ import annotations
 
 import glob
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -64,9 +69,16 @@ def _bind_sources():
     return [BIND_SRC, *(os.path.join(ROOT, "include", h) for h in ("aie_conv.h", "aie_seq.h"))]
 
 
-def _bind_command(out: str):
-    import sysconfig
+def bind_needs() -> str:
+    """What the binding needs and this machine lacks."""
+    if importlib.util.find_spec("torch") is None:
+        return "torch"
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        return "Python's headers"
+    return ""
 
+
+def _bind_command(out: str):
     import torch
     from torch.utils import cpp_extension
     inc = [f for d in (sysconfig.get_paths()["include"], *cpp_extension.include_paths("cuda")) for f in ("-isystem", d)]
@@ -100,8 +112,12 @@ def build(force: bool = False, verbose: bool = False, extra=()) -> str:
         subprocess.run([nvcc(), *NVCC_FLAGS, "-shared", *objs, "-o", LIB + tmp], check=True)
         os.replace(LIB + tmp, LIB)
     if force or _older(BIND, _bind_sources()):
-        subprocess.run(_bind_command(BIND + tmp), check=True)
-        os.replace(BIND + tmp, BIND)
+        lacks = bind_needs()
+        if lacks:
+            print(f"{BIND} is left out: {lacks} not found", file=sys.stderr)
+        else:
+            subprocess.run(_bind_command(BIND + tmp), check=True)
+            os.replace(BIND + tmp, BIND)
     return LIB
 
 

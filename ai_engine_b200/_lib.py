@@ -100,8 +100,9 @@ SIGNATURES = {
     "aie_conv_run_parts": (C.c_int, [_vp, C.POINTER(TView), _vp, _vp, _vp, _vp, _vp, _vp]),
 }
 
-# The argument structs of include/aie_seq.h, packed in one go: pointers and
-# strides (q), sizes (I), flags (i) and floats (f) in the header's order.
+# The argument structs of include/aie_seq.h for callers of the C ABI through
+# ctypes (the package's own calls go through seqcall): pointers and strides (q),
+# sizes (I), flags (i) and floats (f) in the header's order.
 QK_ROPE = struct.Struct("@15q5q2I5q6I2ifI")   # q k v q_out k_out, pages, weights cos_sin positions slots, ...
 PROMPT = struct.Struct("@12qq5I2if")          # q k v out, cu, ...
 PREFIX = struct.Struct("@6q5q2I3qqQ7IifI")    # q out, pages, prefix table lens, workspace, ...

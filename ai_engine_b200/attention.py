@@ -48,7 +48,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     s is tokens cu[s] .. cu[s + 1] of q [tokens, heads, head_dim] and of k, v
     [tokens, kv_heads, head_dim]; with causal a token sees its sequence up to
     itself.  cu is an int32 CUDA tensor [sequences + 1]; it is not copied to
-    the host.  scale defaults to head_dim ** -0.5."""
+    the host.  scale defaults to head_dim ** -0.5.  Tokens of no sequence are
+    left as they are in out, undefined without it.  With causal, a NaN or
+    infinity in v may reach earlier tokens of its sequence too."""
     return _lib.seqcall().prompt_attention(q, k, v, cu, causal, scale, out, stream)
 
 
@@ -61,6 +63,7 @@ def prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tens
     pages ``prefix`` (int32, in order) and are read once for all streams; the
     rest in its own pages, table[b, place // page_size].  As pages.fork leaves
     them, ``prefix`` is any stream's row.  A stream without places gives
-    zeros.  max_len bounds lens (default: what a table row holds); longer
-    streams are cut off there."""
+    zeros; what stands behind a stream's places, NaN and infinities too, never
+    reaches its result.  max_len bounds lens (default: what a table row
+    holds); longer streams are cut off there."""
     return _lib.seqcall().prefix_attention(q, k_pages, v_pages, prefix, prefix_len, table, lens, max_len, scale, out, stream)

@@ -20,7 +20,7 @@
 
 using namespace aie;
 
-// the sizes that the Python layer packs (ai_engine_b200/_lib.py)
+// the sizes that C callers and _lib.py's packed layouts go by
 static_assert(sizeof(aie_qk_rope) == 248 && sizeof(aie_prompt) == 136 && sizeof(aie_prefix) == 176 &&
                   sizeof(aie_pages) == 80,
               "argument layouts");

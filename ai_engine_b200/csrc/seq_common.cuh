@@ -61,6 +61,14 @@ static inline PagesGeom pages_geom(const aie_kv_pages &p)
 // touched before this, which waits for that one's end, and only then lets the
 // launch behind this one be set up.  Back to back, a frame's prompt took 10.25
 // us a call without, of which the kernel is 8.7 us.
+//
+// One exception: with a shared part, prefix_step_kernel reads a call's inputs
+// (lengths, table, queries, the cache's pages) before its wait, and only the
+// shared part's results and its own output after it.  That is right because it
+// stands directly behind attn_tc_kernel in the stream, all of whose blocks have
+// waited for whatever wrote those inputs before they let it start.  Neither may
+// change: no launch between the two, and attn_tc_kernel's wait ahead of its
+// launch_dependents.
 __device__ __forceinline__ void behind_last_launch()
 {
     asm volatile("griddepcontrol.wait;" ::: "memory");

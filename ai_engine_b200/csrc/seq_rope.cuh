@@ -173,9 +173,11 @@ __device__ __forceinline__ void load8f(const float *p, float *f)
 // HPT heads of the token, whose loads are all in flight at once.
 //
 // Bound by memory: 16384 tokens of 32 + 8 heads of 128 with keys and values
-// filed take 86 us, 444 MB at 5.2 TB/s.  Measured there: 5 blocks an SM (96
-// registers) 86 us, 4 89, 6 (80 registers, some spilled) 93; 2 heads a lane
-// 101; blocks of 256 threads 99.
+// filed take 87 us, 444 MB at 5.1 TB/s.  Measured there: 5 blocks an SM (96
+// registers) 86 us, 4 89, 6 (80 registers) 93; 2 heads a lane 101; blocks of 256
+// threads 99.  At 5 blocks the four-heads form spills 20 to 36 bytes a thread in
+// 16 bits.  In f32, where the heads alone take 64 registers, it spills 108 to
+// 164: the same tokens take 187 us, 881 MB at 4.7 TB/s.
 constexpr int kRopeThreads = 128, kRopeBlocks = 5;
 struct RopeVec {
     unsigned q_units, k_units;  // groups of HPT heads of a token

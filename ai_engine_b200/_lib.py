@@ -107,6 +107,9 @@ QK_ROPE = struct.Struct("@15q5q2I5q6I2ifI")   # q k v q_out k_out, pages, weight
 PROMPT = struct.Struct("@12qq5I2if")          # q k v out, cu, ...
 PREFIX = struct.Struct("@6q5q2I3qqQ7IifI")    # q out, pages, prefix table lens, workspace, ...
 PAGES = struct.Struct("@6qQ6I")               # kv refs lens table status workspace, page_bytes, ...
+CROSS = struct.Struct("@15qQ6Iif")            # q k v out, cu_q cu_k workspace, bytes, ...
+KV4_ROWS = struct.Struct("@3q4I7qIi")         # cache, k v, slots, tokens, dtype
+KV4_STEP = struct.Struct("@3q4I9qQ4Iif")      # cache, q out, table lens workspace, bytes, ...
 DT_F32, DT_F16, DT_BF16 = 0, 1, 2             # aie_dtype
 PAGES_FULL, PAGES_BAD_ROW = 1, 2              # aie_pages_status
 
@@ -114,7 +117,14 @@ PAGES_FULL, PAGES_BAD_ROW = 1, 2              # aie_pages_status
 _bp = C.c_char_p
 SEQ_SIGNATURES = {
     "aie_qk_norm_rope": (C.c_int, [_bp, _vp]),
+    "aie_qk_norm_rope_axes": (C.c_int, [_bp, _vp, C.c_uint32, _vp]),
     "aie_prompt_attn": (C.c_int, [_bp, _vp]),
+    "aie_cross_attn": (C.c_int, [_bp, _vp]),
+    "aie_cross_attn_workspace": (C.c_uint64, [_bp]),
+    "aie_kv4_file": (C.c_int, [_bp, _vp]),
+    "aie_kv4_load": (C.c_int, [_bp, _vp]),
+    "aie_kv4_attn": (C.c_int, [_bp, _vp]),
+    "aie_kv4_attn_workspace": (C.c_uint64, [_bp]),
     "aie_prefix_attn": (C.c_int, [_bp, _vp]),
     "aie_prefix_attn_workspace": (C.c_uint64, [_bp]),
     "aie_pages_workspace": (C.c_uint64, [C.c_uint32, C.c_uint32]),

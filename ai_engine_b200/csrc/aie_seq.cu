@@ -13,6 +13,7 @@
 #include "tc_ptx.cuh"
 #include "seq_common.cuh"
 #include "seq_attn.cuh"
+#include "seq_kv4.cuh"
 #include "seq_pages.cuh"
 #include "seq_rope.cuh"
 #include "seq_rows.cuh"
@@ -22,7 +23,7 @@ using namespace aie;
 
 // the sizes that C callers and _lib.py's packed layouts go by
 static_assert(sizeof(aie_qk_rope) == 248 && sizeof(aie_prompt) == 136 && sizeof(aie_prefix) == 176 &&
-                  sizeof(aie_pages) == 80,
+                  sizeof(aie_pages) == 80 && sizeof(aie_cross) == 160 && sizeof(aie_kv4_rows) == 104 && sizeof(aie_kv4_step) == 144,
               "argument layouts");
 
 cudaError_t aie::seq_take_device_error(uint32_t *code)
@@ -94,7 +95,7 @@ static int check_pages(const aie_kv_pages &p, int32_t dt)
 // ------------------------------------------------------ norm, rotation ---
 
 template <typename T>
-static int qk_norm_rope(const aie_qk_rope &p, cudaStream_t s)
+static int qk_norm_rope(const aie_qk_rope &p, const uint8_t *pair_axis, uint32_t axes, cudaStream_t s)
 {
     RopeArgs<T> a;
     a.q = heads_of<T>(p.q); a.k = heads_of<T>(p.k); a.v = heads_of<T>(p.v);
@@ -106,10 +107,12 @@ static int qk_norm_rope(const aie_qk_rope &p, cudaStream_t s)
     a.tokens = (int)p.tokens; a.hq = p.q.data ? (int)p.q_heads : 0; a.hk = (int)p.kv_heads;
     a.d = (int)p.head_dim; a.rot = (int)p.rot_dim; a.max_pos = (int)p.max_pos; a.interleaved = p.interleaved != 0;
     a.eps = p.eps;
+    a.axis = p.rot_dim ? pair_axis : nullptr; a.axes = (int)axes;
     return launched(rope_launch(a, s), "norm and rotation");
 }
 
-extern "C" int aie_qk_norm_rope(const aie_qk_rope *p, void *stream)
+// pair_axis NULL: one position a token
+static int qk_norm_rope(const aie_qk_rope *p, const uint8_t *pair_axis, uint32_t axes, void *stream)
 {
     if (!p) return fail(AIE_E_INVALID, "null arguments");
     TRY(check_dtype(p->dtype));
@@ -133,8 +136,17 @@ extern "C" int aie_qk_norm_rope(const aie_qk_rope *p, void *stream)
     if ((uint64_t)p->tokens * (p->q_heads + 2 * p->kv_heads) > 0x1ffffffffull)
         return fail(AIE_E_UNSUPPORTED, "more than 2^33 heads in one call");
     cudaStream_t s = (cudaStream_t)stream;
-    if (p->dtype == AIE_DT_F32) return qk_norm_rope<float>(*p, s);
-    return p->dtype == AIE_DT_F16 ? qk_norm_rope<__half>(*p, s) : qk_norm_rope<__nv_bfloat16>(*p, s);
+    if (p->dtype == AIE_DT_F32) return qk_norm_rope<float>(*p, pair_axis, axes, s);
+    return p->dtype == AIE_DT_F16 ? qk_norm_rope<__half>(*p, pair_axis, axes, s) : qk_norm_rope<__nv_bfloat16>(*p, pair_axis, axes, s);
+}
+
+extern "C" int aie_qk_norm_rope(const aie_qk_rope *p, void *stream) { return qk_norm_rope(p, nullptr, 1, stream); }
+
+extern "C" int aie_qk_norm_rope_axes(const aie_qk_rope *p, const uint8_t *pair_axis, uint32_t axes, void *stream)
+{
+    if (!axes || axes > 255) return fail(AIE_E_INVALID, "%u axes: 1 to 255", axes);
+    if (!pair_axis && p && p->rot_dim) return fail(AIE_E_INVALID, "pair_axis is NULL");
+    return qk_norm_rope(p, pair_axis, axes, stream);
 }
 
 // ---------------------------------------------------- prompt attention ---
@@ -412,6 +424,140 @@ extern "C" int aie_prefix_attn(const aie_prefix *p, void *stream)
     }
     if (p->dtype == AIE_DT_F32) return prefix_rows<float>(*p, s);
     return p->dtype == AIE_DT_F16 ? prefix_rows<__half>(*p, s) : prefix_rows<__nv_bfloat16>(*p, s);
+}
+
+// ----------------------------------------------------- cross attention ---
+
+static int check_cross(const aie_cross *p)
+{
+    if (!p) return fail(AIE_E_INVALID, "null arguments");
+    TRY(check_dtype(p->dtype));
+    TRY(check_group(p->q_heads, p->kv_heads, p->head_dim, kRowsMaxDim));
+    if (p->tokens > 0x3fffffffu || p->keys > 0x3fffffffu || p->seqs > 0x3fffffffu)
+        return fail(AIE_E_INVALID, "too many tokens, states or sequences");
+    if (!p->cu_q && p->tokens != p->seqs) return fail(AIE_E_INVALID, "%u tokens of %u sequences without cu_q", p->tokens, p->seqs);
+    if ((uint64_t)p->tokens * p->q_heads > 0x1ffffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^33 query rows");
+    return AIE_OK;
+}
+
+extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p) { return check_cross(p) ? 0 : 64; }
+
+template <typename T>
+static int cross_rows(const aie_cross &p, cudaStream_t s)
+{
+    CrossRows<T> a;
+    a.q = heads_of<T>(p.q); a.k = heads_of<T>(p.k); a.v = heads_of<T>(p.v); a.o = heads_of<T>(p.out);
+    a.cu_q = p.cu_q; a.cu_k = p.cu_k;
+    a.tokens = (int)p.tokens; a.keys = (int)p.keys; a.seqs = (int)p.seqs;
+    a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
+    a.scale = p.scale;
+    const long long rows = (long long)p.tokens * p.q_heads;
+    return launched(launch_behind(cross_rows_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "cross attention");
+}
+
+extern "C" int aie_cross_attn(const aie_cross *p, void *stream)
+{
+    TRY(check_cross(p));
+    if (!(p->scale == p->scale)) return fail(AIE_E_INVALID, "scale is NaN");
+    if (!p->tokens || !p->seqs) return AIE_OK;
+    if (!p->cu_k) return fail(AIE_E_INVALID, "cu_k is NULL");
+    TRY(check_heads(p->q, p->dtype, "q"));
+    TRY(check_heads(p->out, p->dtype, "out"));
+    if (p->keys) {
+        TRY(check_heads(p->k, p->dtype, "k"));
+        TRY(check_heads(p->v, p->dtype, "v"));
+    }
+    const uint64_t need = aie_cross_attn_workspace(p);
+    if (p->workspace_bytes < need || !p->workspace || (uintptr_t)p->workspace % 16)
+        return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
+    cudaStream_t s = (cudaStream_t)stream;
+    if (p->dtype == AIE_DT_F32) return cross_rows<float>(*p, s);
+    return p->dtype == AIE_DT_F16 ? cross_rows<__half>(*p, s) : cross_rows<__nv_bfloat16>(*p, s);
+}
+
+// ---------------------------------------------------------- 4-bit cache ---
+
+static int check_kv4(const aie_kv4 &c)
+{
+    if (!c.k || !c.v) return fail(AIE_E_INVALID, "the cache's k or v is NULL");
+    if (!c.head_dim || c.head_dim % 32) return fail(AIE_E_INVALID, "head_dim %u: a multiple of 32", c.head_dim);
+    if (c.head_dim > 256) return fail(AIE_E_UNSUPPORTED, "head_dim %u: at most 256", c.head_dim);
+    if (!c.kv_heads) return fail(AIE_E_INVALID, "no key heads");
+    if (c.kv_heads > 4096) return fail(AIE_E_UNSUPPORTED, "%u key heads: at most 4096", c.kv_heads);
+    if (!c.pages || !c.page_size || c.page_size % 8 || c.pages > 0x3fffffffu || c.page_size > 65536)
+        return fail(AIE_E_INVALID, "a cache of %u pages of %u places (a multiple of 8)", c.pages, c.page_size);
+    const int64_t page = (int64_t)c.kv_heads * c.page_size * c.head_dim * 5 / 8;
+    if (c.page_stride < 0 || (c.pages > 1 && c.page_stride < page))
+        return fail(AIE_E_INVALID, "page_stride %lld for pages of %lld bytes", (long long)c.page_stride, (long long)page);
+    if ((uintptr_t)c.k % 16 || (uintptr_t)c.v % 16 || c.page_stride % 16)
+        return fail(AIE_E_ALIGN, "the cache and its pages must be 16-byte aligned");
+    return AIE_OK;
+}
+
+static int kv4_rows(const aie_kv4_rows *p, bool file, void *stream)
+{
+    if (!p) return fail(AIE_E_INVALID, "null arguments");
+    TRY(check_dtype(p->dtype));
+    TRY(check_kv4(p->cache));
+    if (!p->tokens) return AIE_OK;
+    TRY(check_heads(p->k, p->dtype, "k"));
+    TRY(check_heads(p->v, p->dtype, "v"));
+    if (!p->slots) return fail(AIE_E_INVALID, "slots is NULL");
+    if ((uint64_t)p->tokens * p->cache.kv_heads * (p->cache.head_dim / 8) > 0x7fffff00ull)
+        return fail(AIE_E_UNSUPPORTED, "more than 2^34 elements in one call");
+    cudaStream_t s = (cudaStream_t)stream;
+    const char *what = file ? "filing in 4 bits" : "reading 4 bits";
+    if (p->dtype == AIE_DT_F32) return launched(kv4_rows_launch<float>(*p, file, s), what);
+    return launched(p->dtype == AIE_DT_F16 ? kv4_rows_launch<__half>(*p, file, s) : kv4_rows_launch<__nv_bfloat16>(*p, file, s), what);
+}
+
+extern "C" int aie_kv4_file(const aie_kv4_rows *p, void *stream) { return kv4_rows(p, true, stream); }
+extern "C" int aie_kv4_load(const aie_kv4_rows *p, void *stream) { return kv4_rows(p, false, stream); }
+
+static int check_kv4_step(const aie_kv4_step *p)
+{
+    if (!p) return fail(AIE_E_INVALID, "null arguments");
+    if (p->dtype != AIE_DT_F16 && p->dtype != AIE_DT_BF16) return fail(AIE_E_UNSUPPORTED, "dtype %d: f16 or bf16", p->dtype);
+    TRY(check_kv4(p->cache));
+    TRY(check_group(p->q_heads, p->cache.kv_heads, p->cache.head_dim, 256));
+    if (p->batch > 65535) return fail(AIE_E_UNSUPPORTED, "%u streams: at most 65535", p->batch);
+    if (p->max_len > 0x3fffffffu) return fail(AIE_E_INVALID, "too many places");
+    return AIE_OK;
+}
+
+extern "C" uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p) { return check_kv4_step(p) ? 0 : 64; }
+
+template <typename T>
+static int kv4_step(const aie_kv4_step &p, cudaStream_t s)
+{
+    Kv4Step<T> a;
+    a.g = kv4_geom(p.cache);
+    a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
+    a.table = p.table; a.lens = p.lens;
+    a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads);
+    a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
+    a.scale = p.scale;
+    const long long rows = (long long)p.batch * p.q_heads;
+    return launched(launch_behind(kv4_step_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "attention over 4 bits");
+}
+
+extern "C" int aie_kv4_attn(const aie_kv4_step *p, void *stream)
+{
+    TRY(check_kv4_step(p));
+    if (!(p->scale == p->scale)) return fail(AIE_E_INVALID, "scale is NaN");
+    if (!p->batch) return AIE_OK;
+    TRY(check_heads(p->q, p->dtype, "q"));
+    TRY(check_heads(p->out, p->dtype, "out"));
+    if (!p->lens) return fail(AIE_E_INVALID, "lens is NULL");
+    if (p->max_len) {
+        if (!p->table) return fail(AIE_E_INVALID, "table is NULL");
+        if ((uint64_t)p->table_stride * p->cache.page_size < p->max_len)
+            return fail(AIE_E_INVALID, "rows of %u pages of %u do not hold max_len %u", p->table_stride, p->cache.page_size, p->max_len);
+    }
+    const uint64_t need = aie_kv4_attn_workspace(p);
+    if (p->workspace_bytes < need || !p->workspace || (uintptr_t)p->workspace % 16)
+        return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
+    return p->dtype == AIE_DT_F16 ? kv4_step<__half>(*p, (cudaStream_t)stream) : kv4_step<__nv_bfloat16>(*p, (cudaStream_t)stream);
 }
 
 // --------------------------------------------------------------- pages ---

@@ -12,6 +12,7 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -200,11 +201,11 @@ void arguments(Py_ssize_t got, Py_ssize_t want)
     if (got != want) refuse(PyExc_TypeError, "%lld arguments, not %lld", (long long)want, (long long)got);
 }
 
-// q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_pages, v_pages, slots, q_out, k_out, stream
+// q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_pages, v_pages, slots, q_out, k_out, stream, pair_axis
 PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
 {
     HANDLE_TH_ERRORS
-    arguments(n, 15);
+    arguments(n, 16);
     const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &pos = tensor(a[2], "positions"), &cs = tensor(a[3], "cos_sin");
     const Like l = first_heads(q, "q");
     aie_qk_rope p = {};
@@ -212,8 +213,15 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
     p.k = heads(k, "k", l);
     const int64_t tokens = q.size(0), d = q.size(2);
     if (k.size(0) != tokens || k.size(2) != d) refuse(PyExc_ValueError, "q and k differ in tokens or head_dim");
-    p.positions = (const int32_t *)vector(pos, "positions", at::kInt, l.device);
+    const at::Tensor *axis = optional(a[15], "pair_axis");
+    p.positions = (const int32_t *)vector(pos, "positions", at::kInt, l.device, axis ? 2 : 1);
     p.cos_sin = (const float *)vector(cs, "cos_sin", at::kFloat, l.device, 2);
+    const uint8_t *pair_axis = nullptr;
+    if (axis) {
+        pair_axis = (const uint8_t *)vector(*axis, "pair_axis", at::kByte, l.device);
+        if (axis->size(0) * 2 != cs.size(1))
+            refuse(PyExc_ValueError, "%lld axes of pairs for angles of %lld elements", (long long)axis->size(0), (long long)cs.size(1));
+    }
     if (pos.size(0) != tokens) refuse(PyExc_ValueError, "%lld positions for %lld tokens", (long long)pos.size(0), (long long)tokens);
     for (int i = 0; i < 2; i++)
         if (const at::Tensor *w = optional(a[4 + i], "a weight")) {
@@ -251,7 +259,8 @@ PyObject *qk_norm_rope(PyObject *, PyObject *const *a, Py_ssize_t n)
     p.dtype = l.dtype;
     p.interleaved = truth(a[7]);
     p.eps = (float)real(a[6]);
-    check(aie_qk_norm_rope(&p, on.get()), "aie_qk_norm_rope");
+    if (axis) check(aie_qk_norm_rope_axes(&p, pair_axis, u32(pos.size(1), "axes"), on.get()), "aie_qk_norm_rope_axes");
+    else check(aie_qk_norm_rope(&p, on.get()), "aie_qk_norm_rope");
     if (qo) written(*qo);
     if (ko) written(*ko);
     if (kp) {
@@ -347,19 +356,184 @@ PyObject *prefix_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
     END_HANDLE_TH_ERRORS
 }
 
+// q, k, v, cu_k, cu_q, scale, out, stream
+PyObject *cross_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    arguments(n, 8);
+    const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &v = tensor(a[2], "v"), &cu_k = tensor(a[3], "cu_k");
+    const Like l = first_heads(q, "q");
+    aie_cross p = {};
+    p.q = heads(q, "q", l);
+    p.k = heads(k, "k", l);
+    p.v = heads(v, "v", l);
+    if (k.size(2) != q.size(2)) refuse(PyExc_ValueError, "q and k differ in head_dim");
+    same_shape(v, "v", k, "k");
+    p.cu_k = (const int32_t *)vector(cu_k, "cu_k", at::kInt, l.device);
+    if (cu_k.size(0) < 1) refuse(PyExc_ValueError, "cu_k holds at least one entry");
+    const int64_t seqs = cu_k.size(0) - 1;
+    if (const at::Tensor *cu_q = optional(a[4], "cu_q")) {
+        p.cu_q = (const int32_t *)vector(*cu_q, "cu_q", at::kInt, l.device);
+        if (cu_q->size(0) != seqs + 1)
+            refuse(PyExc_ValueError, "cu_q and cu_k differ in length: %lld and %lld", (long long)cu_q->size(0), (long long)seqs + 1);
+    } else if (q.size(0) != seqs)
+        refuse(PyExc_ValueError, "%lld tokens for %lld sequences: without cu_q each has one", (long long)q.size(0), (long long)seqs);
+    const at::Tensor *o = optional(a[6], "out");
+    OnStream on(a[7], l.device);
+    const at::Tensor out = o ? *o : fresh_like(q);
+    same_shape(out, "out", q, "q");
+    p.out = heads(out, "out", l);
+    p.tokens = u32(q.size(0), "tokens");
+    p.keys = u32(k.size(0), "states");
+    p.seqs = u32(seqs, "sequences");
+    p.q_heads = u32(q.size(1), "q's heads");
+    p.kv_heads = u32(k.size(1), "k's heads");
+    p.head_dim = u32(q.size(2), "head_dim");
+    p.dtype = l.dtype;
+    p.scale = a[5] == Py_None ? 1.f / std::sqrt((float)q.size(2)) : (float)real(a[5]);
+    p.workspace_bytes = std::max<uint64_t>(aie_cross_attn_workspace(&p), 16);
+    const at::Tensor ws = scratch((int64_t)p.workspace_bytes, at::kByte, l.device);
+    p.workspace = ws.data_ptr();
+    check(aie_cross_attn(&p, on.get()), "aie_cross_attn");
+    if (o) written(*o);
+    return o ? Py_NewRef(a[6]) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- the 4-bit cache
+
+// k_pages or v_pages: [pages, kv_heads, page_size, head_dim * 5 / 8] bytes, a page's side by side
+void check_kv4(const at::Tensor &t, const char *name, int device)
+{
+    if (t.scalar_type() != at::kByte || !t.is_cuda() || t.dim() != 4 || (device >= 0 && t.get_device() != device))
+        refuse(PyExc_TypeError, "%s must be a uint8 CUDA tensor [pages, kv_heads, page_size, head_dim * 5 / 8]", name);
+    const int64_t row = t.size(3), block = t.size(2) * row;
+    if (row == 0 || row % 20 || t.stride(3) != 1 || t.stride(2) != row || (t.size(1) > 1 && t.stride(1) != block))
+        refuse(PyExc_ValueError, "%s must hold heads of a multiple of 32 elements, a page's bytes side by side", name);
+}
+
+aie_kv4 cache4(const at::Tensor &k, const at::Tensor &v, int device)
+{
+    check_kv4(k, "k_pages", device);
+    check_kv4(v, "v_pages", device);
+    if (k.sizes() != v.sizes() || k.strides() != v.strides())
+        refuse(PyExc_ValueError, "k_pages and v_pages must have the same shape and strides");
+    return {k.data_ptr(), v.data_ptr(), k.stride(0), u32(k.size(0), "pages"), u32(k.size(2), "page_size"), u32(k.size(1), "kv_heads"),
+            u32(k.size(3) / 5 * 8, "head_dim")};
+}
+
+void same_heads4(const at::Tensor &t, const char *name, const aie_kv4 &c)
+{
+    if (t.size(1) != (int64_t)c.kv_heads || t.size(2) != (int64_t)c.head_dim)
+        refuse(PyExc_ValueError, "the cache holds %u heads of %u, %s %lld of %lld", c.kv_heads, c.head_dim, name, (long long)t.size(1),
+                                (long long)t.size(2));
+}
+
+// k, v, k_pages, v_pages, slots, stream
+PyObject *kv4_file(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    arguments(n, 6);
+    const at::Tensor &k = tensor(a[0], "k"), &v = tensor(a[1], "v"), &kp = tensor(a[2], "k_pages"), &vp = tensor(a[3], "v_pages"),
+                     &slots = tensor(a[4], "slots");
+    const Like l = first_heads(k, "k");
+    aie_kv4_rows p = {};
+    p.cache = cache4(kp, vp, l.device);
+    p.k = heads(k, "k", l);
+    p.v = heads(v, "v", l);
+    same_shape(v, "v", k, "k");
+    same_heads4(k, "k", p.cache);
+    p.slots = (const int64_t *)vector(slots, "slots", at::kLong, l.device);
+    if (slots.size(0) != k.size(0)) refuse(PyExc_ValueError, "%lld slots for %lld tokens", (long long)slots.size(0), (long long)k.size(0));
+    p.tokens = u32(k.size(0), "tokens");
+    p.dtype = l.dtype;
+    OnStream on(a[5], l.device);
+    check(aie_kv4_file(&p, on.get()), "aie_kv4_file");
+    written(kp);
+    written(vp);
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// k_pages, v_pages, slots, dtype, stream
+PyObject *kv4_load(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    arguments(n, 5);
+    const at::Tensor &kp = tensor(a[0], "k_pages"), &vp = tensor(a[1], "v_pages"), &slots = tensor(a[2], "slots");
+    aie_kv4_rows p = {};
+    p.cache = cache4(kp, vp, -1);
+    const int device = (int)kp.get_device();
+    p.slots = (const int64_t *)vector(slots, "slots", at::kLong, device);
+    if (!THPDtype_Check(a[3])) refuse(PyExc_TypeError, "dtype must be a torch dtype");
+    const at::ScalarType type = ((THPDtype *)a[3])->scalar_type;
+    p.dtype = type == at::kFloat ? AIE_DT_F32 : type == at::kHalf ? AIE_DT_F16 : type == at::kBFloat16 ? AIE_DT_BF16 : -1;
+    if (p.dtype < 0) refuse(PyExc_TypeError, "dtype must be float16, bfloat16 or float32");
+    p.tokens = u32(slots.size(0), "tokens");
+    OnStream on(a[4], device);
+    at::Tensor out[2];
+    for (at::Tensor &t : out)
+        t = at::detail::empty_cuda({slots.size(0), kp.size(1), (int64_t)p.cache.head_dim}, type, kp.device(), std::nullopt);
+    p.k = {out[0].data_ptr(), out[0].stride(0), out[0].stride(1)};
+    p.v = {out[1].data_ptr(), out[1].stride(0), out[1].stride(1)};
+    check(aie_kv4_load(&p, on.get()), "aie_kv4_load");
+    return Py_BuildValue("(NN)", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+    END_HANDLE_TH_ERRORS
+}
+
+// q, k_pages, v_pages, table, lens, max_len, scale, out, stream
+PyObject *kv4_attention(PyObject *, PyObject *const *a, Py_ssize_t n)
+{
+    HANDLE_TH_ERRORS
+    arguments(n, 9);
+    const at::Tensor &q = tensor(a[0], "q"), &kp = tensor(a[1], "k_pages"), &vp = tensor(a[2], "v_pages"),
+                     &table = tensor(a[3], "table"), &lens = tensor(a[4], "lens");
+    const Like l = first_heads(q, "q");
+    aie_kv4_step p = {};
+    p.cache = cache4(kp, vp, l.device);
+    p.q = heads(q, "q", l);
+    if (q.size(2) != (int64_t)p.cache.head_dim)
+        refuse(PyExc_ValueError, "the cache holds heads of %u, q of %lld", p.cache.head_dim, (long long)q.size(2));
+    p.table = (const int32_t *)vector(table, "table", at::kInt, l.device, 2);
+    p.lens = (const int32_t *)vector(lens, "lens", at::kInt, l.device);
+    const int64_t b = q.size(0);
+    if (table.size(0) != b || lens.size(0) != b)
+        refuse(PyExc_ValueError, "%lld streams, but %lld table rows and %lld lengths", (long long)b, (long long)table.size(0),
+                                (long long)lens.size(0));
+    const at::Tensor *o = optional(a[7], "out");
+    OnStream on(a[8], l.device);
+    const at::Tensor out = o ? *o : fresh_like(q);
+    same_shape(out, "out", q, "q");
+    p.out = heads(out, "out", l);
+    p.batch = u32(b, "the batch");
+    p.q_heads = u32(q.size(1), "q's heads");
+    p.max_len = u32(a[5] == Py_None ? table.size(1) * (int64_t)p.cache.page_size : integer(a[5]), "max_len");
+    p.table_stride = u32(table.size(1), "the table's width");
+    p.dtype = l.dtype;
+    p.scale = a[6] == Py_None ? 1.f / std::sqrt((float)q.size(2)) : (float)real(a[6]);
+    p.workspace_bytes = std::max<uint64_t>(aie_kv4_attn_workspace(&p), 16);
+    const at::Tensor ws = scratch((int64_t)p.workspace_bytes, at::kByte, l.device);
+    p.workspace = ws.data_ptr();
+    check(aie_kv4_attn(&p, on.get()), "aie_kv4_attn");
+    if (o) written(*o);
+    return o ? Py_NewRef(a[7]) : THPVariable_Wrap(out);
+    END_HANDLE_TH_ERRORS
+}
+
 // ---- pages
 
 // kv into p; its device
 int pack_kv(PyObject *o, aie_pages &p)
 {
     const at::Tensor &kv = no_grad(tensor(o, "kv"), "kv");
-    if (dtype_id(kv) < 0 || !kv.is_cuda() || kv.dim() != 6 || kv.size(1) != 2 || !kv.is_contiguous())
+    const bool bytes = kv.scalar_type() == at::kByte;  // 4 bits an element: heads, then places
+    if ((!bytes && dtype_id(kv) < 0) || !kv.is_cuda() || kv.dim() != 6 || kv.size(1) != 2 || !kv.is_contiguous())
         refuse(PyExc_TypeError, "kv must be a contiguous float16, bfloat16 or float32 CUDA tensor "
-                               "[layers, 2, pages, page_size, kv_heads, head_dim]");
+                               "[layers, 2, pages, page_size, kv_heads, head_dim], or a uint8 one of pages.new_cache4");
     p.kv = kv.data_ptr();
     p.layers = u32(kv.size(0), "layers");
     p.pages = u32(kv.size(2), "pages");
-    p.page_size = u32(kv.size(3), "page_size");
+    p.page_size = u32(kv.size(bytes ? 4 : 3), "page_size");
     p.page_bytes = (uint64_t)(kv.size(3) * kv.size(4) * kv.size(5) * kv.element_size());
     return (int)kv.get_device();
 }
@@ -493,8 +667,9 @@ PyObject *pages_compact(PyObject *, PyObject *const *a, Py_ssize_t n)
 }
 
 #define FN(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FN(qk_norm_rope), FN(prompt_attention), FN(prefix_attention), FN(pages_grow), FN(pages_fork),
-                         FN(pages_copy),   FN(pages_free),       FN(pages_compact),    {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FN(qk_norm_rope), FN(prompt_attention), FN(prefix_attention), FN(cross_attention), FN(kv4_file),
+                         FN(kv4_load),     FN(kv4_attention),    FN(pages_grow),       FN(pages_fork),      FN(pages_copy),
+                         FN(pages_free),   FN(pages_compact),    {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_seqcall", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

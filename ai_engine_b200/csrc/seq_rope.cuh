@@ -22,7 +22,19 @@ struct RopeArgs {
     const int64_t *slots;
     int tokens, hq, hk, d, rot, max_pos, interleaved;
     float eps;
+    const uint8_t *axis;  // each pair's axis, or nullptr: one position a token
+    int axes;             // positions of a token
 };
+
+// The cosines and sines of pair i of token t: its own row of the table where the
+// positions have axes.
+template <typename T>
+__device__ __forceinline__ const float *rope_angles(const RopeArgs<T> &a, int t, int axis)
+{
+    if (axis >= a.axes) return nullptr;
+    const int pos = a.pos[(long long)t * a.axes + axis];
+    return pos >= 0 && pos < a.max_pos ? a.cs + (long long)pos * a.rot : nullptr;
+}
 
 // Where a token's head stands in the cache, or nullptr.
 template <typename T>
@@ -39,7 +51,7 @@ constexpr int kRopeMaxDim = 512;
 // Any head size, stride and alignment: one warp per head of a token (query
 // heads, then key heads, then value heads, which are only filed), the normed
 // head in shared memory while it is rotated.
-template <typename T>
+template <typename T, bool AXES>
 __global__ void __launch_bounds__(128) rope_row_kernel(RopeArgs<T> a)
 {
     __shared__ float buf[4][kRopeMaxDim];
@@ -78,18 +90,18 @@ __global__ void __launch_bounds__(128) rope_row_kernel(RopeArgs<T> a)
     T *o1 = key ? (a.ko.p ? a.ko.at(t, h) : nullptr) : a.qo.at(t, h);
     T *o2 = key ? rope_slot(a.kp, a.pg, a.slots, t, h) : nullptr;
     const int half = a.rot >> 1;
-    const int pos = a.rot ? a.pos[t] : 0;
-    const bool ok = pos >= 0 && pos < a.max_pos;
-    const float *cs = a.cs + (long long)(ok ? pos : 0) * a.rot;
+    const float *cs = !AXES && a.rot ? rope_angles(a, t, 0) : nullptr;
     for (int i = lane; i < a.d; i += 32) {
         float v = y[i];
         if (i < a.rot) {
             const int f = a.interleaved ? i >> 1 : (i < half ? i : i - half);
             const bool first = a.interleaved ? !(i & 1) : i < half;
             const float other = y[a.interleaved ? i ^ 1 : (first ? i + half : i - half)];
-            const float c = cs[f], s = cs[half + f];
-            v = first ? v * c - other * s : v * c + other * s;
-            if (!ok) v = __int_as_float(0x7fffffff);
+            if constexpr (AXES) cs = rope_angles(a, t, a.axis[f]);
+            if (cs) {
+                const float c = cs[f], s = cs[half + f];
+                v = first ? v * c - other * s : v * c + other * s;
+            } else v = __int_as_float(0x7fffffff);
         }
         const T r = from_f32<T>(v);
         if (o1) o1[i] = r;
@@ -186,7 +198,7 @@ struct RopeVec {
     float inv_d;
 };
 
-template <typename T, int LPR, int HPT, bool INTERLEAVED>
+template <typename T, int LPR, int HPT, bool INTERLEAVED, bool AXES>
 __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(const RopeArgs<T> a, const RopeVec g)
 {
     behind_last_launch();
@@ -253,15 +265,24 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
             sn[k] = 0.f;
         }
         if (turn) {
-            const int pos = a.pos[t];
-            if (pos >= 0 && pos < a.max_pos) {
-                // angles: e0 .. e0 + 7 of the halves, or of the eight neighbouring pairs
-                const float *cs = a.cs + (long long)pos * a.rot + lane * 8;
-                load8f(cs, c);
-                load8f(cs + half, sn);
+            // angles: e0 .. e0 + 7 of the halves, or of the eight neighbouring pairs
+            uint2 ax = make_uint2(0, 0);  // their axes
+            if constexpr (AXES) ax = *(const uint2 *)(a.axis + lane * 8);
+            if (!AXES || (ax.x == ax.y && ax.x == (ax.x & 255) * 0x01010101u)) {
+                if (const float *cs = rope_angles(a, t, ax.x & 255)) {
+                    load8f(cs + lane * 8, c);
+                    load8f(cs + lane * 8 + half, sn);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) c[k] = sn[k] = __int_as_float(0x7fffffff);
+                }
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) c[k] = sn[k] = __int_as_float(0x7fffffff);
+                for (int k = 0; k < 8; k++) {
+                    const float *cs = rope_angles(a, t, ((k < 4 ? ax.x : ax.y) >> 8 * (k & 3)) & 255);
+                    c[k] = cs ? cs[lane * 8 + k] : __int_as_float(0x7fffffff);
+                    sn[k] = cs ? cs[lane * 8 + k + half] : __int_as_float(0x7fffffff);
+                }
             }
         }
         if (w) {
@@ -339,7 +360,7 @@ static bool rope_vec_ok(const RopeArgs<T> &a)
     auto ok = [&](const HeadsOf<T> &h) { return !h.p || ((uintptr_t)h.p % 16 == 0 && h.ts % unit == 0 && h.hs % unit == 0); };
     auto ptr = [](const void *p) { return (uintptr_t)p % 16 == 0; };
     return a.d % 16 == 0 && a.rot % 16 == 0 && (unsigned long long)a.tokens * (a.hq + 2 * a.hk) < 1ull << 32 && ok(a.q) && ok(a.k) && ok(a.v) && ok(a.qo) && ok(a.ko) && ptr(a.kp) && ptr(a.vp) &&
-           (!a.kp || (a.pg.ps % unit == 0 && a.pg.ts % unit == 0 && a.pg.hs % unit == 0)) && ptr(a.wq) && ptr(a.wk) && ptr(a.cs);
+           (!a.kp || (a.pg.ps % unit == 0 && a.pg.ts % unit == 0 && a.pg.hs % unit == 0)) && ptr(a.wq) && ptr(a.wk) && ptr(a.cs) && (uintptr_t)a.axis % 8 == 0;
 }
 
 template <typename T, int LPR, int HPT>
@@ -354,8 +375,9 @@ static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
     g.slots32 = (unsigned long long)a.pg.pages * a.pg.size <= 0xffffffffull;
     g.inv_d = 1.0f / (float)a.d;
     const unsigned grid = (unsigned)(((unsigned long long)g.end * LPR + kRopeThreads - 1) / kRopeThreads);
-    return launch_behind(a.interleaved ? rope_vec_kernel<T, LPR, HPT, true> : rope_vec_kernel<T, LPR, HPT, false>, grid, kRopeThreads,
-                         0, s, a, g);
+    auto *fn = a.axis ? (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, true> : rope_vec_kernel<T, LPR, HPT, false, true>)
+                      : (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, false> : rope_vec_kernel<T, LPR, HPT, false, false>);
+    return launch_behind(fn, grid, kRopeThreads, 0, s, a, g);
 }
 
 // So few heads that one at a time they are all resident at once: one at a time
@@ -378,7 +400,7 @@ static cudaError_t rope_launch(const RopeArgs<T> &a, cudaStream_t s)
         return rope_vec_launch<T, 32>(a, s);
     }
     const long long units = (long long)a.tokens * (a.hq + a.hk + (a.vp ? a.hk : 0));
-    return launch_behind(rope_row_kernel<T>, (unsigned)((units + 3) / 4), 128, 0, s, a);
+    return launch_behind(a.axis ? rope_row_kernel<T, true> : rope_row_kernel<T, false>, (unsigned)((units + 3) / 4), 128, 0, s, a);
 }
 
 }  // namespace aie

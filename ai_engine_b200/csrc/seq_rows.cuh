@@ -130,6 +130,34 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(PromptRows<T> a)
     attend_row<T>(qs[warp], keys, (a.causal ? t + 1 : end) - first, a.d, a.o.at(t, h), lane);
 }
 
+// Packed tokens and the states that their sequences see.
+template <typename T>
+struct CrossRows {
+    HeadsOf<T> q, k, v, o;
+    const int32_t *cu_q, *cu_k;
+    int tokens, keys, seqs, hq, group, d;
+    float scale;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(128) cross_rows_kernel(CrossRows<T> a)
+{
+    __shared__ float qs[4][kRowsMaxDim];
+    behind_last_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long row = (long long)blockIdx.x * 4 + warp;
+    if (row >= (long long)a.tokens * a.hq) return;
+    const int t = (int)(row / a.hq), h = (int)(row % a.hq);
+    const int s = a.cu_q ? find_seq(a.cu_q, a.seqs, t) : t;
+    if (s >= a.seqs || (a.cu_q && t < a.cu_q[s])) return;
+    const int first = min(max(a.cu_k[s], 0), a.keys), end = min(a.cu_k[s + 1], a.keys);
+    const T *q = a.q.at(t, h);
+    for (int i = lane; i < a.d; i += 32) qs[warp][i] = to_f32(q[i]) * a.scale;
+    __syncwarp();
+    const PackedKeys<T> keys{a.k, a.v, first, h / a.group};
+    attend_row<T>(qs[warp], keys, end - first, a.d, a.o.at(t, h), lane);
+}
+
 template <typename T>
 struct PrefixRows {
     HeadsOf<T> q, o;

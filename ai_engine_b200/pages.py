@@ -2,7 +2,7 @@
 (aie_pages_* of ``include/aie_seq.h``).
 
 The cache is one tensor ``kv`` [layers, 2, pages, page_size, kv_heads,
-head_dim] (keys, then values); its bookkeeping four int32 CUDA tensors
+head_dim] (keys, then values), or one in 4 bits (``new_cache4``); its bookkeeping four int32 CUDA tensors
 (``PageState``).  A row of the table is one stream.  All decisions are made on
 the device, in the lists' order and lowest free page first, so a call can be
 captured in a CUDA graph and nothing is copied to the host; what a call could
@@ -38,6 +38,17 @@ def new_cache(layers: int, pages: int, page_size: int, kv_heads: int, head_dim: 
               device="cuda") -> torch.Tensor:
     """An empty cache; kv[layer, 0] and kv[layer, 1] are a layer's k_pages and v_pages."""
     return torch.zeros((layers, 2, pages, page_size, kv_heads, head_dim), dtype=dtype, device=device)
+
+
+def new_cache4(layers: int, pages: int, page_size: int, kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """An empty cache in 4 bits: uint8 [layers, 2, pages, kv_heads, page_size,
+    head_dim * 5 / 8], for attention.kv4_file, kv4_load and kv4_attention and for
+    fork, copy and compact.  A page and head's bytes are one block: its places'
+    codes, then their groups' scales and lowest values (aie_kv4).  head_dim is a
+    multiple of 32 up to 256, page_size of 8."""
+    if head_dim % 32 or not 0 < head_dim <= 256 or page_size % 8 or page_size <= 0:
+        raise ValueError(f"pages of {page_size} places of heads of {head_dim}: multiples of 8 and of 32, heads up to 256")
+    return torch.zeros((layers, 2, pages, kv_heads, page_size, head_dim * 5 // 8), dtype=torch.uint8, device=device)
 
 
 def grow(st: PageState, page_size: int, rows: torch.Tensor, counts: torch.Tensor, tokens: int, stream=None) -> torch.Tensor:

@@ -10,6 +10,12 @@
  *                          paged cache, the part they share computed once
  *   aie_pages_*            upkeep of the cache's pages: grow, fork, copy,
  *                          free, compact
+ *   aie_qk_norm_rope_axes  the norm and rotation by positions along several
+ *                          axes (time, height, width)
+ *   aie_cross_attn         attention of packed tokens, or of one token per
+ *                          sequence, to states of another length
+ *   aie_kv4_*              a paged cache in 4 bits: filing, reading back, and
+ *                          the one-token attention over it
  *
  * ai_engine has no counterpart of these.  The conventions are aie_conv.h's:
  * caller-owned device buffers, calls that are asynchronous on the caller's
@@ -71,6 +77,13 @@ typedef struct aie_qk_rope {
 } aie_qk_rope;
 AIE_API int aie_qk_norm_rope(const aie_qk_rope *p, void *stream);
 
+/* The same with positions along `axes` axes (1 to 255), positions[t * axes + a] on
+ * the device: pair i of the rotation takes its angle from column i of cos_sin's
+ * row for the position along axis pair_axis[i] (device, [rot_dim / 2]).  A
+ * position outside [0, max_pos), or an axis that does not exist, gives NaN in
+ * the pair's elements. */
+AIE_API int aie_qk_norm_rope_axes(const aie_qk_rope *p, const uint8_t *pair_axis, uint32_t axes, void *stream);
+
 /* out[t] = sum_j softmax_j(scale q[t] . k[j]) v[j] over the tokens j of t's
  * own sequence (causal: j <= t).  Sequence s is tokens cu[s] .. cu[s + 1];
  * cu (device, [seqs + 1], not decreasing, within 0 .. tokens) is read on the
@@ -86,6 +99,27 @@ typedef struct aie_prompt {
     float scale;
 } aie_prompt;
 AIE_API int aie_prompt_attn(const aie_prompt *p, void *stream);
+
+/* out[t] = sum_j softmax_j(scale q[t] . k[j]) v[j] over the states j of t's
+ * sequence s: tokens cu_q[s] .. cu_q[s + 1] of q see states cu_k[s] .. cu_k[s + 1]
+ * of k and v.  cu_q NULL: token s is sequence s's one token (tokens == seqs).
+ * Both lists (device, [seqs + 1], not decreasing, within 0 .. tokens and 0 ..
+ * keys) are read on the device.  A sequence without states gives zeros; tokens
+ * of no sequence are left unwritten.  Values of other sequences, infinities and
+ * NaN among them, never reach a result.
+ * workspace: aie_cross_attn_workspace(p) bytes, 16-byte aligned, its contents
+ * unspecified before and after; calls that may overlap need one each. */
+typedef struct aie_cross {
+    aie_heads q, k, v, out;
+    const int32_t *cu_q, *cu_k;
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint32_t tokens, keys, seqs, q_heads, kv_heads, head_dim;
+    int32_t dtype;
+    float scale;
+} aie_cross;
+AIE_API uint64_t aie_cross_attn_workspace(const aie_cross *p);
+AIE_API int aie_cross_attn(const aie_cross *p, void *stream);
 
 /* One query token for each of `batch` streams: out[b] = sum_j softmax_j(scale
  * q[b] . k[j]) v[j] over the first lens[b] places of stream b.  Places below
@@ -114,12 +148,69 @@ typedef struct aie_prefix {
 AIE_API uint64_t aie_prefix_attn_workspace(const aie_prefix *p);
 AIE_API int aie_prefix_attn(const aie_prefix *p, void *stream);
 
+/* A paged cache of keys and values in 4 bits.  Elements 32 g .. 32 g + 31 of a
+ * head are a group with a scale s and a lowest value lo, both f16: its elements
+ * are lo + code * s, codes 0 to 15.  The block of page p and head h is the
+ * page_size * head_dim * 5 / 8 bytes at k + p * page_stride + h * (block bytes)
+ * (v alike): first the codes, head_dim / 2 bytes a place, two to a byte, the even
+ * element in the low half; then the groups' (s, lo) pairs, head_dim / 8 bytes a
+ * place.  head_dim is a multiple of 32 up to 256, page_size of 8; k, v and
+ * page_stride (in bytes) are 16-byte aligned. */
+typedef struct aie_kv4 {
+    void *k, *v;
+    int64_t page_stride;
+    uint32_t pages, page_size, kv_heads, head_dim;
+} aie_kv4;
+
+/* Keys and values of `tokens` tokens and the places they stand at: slot slots[t]
+ * = page * page_size + place (read on the device).
+ * file: k and v go into the cache.  With x a group's elements, clamped to
+ * +-65504: lo = f16(min x), s = f16(max(0, (max x - lo) / 15)), code =
+ * round((x - lo) / s), ties to even, kept within 0 .. 15, and 0 where s is 0; as
+ * in 64 bits.  A group that holds a NaN or an infinity reads as NaN.  A slot
+ * outside the cache (-1) files nothing; two tokens with one slot leave that
+ * place undefined.
+ * load: k and v receive the values, rounded once; a slot outside the cache
+ * gives zeros. */
+typedef struct aie_kv4_rows {
+    aie_kv4 cache;
+    aie_heads k, v;
+    const int64_t *slots;
+    uint32_t tokens;
+    int32_t dtype;
+} aie_kv4_rows;
+AIE_API int aie_kv4_file(const aie_kv4_rows *p, void *stream);
+AIE_API int aie_kv4_load(const aie_kv4_rows *p, void *stream);
+
+/* One query token for each of `batch` streams over the 4-bit cache: out[b] =
+ * sum_j softmax_j(scale q[b] . k[j]) v[j] over the first lens[b] places of
+ * stream b; place j stands in page table[b * table_stride + j / page_size].
+ * f16 and bf16.  A stream with lens[b] <= 0 gives zeros; lens above max_len
+ * count as max_len.  table and lens are read on the device.  Page numbers
+ * outside the cache are never read from; the stream's result is then
+ * unspecified.  Places from lens[b] on, whatever they hold, never reach stream
+ * b's result.
+ * workspace: aie_kv4_attn_workspace(p) bytes, 16-byte aligned, its contents
+ * unspecified before and after; calls that may overlap need one each. */
+typedef struct aie_kv4_step {
+    aie_kv4 cache;
+    aie_heads q, out;
+    const int32_t *table, *lens;
+    void *workspace;
+    uint64_t workspace_bytes;
+    uint32_t batch, q_heads, max_len, table_stride;
+    int32_t dtype;
+    float scale;
+} aie_kv4_step;
+AIE_API uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p);
+AIE_API int aie_kv4_attn(const aie_kv4_step *p, void *stream);
+
 /* The cache's bookkeeping, all on the device: how many rows (streams) hold
  * each page, how many tokens each row has, and its pages in order
  * (table[r * width + i], -1 behind the last).  status collects what the
  * calls below could not do (aie_pages_status bits, OR'ed, never cleared). */
 typedef struct aie_pages {
-    void *kv;                    /* [layers][2][pages][page_bytes], K and V */
+    void *kv;                    /* [layers][2][pages][page_bytes], K and V, in any type */
     int32_t *refs, *lens, *table, *status;
     int32_t *workspace;          /* aie_pages_workspace(pages, n) bytes */
     uint64_t page_bytes;         /* of one page of one layer's K */

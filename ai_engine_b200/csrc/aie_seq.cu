@@ -15,6 +15,7 @@
 #include "seq_attn.cuh"
 #include "seq_kv4.cuh"
 #include "seq_pages.cuh"
+#include "seq_read.cuh"
 #include "seq_rope.cuh"
 #include "seq_rows.cuh"
 #include "seq_step.cuh"
@@ -440,7 +441,34 @@ static int check_cross(const aie_cross *p)
     return AIE_OK;
 }
 
-extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p) { return check_cross(p) ? 0 : 64; }
+// Whether one token of each sequence goes over the states in equal parts:
+// 16-bit heads in whole 16-byte pieces.
+static bool cross_read_ok(const aie_cross &p)
+{
+    auto ok = [](const aie_heads &h) { return (uintptr_t)h.data % 16 == 0 && h.token_stride % 8 == 0 && h.head_stride % 8 == 0; };
+    return !p.cu_q && p.dtype != AIE_DT_F32 && p.head_dim % 8 == 0 && ok(p.k) && ok(p.v) &&
+           (uint64_t)p.seqs * p.q_heads <= 0x7fffffffull;
+}
+
+extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p)
+{
+    if (check_cross(p)) return 0;
+    if (cross_read_ok(*p)) return read_plan(p->seqs, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
+    return 64;
+}
+
+static int cross_read(const aie_cross &p, cudaStream_t s)
+{
+    ReadArgs a = {};
+    const ReadPlan w = read_plan(p.seqs, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
+    read_args(a, w, p.q, p.out, p.workspace);
+    a.k = p.k.data; a.k_ts = p.k.token_stride; a.k_hs = p.k.head_stride;
+    a.v = p.v.data; a.v_ts = p.v.token_stride; a.v_hs = p.v.head_stride;
+    a.cu = p.cu_k; a.keys = (int)p.keys;
+    a.seqs = (int)p.seqs; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
+    a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
+    return launched(a.bf16 ? read16_launch<__nv_bfloat16>(a, w.nt, s) : read16_launch<__half>(a, w.nt, s), "cross attention");
+}
 
 template <typename T>
 static int cross_rows(const aie_cross &p, cudaStream_t s)
@@ -471,6 +499,7 @@ extern "C" int aie_cross_attn(const aie_cross *p, void *stream)
     if (p->workspace_bytes < need || !p->workspace || (uintptr_t)p->workspace % 16)
         return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
     cudaStream_t s = (cudaStream_t)stream;
+    if (cross_read_ok(*p)) return cross_read(*p, s);
     if (p->dtype == AIE_DT_F32) return cross_rows<float>(*p, s);
     return p->dtype == AIE_DT_F16 ? cross_rows<__half>(*p, s) : cross_rows<__nv_bfloat16>(*p, s);
 }
@@ -525,20 +554,36 @@ static int check_kv4_step(const aie_kv4_step *p)
     return AIE_OK;
 }
 
-extern "C" uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p) { return check_kv4_step(p) ? 0 : 64; }
+static ReadPlan kv4_plan(const aie_kv4_step &p)
+{
+    return read_plan(p.batch, p.cache.kv_heads, p.q_heads / p.cache.kv_heads, p.cache.head_dim);
+}
 
-template <typename T>
+extern "C" uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p) { return check_kv4_step(p) ? 0 : kv4_plan(*p).bytes; }
+
 static int kv4_step(const aie_kv4_step &p, cudaStream_t s)
 {
-    Kv4Step<T> a;
-    a.g = kv4_geom(p.cache);
-    a.q = heads_of<T>(p.q); a.o = heads_of<T>(p.out);
-    a.table = p.table; a.lens = p.lens;
-    a.batch = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads);
-    a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
-    a.scale = p.scale;
-    const long long rows = (long long)p.batch * p.q_heads;
-    return launched(launch_behind(kv4_step_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "attention over 4 bits");
+    ReadArgs a = {};
+    const ReadPlan w = kv4_plan(p);
+    if ((uint64_t)p.batch * w.heads * (p.max_len / 32 + 1ull) / w.workers > 0x7ffffff0ull)
+        return fail(AIE_E_UNSUPPORTED, "too many places in one call");
+    read_args(a, w, p.q, p.out, p.workspace);
+    a.g = kv4_geom(p.cache); a.size = make_fastdiv(a.g.size);
+    a.table = p.table; a.lens = p.lens; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
+    a.seqs = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads); a.d = a.g.d;
+    a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
+    cudaError_t e;
+    switch (a.d / 32) {
+    case 1: e = read4_launch<1>(a, w.nt, s); break;
+    case 2: e = read4_launch<2>(a, w.nt, s); break;
+    case 3: e = read4_launch<3>(a, w.nt, s); break;
+    case 4: e = read4_launch<4>(a, w.nt, s); break;
+    case 5: e = read4_launch<5>(a, w.nt, s); break;
+    case 6: e = read4_launch<6>(a, w.nt, s); break;
+    case 7: e = read4_launch<7>(a, w.nt, s); break;
+    default: e = read4_launch<8>(a, w.nt, s); break;
+    }
+    return launched(e, "attention over 4 bits");
 }
 
 extern "C" int aie_kv4_attn(const aie_kv4_step *p, void *stream)
@@ -557,7 +602,7 @@ extern "C" int aie_kv4_attn(const aie_kv4_step *p, void *stream)
     const uint64_t need = aie_kv4_attn_workspace(p);
     if (p->workspace_bytes < need || !p->workspace || (uintptr_t)p->workspace % 16)
         return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
-    return p->dtype == AIE_DT_F16 ? kv4_step<__half>(*p, (cudaStream_t)stream) : kv4_step<__nv_bfloat16>(*p, (cudaStream_t)stream);
+    return kv4_step(*p, (cudaStream_t)stream);
 }
 
 // --------------------------------------------------------------- pages ---

@@ -1,4 +1,4 @@
-// A paged cache in 4 bits: filing, reading back, and one-token attention over it.
+// A paged cache in 4 bits: filing and reading back.
 //
 //   lo = f16(min x),  s = f16((max x - lo) / 15),  code = rint((x - lo) / s),
 //   x' = lo + code s
@@ -190,83 +190,6 @@ static cudaError_t kv4_rows_launch(const aie_kv4_rows &p, bool file, cudaStream_
     };
     a.vec = ok(p.k) && ok(p.v);
     return launch_behind(file ? kv4_file_kernel<T> : kv4_load_kernel<T>, (a.pieces + 127) / 128, 128, 0, s, a);
-}
-
-// ---------------------------------------------------------- attention ---
-
-template <typename T>
-struct Kv4Step {
-    Kv4Geom g;
-    HeadsOf<T> q, o;
-    const int32_t *table, *lens;
-    int batch, hq, group, max_len, table_stride;
-    float scale;
-};
-
-// One warp per stream and query head, a place a lane.
-template <typename T>
-__global__ void __launch_bounds__(128) kv4_step_kernel(const Kv4Step<T> a)
-{
-    __shared__ float qs[4][256];
-    behind_last_launch();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = a.g.d;
-    const long long row = (long long)blockIdx.x * 4 + warp;
-    if (row >= (long long)a.batch * a.hq) return;
-    const int b = (int)(row / a.hq), h = (int)(row % a.hq), kvh = h / a.group;
-    const int n = min(a.lens[b], a.max_len);
-    const T *q = a.q.at(b, h);
-    for (int i = lane; i < d; i += 32) qs[warp][i] = to_f32(q[i]) * a.scale;
-    __syncwarp();
-    float acc[8], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; i++) acc[i] = 0.f;
-    for (int j0 = 0; j0 < n; j0 += 32) {
-        const int j = j0 + lane;
-        const int page = j < n ? a.table[(long long)b * a.table_stride + j / a.g.size] : -1;
-        const bool real = page >= 0 && page < a.g.pages;
-        float s = -INFINITY;
-        long long off = 0;
-        const int place = j % a.g.size;
-        if (real) {
-            off = page * a.g.page_stride + kvh * a.g.block();
-            const uint8_t *blk = a.g.k + off;
-            s = 0.f;
-            for (int i = 0; i < d; i += 8) {
-                float f[8];
-                kv4_values(*(const uint32_t *)(blk + (place * d + i) / 2), *(const uint32_t *)(blk + a.g.size * d / 2 + place * d / 8 + i / 32 * 4), f);
-                for (int e = 0; e < 8; e++) s = fmaf(qs[warp][i + e], f[e], s);
-            }
-        }
-        const float top = fmaxf(m, warp_max(s));
-        const float old = m == top ? 1.f : expf(m - top);
-        const float p = !real || (top == -INFINITY && s == -INFINITY) ? 0.f : expf(s - top);
-        l = fmaf(l, old, warp_sum(p));
-        m = top;
-#pragma unroll
-        for (int i = 0; i < 8; i++) acc[i] *= old;
-        unsigned todo = __ballot_sync(0xffffffffu, real);
-        while (todo) {
-            const int src = __ffs(todo) - 1;
-            todo &= todo - 1;
-            const float pj = __shfl_sync(0xffffffffu, p, src);
-            const uint8_t *blk = a.g.v + __shfl_sync(0xffffffffu, off, src);
-            const int at = __shfl_sync(0xffffffffu, place, src);
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int e = lane + 32 * i;
-                if (e < d) {
-                    const uint32_t c = blk[(at * d + e) / 2] >> 4 * (e & 1) & 15;
-                    const uint32_t pair = *(const uint32_t *)(blk + a.g.size * d / 2 + at * d / 8 + i * 4);
-                    const float2 sl = __half22float2(*(const __half2 *)&pair);
-                    acc[i] = fmaf(pj, fmaf((float)c, sl.x, sl.y), acc[i]);
-                }
-            }
-        }
-    }
-    T *out = a.o.at(b, h);
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (lane + 32 * i < d) out[lane + 32 * i] = from_f32<T>(n > 0 ? acc[i] / l : 0.f);
 }
 
 }  // namespace aie

@@ -1,0 +1,724 @@
+// One query token for each of many sequences over the sequence's own keys: the
+// frames' states (packed, 16 bits) or the places of the 4-bit cache.
+//
+//   S^T = K Q^T,  P = 2^(S - m),  O^T = V^T P^T,  out = O / l
+//
+// with m, l and O carried along.  Each key is read once for the group of query
+// heads that share it: memory-bound, so everything goes by keeping copies in
+// flight.  K and V are the M side of the products (m16n8k16): 16 keys or 16
+// elements of V by 8 query heads, so that a group of up to 8 heads wastes no
+// more than the rest of 8 columns, and 4-bit codes become operands in the
+// registers that they are loaded to.
+//
+// The sequences' tiles of keys, for every key head one after the other, are one
+// long list, and each warp takes an equal part of it, whatever the lengths are:
+// no sequence is too long for a warp, nor many short ones too uneven.  A warp
+// copies its own tiles ahead (cp.async, a ring of its own; nothing is waited for
+// but its own copies) and shares nothing with the others.  Where a sequence's
+// tiles end up in several warps, each leaves a partial result (O / l and log2 of
+// the weights' sum), and a second launch joins them:
+//   out = sum 2^(lse_i - lse) O_i.
+// Partial result number `warp + sequence` is its own for every pair that meet,
+// since both only grow along the list.  Fixed order throughout: results repeat
+// bit for bit.
+//
+// Rounding to fewer bits: the weights to 16 bits for the product with V (l sums
+// them unrounded; f16 weights 2^7 times as large, as in attn_tc_kernel), the
+// result, and over the 4-bit cache lo + code s to f16 for that product, by
+// 2^-12 of it, where the weights lose as much.
+#pragma once
+#include "seq_kv4.cuh"
+#include "seq_step.cuh"
+
+namespace aie {
+
+constexpr int kRdWarps = 4, kRdThreads = 32 * kRdWarps;
+
+struct ReadArgs {
+    const void *q;
+    void *out;
+    long long q_ts, q_hs, o_ts, o_hs;
+    // the sequences' keys: packed states ...
+    const void *k, *v;
+    long long k_ts, k_hs, v_ts, v_hs;
+    const int32_t *cu;
+    int keys;
+    // ... or places of pages
+    Kv4Geom g;
+    FastDiv size;
+    const int32_t *table, *lens;
+    int max_len, table_stride;
+    int seqs, hq, group, d;
+    int zs, heads;           // blocks of a group's query heads; key heads times those
+    int rows;                // query heads of a block that are kept
+    int bf16;
+    float scale;
+    // workspace
+    long long *before;       // [seqs + 1]: tiles of the sequences before
+    float *part_lse, *part_o;
+    int workers;
+};
+
+__device__ __forceinline__ int read_len(const ReadArgs &a, int s)
+{
+    if (a.lens) return min(max(a.lens[s], 0), a.max_len);
+    const int from = min(max(a.cu[s], 0), a.keys), to = min(max(a.cu[s + 1], 0), a.keys);
+    return max(to - from, 0);
+}
+
+// Tiles a warp takes of `total`.
+__device__ __forceinline__ long long read_share(long long total, int workers) { return max((total + workers - 1) / workers, 1ll); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes)
+{
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix2(uint32_t addr, uint32_t (&r)[2])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix2_t(uint32_t addr, uint32_t (&r)[2])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(addr) : "memory");
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
+{
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+// (x & mask) | one, two halves at a time
+__device__ __forceinline__ uint32_t pick(uint32_t x, uint32_t mask, uint32_t one)
+{
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(one));
+    return y;
+}
+
+// Four codes of each half of a word as f16 pairs: code i of the lower half and of
+// the upper.  A code in an f16's fraction, four bits under 16 or eight under
+// 256, is that number plus the code.
+struct Codes {
+    uint32_t p[4];  // 256 + code 0, 16 + code 1, 256 + code 2, 16 + code 3
+    __device__ __forceinline__ Codes(uint32_t w)
+    {
+        const uint32_t lo = w << 2, hi = w >> 6;
+        p[0] = pick(lo, 0x003C003Cu, 0x5C005C00u);
+        p[1] = pick(lo, 0x03C003C0u, 0x4C004C00u);
+        p[2] = pick(hi, 0x003C003Cu, 0x5C005C00u);
+        p[3] = pick(hi, 0x03C003C0u, 0x4C004C00u);
+    }
+};
+
+// N 32-bit words of shared memory from an address aligned to the whole of them.
+template <int N>
+__device__ __forceinline__ void shared_words(const uint32_t *p, uint32_t (&w)[N])
+{
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const uint4 x = *(const uint4 *)(p + i);
+            w[i] = x.x; w[i + 1] = x.y; w[i + 2] = x.z; w[i + 3] = x.w;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const uint2 x = *(const uint2 *)(p + i);
+            w[i] = x.x; w[i + 1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = p[i];
+    }
+}
+
+// DC: groups of 32 elements (4 bits) or steps of 16 (16 bits).  A stage of a
+// warp's ring holds one tile: K rows, then V rows, a row padded to an odd number
+// of 16-byte pieces so that eight rows' pieces are in different banks; then, in
+// 4 bits, the groups' pairs of K and of V.
+template <bool KV4, int DC>
+struct ReadTile {
+    static constexpr int kKeys = KV4 ? 32 : 16;
+    static constexpr int kPieces = KV4 ? DC : 2 * DC;       // of a row
+    static constexpr uint32_t kRow = (kPieces | 1) * 16;
+    static constexpr uint32_t kSide = kKeys * kRow;         // K or V
+    static constexpr uint32_t kPairs = KV4 ? kKeys * DC * 4 : 0;
+    static constexpr uint32_t kStage = 2 * kSide + 2 * kPairs;
+};
+
+// T: the operands' type, f16 in 4 bits.
+template <typename T, bool KV4, int DC, int NT, int STAGES>
+__global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
+{
+    using Tile = ReadTile<KV4, DC>;
+    constexpr int MT = Tile::kKeys / 16, OT = KV4 ? 2 * DC : DC;  // tiles of 16 keys; of 16 elements of V
+    extern __shared__ __align__(16) char smem[];
+    __shared__ long long scan[kRdThreads], warp_sum_[kRdWarps];
+    behind_last_launch();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- tiles before each thread's sequences, and in all
+    const int per = (a.seqs + kRdThreads - 1) / kRdThreads, s_from = tid * per, s_to = min(s_from + per, a.seqs);
+    long long mine = 0;
+    for (int s = s_from; s < s_to; s++) mine += (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys;
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 31) warp_sum_[warp] = upto;
+    __syncthreads();
+    long long tiles = 0, base = upto - mine;
+#pragma unroll
+    for (int i = 0; i < kRdWarps; i++) {
+        if (i < warp) base += warp_sum_[i];
+        tiles += warp_sum_[i];
+    }
+    scan[tid] = base;
+    if (blockIdx.x == 0) {  // for the joining launch
+        for (int s = s_from; s < s_to; s++) {
+            a.before[s] = base;
+            base += (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys;
+        }
+        if (tid == 0) a.before[a.seqs] = tiles;
+    }
+    __syncthreads();
+    const long long total = tiles * a.heads, share = read_share(total, a.workers);
+    const int worker = blockIdx.x * kRdWarps + warp;
+    const long long begin = worker * share;
+    if (begin >= total) return;
+    const int count = (int)min(share, total - begin);
+
+    // ---- where the warp's part begins
+    struct Place {
+        int s, head, tile, len;  // sequence; key head and block of query heads; tile of the sequence
+    } at;
+    {
+        at.head = (int)(begin / tiles);
+        long long left = begin - at.head * tiles;
+        // the last thread whose sequences begin at or before it
+        int t = 0;
+#pragma unroll
+        for (int i = 0; i < kRdWarps; i++) t += __popc(__ballot_sync(0xffffffffu, scan[i * 32 + lane] <= left));
+        t--;
+        left -= scan[t];
+        for (at.s = t * per;; at.s++) {
+            at.len = read_len(a, at.s);
+            const int n = (at.len + Tile::kKeys - 1) / Tile::kKeys;
+            if (left < n) break;
+            left -= n;
+        }
+        at.tile = (int)left;
+    }
+    auto advance = [&](Place &p) {
+        if (++p.tile * Tile::kKeys < p.len) return;
+        p.tile = 0;
+        do {
+            if (++p.s == a.seqs) {
+                p.s = 0;
+                p.head++;
+            }
+            p.len = read_len(a, p.s);
+        } while (!p.len);
+    };
+
+    char *const ring = smem + warp * (STAGES * Tile::kStage);
+    const uint32_t ring_at = smem_u32(ring);
+
+    // ---- copies
+    Place ahead = at;
+    long long page_at = 0;  // 4 bits: a lane's page (of 8 places of the tile), and the first place in it
+    int page_place = 0;
+    bool page_real = false;
+    auto look_up = [&] {
+        if constexpr (KV4) {
+            const int place = ahead.tile * Tile::kKeys + (lane & 3) * 8, i = fdiv(place, a.size);
+            const int page = place < ahead.len ? a.table[(long long)ahead.s * a.table_stride + i] : -1;
+            page_real = page >= 0 && page < a.g.pages;
+            page_at = page_real ? page * a.g.page_stride + (ahead.head / a.zs) * a.g.block() : 0;
+            page_place = place - i * a.g.size;
+        }
+    };
+    auto copy_tile = [&](int stage) {
+        const uint32_t dst = ring_at + stage * Tile::kStage;
+        const int rows = ahead.len - ahead.tile * Tile::kKeys;  // that exist; the others are zeros
+        if constexpr (KV4) {
+#pragma unroll
+            for (int i = 0; i < DC; i++) {
+                const int c = i * 32 + lane, row = c / DC, piece = c - row * DC, eight = row >> 3;
+                const long long off = __shfl_sync(0xffffffffu, page_at, eight) +
+                                      (__shfl_sync(0xffffffffu, page_place, eight) + (row & 7)) * (16 * DC) + piece * 16;
+                const int n = __shfl_sync(0xffffffffu, (int)page_real, eight) && row < rows ? 16 : 0;
+                copy16(dst + row * Tile::kRow + piece * 16, a.g.k + off, n);
+                copy16(dst + Tile::kSide + row * Tile::kRow + piece * 16, a.g.v + off, n);
+            }
+            // pairs: 16 bytes a lane, DC * 2 lanes to 8 places
+            const int eight = min(lane / (2 * DC), 3), in = lane * 16 - eight * 32 * DC;
+            const long long from = __shfl_sync(0xffffffffu, page_at, eight);
+            const int place = __shfl_sync(0xffffffffu, page_place, eight), real = __shfl_sync(0xffffffffu, (int)page_real, eight);
+#pragma unroll
+            for (int i = 0; i < (DC + 3) / 4; i++) {
+                // heads of more than 128: another round of 32 lanes
+                const int c = i * 32 + lane;
+                if (DC > 4 || c < 8 * DC) {
+                    int e8 = eight, in_ = in, pl = place, re = real;
+                    long long fr = from;
+                    if constexpr (DC > 4) {
+                        e8 = min(c / (2 * DC), 3);
+                        in_ = c * 16 - e8 * 32 * DC;
+                        pl = __shfl_sync(0xffffffffu, page_place, e8);
+                        re = __shfl_sync(0xffffffffu, (int)page_real, e8);
+                        fr = __shfl_sync(0xffffffffu, page_at, e8);
+                    }
+                    if (c < 8 * DC) {
+                        const long long off = fr + (long long)a.g.size * (16 * DC) + pl * (4 * DC) + in_;
+                        const int n = re ? min(max((rows - e8 * 8) * 4 * DC - in_, 0), 16) : 0;
+                        copy16(dst + 2 * Tile::kSide + c * 16, a.g.k + off, n);
+                        copy16(dst + 2 * Tile::kSide + Tile::kPairs + c * 16, a.g.v + off, n);
+                    }
+                }
+            }
+        } else {
+            const long long key = min(max(a.cu[ahead.s], 0), a.keys) + (long long)ahead.tile * Tile::kKeys;
+            const int kvh = ahead.head / a.zs;
+            const T *k = (const T *)a.k + key * a.k_ts + kvh * a.k_hs, *v = (const T *)a.v + key * a.v_ts + kvh * a.v_hs;
+#pragma unroll
+            for (int i = 0; i < DC; i++) {
+                const int c = i * 32 + lane, row = c / (2 * DC), piece = c % (2 * DC);
+                const bool real = row < rows && piece * 8 < a.d;
+                copy16(dst + row * Tile::kRow + piece * 16, real ? k + row * a.k_ts + piece * 8 : k, real ? 16 : 0);
+                copy16(dst + Tile::kSide + row * Tile::kRow + piece * 16, real ? v + row * a.v_ts + piece * 8 : v, real ? 16 : 0);
+            }
+        }
+    };
+    int copied = 0;
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; i++) {
+        if (copied < count) {
+            copy_tile(i);
+            if (++copied < count) {
+                advance(ahead);
+                look_up();
+            }
+        }
+        copies_commit();
+    }
+
+    // ---- products
+    const int r = lane >> 2, c2 = (lane & 3) * 2;  // a lane's rows r, r + 8 and columns c2, c2 + 1 of a product
+    const float sl = fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
+    uint32_t qb[NT][KV4 ? 2 * DC : DC][2];
+    float q_c[KV4 ? DC : 1][NT][2], q_sum[KV4 ? DC : 1][NT][2];  // 4 bits: what the codes' offsets add to a group, and its sum of q
+    float slq[NT][2];                                            // scale of a column's scores, in binary orders
+    float o[OT][NT][4], m[NT][2], l[NT][2];
+    bool fresh = true;
+    int first_tile = 0, stage = 0;  // of the sequence's tiles; of the ring
+    for (int i = 0; i < count; i++) {
+        if (fresh) {
+            fresh = false;
+            first_tile = at.tile;
+            const int kvh = at.head / a.zs, row0 = at.head % a.zs * (8 * NT), heads = min(a.group - row0, 8 * NT);
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const int n = nt * 8 + r;
+                const long long qat = (long long)at.s * a.q_ts + (long long)(kvh * a.group + row0 + n) * a.q_hs;
+                if constexpr (KV4) {
+                    float f[DC][8], top = 0.f;
+#pragma unroll
+                    for (int g = 0; g < DC; g++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const long long x = qat + g * 32 + (lane & 3) * 8 + e;
+                            f[g][e] = n >= heads ? 0.f
+                                      : a.bf16   ? __bfloat162float(((const __nv_bfloat16 *)a.q)[x])
+                                                 : __half2float(((const __half *)a.q)[x]);
+                            f[g][e] *= sign;
+                            top = fmaxf(top, fabsf(f[g][e]));
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // a power of two that brings the largest to 2^8 .. 2^9: exact, and in f16
+                    // nothing that counts is subnormal
+                    const int ex = (int)(__float_as_uint(top) >> 23);
+                    const int k = top > 0.f ? min(max(8 + 127 - ex, -120), 120) : 0;
+                    const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+                    for (int g = 0; g < DC; g++) {
+                        float even = 0.f, odd = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float x = __half2float(__float2half_rn(f[g][e] * up));
+                            f[g][e] = x;
+                            if (e & 1) odd += x;
+                            else even += x;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) qb[nt][2 * g + (e >> 1)][e & 1] = pack2<__half>(f[g][e], f[g][e + 4]);
+                        float cc = fmaf(256.f, even, 16.f * odd), su = even + odd;
+#pragma unroll
+                        for (int x = 1; x < 4; x <<= 1) {
+                            cc += __shfl_xor_sync(0xffffffffu, cc, x);
+                            su += __shfl_xor_sync(0xffffffffu, su, x);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            q_c[g][nt][j] = __shfl_sync(0xffffffffu, cc, (c2 + j) * 4);
+                            q_sum[g][nt][j] = __shfl_sync(0xffffffffu, su, (c2 + j) * 4);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; j++) slq[nt][j] = fmaxf(sl * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f);
+                } else {
+                    const T *q = (const T *)a.q + qat;
+#pragma unroll
+                    for (int k = 0; k < DC; k++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int d = k * 16 + e * 8 + c2;
+                            const bool real = n < heads && d < a.d;  // d is even
+                            qb[nt][k][e] = real ? pack2<T>(sign * to_f32(q[d]), sign * to_f32(q[d + 1])) : 0u;
+                        }
+                    slq[nt][0] = slq[nt][1] = fmaxf(sl, 1e-37f);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    m[nt][j] = -INFINITY;
+                    l[nt][j] = 0.f;
+                }
+#pragma unroll
+                for (int x = 0; x < OT; x++) o[x][nt][0] = o[x][nt][1] = o[x][nt][2] = o[x][nt][3] = 0.f;
+            }
+        }
+
+        // the next copy goes where the last tile was
+        if (copied < count) {
+            copy_tile(stage ? stage - 1 : STAGES - 1);
+            if (++copied < count) {
+                advance(ahead);
+                look_up();
+            }
+        }
+        copies_commit();
+        copies_wait<STAGES - 1>();
+        __syncwarp();
+
+        const char *const st = ring + stage * Tile::kStage;
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        const uint32_t kt = smem_u32(st), vt = kt + Tile::kSide;
+        // ---- scores: keys r and r + 8 of each 16, query heads c2 and c2 + 1
+        float s[MT][NT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
+            if constexpr (KV4) {
+                const uint32_t *pk = (const uint32_t *)(st + 2 * Tile::kSide) + (mt * 16 + r) * DC;
+                uint32_t p0[DC], p1[DC];
+                shared_words<DC>(pk, p0);
+                shared_words<DC>(pk + 8 * DC, p1);
+#pragma unroll
+                for (int g = 0; g < DC; g++) {
+                    uint32_t w[2];
+                    ldmatrix2(kt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
+                    const Codes x0(w[0]), x1(w[1]);
+                    const float2 f0 = __half22float2(*(const __half2 *)&p0[g]), f1 = __half22float2(*(const __half2 *)&p1[g]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float acc[4] = {-q_c[g][nt][0], -q_c[g][nt][1], -q_c[g][nt][0], -q_c[g][nt][1]};
+                        mma16816<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
+                        mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            s[mt][nt][j] = fmaf(f0.x, acc[j], fmaf(f0.y, q_sum[g][nt][j], s[mt][nt][j]));
+                            s[mt][nt][2 + j] = fmaf(f1.x, acc[2 + j], fmaf(f1.y, q_sum[g][nt][j], s[mt][nt][2 + j]));
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < DC; k++) {
+                    uint32_t w[4];
+                    ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (2 * k + (lane >> 4)) * 16, w);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                }
+            }
+        }
+        const int here = at.len - at.tile * Tile::kKeys;
+        if (here < Tile::kKeys) {
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (mt * 16 + r + (j >> 1) * 8 >= here) s[mt][nt][j] = -INFINITY;
+        }
+        // ---- weights
+        float top[NT][2];
+        bool grow = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                float x = m[nt][j];
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) x = max3(x, s[mt][nt][j], s[mt][nt][2 + j]);
+                top[nt][j] = x;
+                grow |= (x - m[nt][j]) * slq[nt][j] > 8.f;  // as in attn_tc_kernel: smaller steps leave m
+            }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float x = top[nt][j];
+#pragma unroll
+                    for (int e = 4; e < 32; e <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
+                    const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
+                    m[nt][j] = x;
+                    l[nt][j] *= f;
+#pragma unroll
+                    for (int t = 0; t < OT; t++) {
+                        o[t][nt][j] *= f;
+                        o[t][nt][2 + j] *= f;
+                    }
+                }
+        }
+        uint32_t pb[MT][NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            float off[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], kWeightShift<T>);
+#pragma unroll
+            for (int mt = 0; mt < MT; mt++) {
+                float e[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) e[j] = ex2(fmaf(s[mt][nt][j], slq[nt][j & 1], off[j & 1]));
+                l[nt][0] += e[0] + e[2];
+                l[nt][1] += e[1] + e[3];
+                pb[mt][nt][0] = transpose8x8(pack2<T>(e[0], e[1]));
+                pb[mt][nt][1] = transpose8x8(pack2<T>(e[2], e[3]));
+            }
+        }
+        // ---- values
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++) {
+            if constexpr (KV4) {
+                // (s, lo) of keys c2, c2 + 1 and of 8 further on, two keys to a register
+                const uint32_t *pv = (const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + (mt * 16 + c2) * DC;
+                uint32_t p0[DC], p1[DC], p2[DC], p3[DC];
+                shared_words<DC>(pv, p0);
+                shared_words<DC>(pv + DC, p1);
+                shared_words<DC>(pv + 8 * DC, p2);
+                shared_words<DC>(pv + 9 * DC, p3);
+#pragma unroll
+                for (int g = 0; g < DC; g++) {
+                    uint32_t w[2];
+                    ldmatrix2_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
+                    const Codes x0(w[0]), x1(w[1]);
+                    const uint32_t s0 = __byte_perm(p0[g], p1[g], 0x5410), l0 = __byte_perm(p0[g], p1[g], 0x7632);
+                    const uint32_t s1 = __byte_perm(p2[g], p3[g], 0x5410), l1 = __byte_perm(p2[g], p3[g], 0x7632);
+                    uint32_t v0[4], v1[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const __half2 less = __float2half2_rn(e & 1 ? -16.f : -256.f);
+                        const __half2 y0 = __hfma2(__hadd2(*(const __half2 *)&x0.p[e], less), *(const __half2 *)&s0, *(const __half2 *)&l0);
+                        const __half2 y1 = __hfma2(__hadd2(*(const __half2 *)&x1.p[e], less), *(const __half2 *)&s1, *(const __half2 *)&l1);
+                        v0[e] = *(const uint32_t *)&y0;
+                        v1[e] = *(const uint32_t *)&y1;
+                    }
+                    // rows r: elements 4 r + 0 (+ 2), rows r + 8: 4 r + 1 (+ 3)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        mma16816<T>(o[2 * g][nt], {v0[0], v0[1], v1[0], v1[1]}, pb[mt][nt][0], pb[mt][nt][1]);
+                        mma16816<T>(o[2 * g + 1][nt], {v0[2], v0[3], v1[2], v1[3]}, pb[mt][nt][0], pb[mt][nt][1]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int t = 0; t < DC; t++) {
+                    // as stored: keys 0-7 and 8-15 by elements 0-7, then 8-15
+                    uint32_t w[4];
+                    ldmatrix4_t(vt + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * Tile::kRow + (2 * t + (lane >> 3 & 1)) * 16, w);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) mma16816<T>(o[t][nt], w, pb[mt][nt][0], pb[mt][nt][1]);
+                }
+            }
+        }
+        __syncwarp();  // the tile is read before the copy that replaces it
+
+        // ---- end of the sequence, or of the warp's part
+        const bool ends = (at.tile + 1) * Tile::kKeys >= at.len;
+        if (ends || i + 1 == count) {
+            const bool whole = ends && first_tile == 0;
+            const int kvh = at.head / a.zs, row0 = at.head % a.zs * (8 * NT), heads = min(a.group - row0, 8 * NT);
+            const long long part = (long long)worker + (long long)at.head * a.seqs + at.s;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    float sum = l[nt][j];
+#pragma unroll
+                    for (int e = 4; e < 32; e <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+                    const int n = nt * 8 + c2 + j;
+                    if (n >= heads) continue;
+                    // of several parts, one with scores of -inf alone (the sum is 0) has no weight
+                    const float f = sum == 0.f && !whole ? 0.f : 1.f / sum;
+                    const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
+                    const long long pat = (part * a.rows + n) * a.d;
+                    if (!whole && r == 0)
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - kWeightShift<T>);
+#pragma unroll
+                    for (int t = 0; t < OT; t++)
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            const int d = KV4 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 + e : t * 16 + e * 8 + r;
+                            const float x = o[t][nt][2 * e + j] * f;
+                            if (!KV4 && d >= a.d) continue;
+                            if (!whole) a.part_o[pat + d] = x;
+                            else if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
+                            else ((__half *)a.out)[oat + d] = __float2half_rn(x);
+                        }
+                }
+            fresh = true;
+        }
+        if (i + 1 < count) advance(at);
+    }
+}
+
+// Sequences whose tiles more than one warp took, and those without any: a block
+// per sequence and query head.
+struct JoinArgs {
+    void *out;
+    long long o_ts, o_hs;
+    const long long *before;
+    const float *part_lse, *part_o;
+    int seqs, hq, group, d, zs, heads, rows, bf16, workers;
+};
+
+__global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
+{
+    __shared__ float sums[kRdWarps][256], weights[kRdWarps];
+    behind_last_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int s = blockIdx.x / a.hq, h = blockIdx.x % a.hq, kvh = h / a.group, in = h % a.group;
+    const int head = kvh * a.zs + in / a.rows, row = in % a.rows;
+    const long long tiles = a.before[a.seqs], from = a.before[s], n = a.before[s + 1] - from;
+    const long long share = read_share(tiles * a.heads, a.workers), at = head * tiles + from;
+    const long long first = at / share, last = n ? (at + n - 1) / share : first - 1;
+    const long long oat = (long long)s * a.o_ts + (long long)h * a.o_hs;
+    auto store = [&](int d, float x) {
+        if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
+        else ((__half *)a.out)[oat + d] = __float2half_rn(x);
+    };
+    if (first == last) return;
+    if (n == 0) {
+        for (int d = threadIdx.x; d < a.d; d += kRdThreads) store(d, 0.f);
+        return;
+    }
+    const int parts = (int)(last - first + 1);
+    const long long id = first + (long long)head * a.seqs + s;
+    const float *lse = a.part_lse + id * a.rows + row, *po = a.part_o + (id * a.rows + row) * a.d;
+    float top = -INFINITY;
+    for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[(long long)i * a.rows]);
+    top = warp_max(top);
+    // a warp every fourth part, a lane four neighbouring elements (of 128 at a time)
+    float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+    float sum = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < parts; i += kRdWarps) {
+        const float w = lse[(long long)i * a.rows], f = w == -INFINITY ? 0.f : ex2(w - top);
+        sum += f;
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (k * 128 + lane * 4 < a.d) add_scaled(x[k], f, *(const float4 *)(po + (long long)i * a.rows * a.d + k * 128 + lane * 4));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) *(float4 *)&sums[warp][k * 128 + lane * 4] = x[k];
+    if (lane == 0) weights[warp] = sum;
+    __syncthreads();
+    const float all = 1.f / (weights[0] + weights[1] + weights[2] + weights[3]);
+    for (int d = threadIdx.x; d < a.d; d += kRdThreads) store(d, (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) * all);
+}
+
+// --------------------------------------------------------------- host ---
+
+// How a call is computed: query heads of a block of a group, how many blocks, and
+// the workspace.
+struct ReadPlan {
+    int nt, zs, heads, rows, workers;
+    uint64_t lse_at, o_at, bytes;
+};
+
+constexpr int kRdBlocks = 2;  // of an SM
+
+static ReadPlan read_plan(uint32_t seqs, uint32_t kv_heads, uint32_t group, uint32_t d)
+{
+    ReadPlan w;
+    w.nt = group > 8 && d <= 128 ? 2 : 1;  // with heads of 256 the results of 16 would not fit the registers
+    w.zs = (int)(group + 8 * w.nt - 1) / (8 * w.nt);
+    w.heads = (int)kv_heads * w.zs;
+    w.rows = (int)std::min<uint32_t>(group, 8 * w.nt);
+    w.workers = kRdBlocks * tc_sm_count() * kRdWarps;
+    const uint64_t parts = (uint64_t)w.workers + (uint64_t)w.heads * seqs;
+    auto up = [](uint64_t x) { return (x + 31) / 32 * 32; };
+    w.lse_at = up((seqs + 1ull) * 8);
+    w.o_at = up(w.lse_at + parts * w.rows * 4);
+    w.bytes = w.o_at + parts * w.rows * d * 4 + 32;
+    return w;
+}
+
+template <typename T, bool KV4, int DC, int NT>
+static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
+{
+    // the deepest ring with which kRdBlocks blocks fit an SM
+    constexpr uint32_t one = kRdWarps * ReadTile<KV4, DC>::kStage, room = (228 * 1024 / kRdBlocks - 1024 - 2048) / one;
+    constexpr int stages = room > 6 ? 6 : room < 2 ? 2 : (int)room;
+    auto *fn = &read_kernel<T, KV4, DC, NT, stages>;
+    cudaError_t e = ensure_smem_attr((const void *)fn, stages * one);
+    if (e != cudaSuccess) return e;
+    e = launch_behind(fn, (unsigned)(a.workers / kRdWarps), kRdThreads, stages * one, s, a);
+    if (e != cudaSuccess) return e;
+    const JoinArgs j{a.out, a.o_ts, a.o_hs, a.before, a.part_lse, a.part_o, a.seqs, a.hq, a.group, a.d, a.zs, a.heads, a.rows, a.bf16,
+                     a.workers};
+    return launch_behind(read_join_kernel, (unsigned)((long long)a.seqs * a.hq), kRdThreads, 0, s, j);
+}
+
+static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const aie_heads &out, void *workspace)
+{
+    a.q = q.data; a.q_ts = q.token_stride; a.q_hs = q.head_stride;
+    a.out = out.data; a.o_ts = out.token_stride; a.o_hs = out.head_stride;
+    a.zs = w.zs; a.heads = w.heads; a.rows = w.rows; a.workers = w.workers;
+    char *ws = (char *)(((uintptr_t)workspace + 31) / 32 * 32);
+    a.before = (long long *)ws;
+    a.part_lse = (float *)(ws + w.lse_at);
+    a.part_o = (float *)(ws + w.o_at);
+}
+
+template <int DC>
+static cudaError_t read4_launch(const ReadArgs &a, int nt, cudaStream_t s)
+{
+    if constexpr (DC <= 4)
+        if (nt == 2) return read_launch<__half, true, DC, 2>(a, s);
+    return read_launch<__half, true, DC, 1>(a, s);
+}
+
+template <typename T>
+static cudaError_t read16_launch(const ReadArgs &a, int nt, cudaStream_t s)
+{
+    if (a.d > 128) return read_launch<T, false, 16, 1>(a, s);
+    if (a.d > 64) return nt == 2 ? read_launch<T, false, 8, 2>(a, s) : read_launch<T, false, 8, 1>(a, s);
+    return nt == 2 ? read_launch<T, false, 4, 2>(a, s) : read_launch<T, false, 4, 1>(a, s);
+}
+
+}  // namespace aie

@@ -177,7 +177,14 @@ template <typename T>
 static cudaError_t attn_prompt_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
                                       unsigned grid, cudaStream_t s)
 {
-    return a.d <= 64 ? attn_launch<T, 1, false>(q, k, v, a, grid, s) : attn_launch<T, 2, false>(q, k, v, a, grid, s);
+    return a.d <= 64 ? attn_launch<T, 1, kAtPrompt>(q, k, v, a, grid, s) : attn_launch<T, 2, kAtPrompt>(q, k, v, a, grid, s);
+}
+
+// What 16-bit results are aligned to in every row.
+static int out_bytes(const aie_heads &out, uint32_t head_dim)
+{
+    const uint64_t bits = (uintptr_t)out.data | 2 * out.token_stride | 2 * out.head_stride;
+    return bits % 32 == 0 && head_dim % 16 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
 }
 
 static int prompt_tc(const aie_prompt &p, cudaStream_t s)
@@ -190,8 +197,7 @@ static int prompt_tc(const aie_prompt &p, cudaStream_t s)
     a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
     a.causal = p.causal != 0;
-    const uint64_t bits = (uintptr_t)p.out.data | 2 * p.out.token_stride | 2 * p.out.head_stride;
-    a.out_bytes = bits % 32 == 0 && p.head_dim % 16 == 0 ? 32 : bits % 16 == 0 ? 16 : 2;
+    a.out_bytes = out_bytes(p.out, p.head_dim);
     a.scale_log2 = p.scale * 1.4426950408889634f;
     const bool bf16 = p.dtype == AIE_DT_BF16;
     CUtensorMap q, k, v;
@@ -309,7 +315,7 @@ template <typename T>
 static cudaError_t attn_prefix_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
                                       unsigned grid, cudaStream_t s)
 {
-    return a.d <= 64 ? attn_launch<T, 1, true>(q, k, v, a, grid, s) : attn_launch<T, 2, true>(q, k, v, a, grid, s);
+    return a.d <= 64 ? attn_launch<T, 1, kAtPaged>(q, k, v, a, grid, s) : attn_launch<T, 2, kAtPaged>(q, k, v, a, grid, s);
 }
 
 // The cache's maps, for both parts: boxes inside one page, whole boxes to both
@@ -450,11 +456,76 @@ static bool cross_read_ok(const aie_cross &p)
            (uint64_t)p.seqs * p.q_heads <= 0x7fffffffull;
 }
 
+// Whether packed tokens go over the states on the tensor cores.
+static bool cross_tc_ok(const aie_cross &p)
+{
+    return p.keys && attn_heads_ok(p.dtype, p.q_heads, p.kv_heads, p.head_dim, p.scale) && p.cu_q &&
+           attn_addressable(p.q.data, p.q.token_stride, p.q.head_stride, p.tokens, p.q_heads) &&
+           attn_addressable(p.k.data, p.k.token_stride, p.k.head_stride, p.keys, p.kv_heads) &&
+           attn_addressable(p.v.data, p.v.token_stride, p.v.head_stride, p.keys, p.kv_heads);
+}
+
+// No more pairs of tiles than whole ones, and one that is not whole per
+// sequence.  Where they fill the SMs less than twice, their steps are cut.
+struct CrossPlan {
+    int capacity;
+    uint64_t pairs, grid, bytes;
+};
+
+static CrossPlan cross_plan(const aie_cross &p)
+{
+    CrossPlan w = {};
+    const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads), sms = tc_sm_count();
+    w.pairs = p.tokens / (2 * tpt) + std::min(p.seqs, p.tokens);
+    if (w.pairs * p.kv_heads < 2ull * sms) w.capacity = std::max(1, sms / (int)p.kv_heads);
+    w.grid = (w.pairs + w.capacity) * p.kv_heads;
+    w.bytes = 64 + (w.capacity ? w.grid * 2 * kAtTile * (p.head_dim + 1) * 4 : 0);
+    return w;
+}
+
 extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p)
 {
     if (check_cross(p)) return 0;
     if (cross_read_ok(*p)) return read_plan(p->seqs, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
-    return 64;
+    return cross_tc_ok(*p) ? cross_plan(*p).bytes : 64;
+}
+
+template <typename T>
+static cudaError_t attn_cross_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
+                                     const CrossPlan &w, cudaStream_t s)
+{
+    cudaError_t e = a.d <= 64 ? attn_launch<T, 1, kAtCross>(q, k, v, a, (unsigned)w.grid, s)
+                              : attn_launch<T, 2, kAtCross>(q, k, v, a, (unsigned)w.grid, s);
+    if (e != cudaSuccess || !a.capacity) return e;
+    return launch_behind(cross_join_kernel<T>, (unsigned)(w.pairs * a.kv_heads * 8), 256, 0, s, a);
+}
+
+static int cross_tc(const aie_cross &p, cudaStream_t s)
+{
+    const CrossPlan w = cross_plan(p);
+    if (w.grid > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "too many tiles");
+    AttnArgs a = {};
+    a.cu = p.cu_q; a.cu_k = p.cu_k;
+    a.out = p.out.data;
+    a.out_ts = p.out.token_stride; a.out_hs = p.out.head_stride;
+    char *ws = (char *)(((uintptr_t)p.workspace + 31) / 32 * 32);
+    a.part_o = (float *)ws;
+    a.part_lse = (float *)(ws + (w.capacity ? w.grid * 2 * kAtTile * p.head_dim * 4 : 0));
+    a.tokens = (int)p.tokens; a.seqs = (int)p.seqs; a.keys = (int)p.keys; a.capacity = w.capacity;
+    a.splits = (int)(w.grid / p.kv_heads);
+    a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
+    a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
+    a.out_bytes = out_bytes(p.out, p.head_dim);
+    a.scale_log2 = p.scale * 1.4426950408889634f;
+    const bool bf16 = p.dtype == AIE_DT_BF16;
+    CUtensorMap q, k, v;
+    if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.tokens, p.q.token_stride, 0, 0, a.group,
+                  a.tokens_per_tile) ||
+        !attn_map(&k, bf16, p.k.data, p.head_dim, p.kv_heads, p.k.head_stride, p.keys, p.k.token_stride, 0, 0, 1, kAtTile) ||
+        !attn_map(&v, bf16, p.v.data, p.head_dim, p.kv_heads, p.v.head_stride, p.keys, p.v.token_stride, 0, 0, 1, kAtTile))
+        return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
+    return launched(bf16 ? attn_cross_launch<__nv_bfloat16>(q, k, v, a, w, s) : attn_cross_launch<__half>(q, k, v, a, w, s),
+                    "cross attention");
 }
 
 static int cross_read(const aie_cross &p, cudaStream_t s)
@@ -500,6 +571,7 @@ extern "C" int aie_cross_attn(const aie_cross *p, void *stream)
         return fail(AIE_E_INVALID, "workspace: %llu bytes, 16-byte aligned, are needed", (unsigned long long)need);
     cudaStream_t s = (cudaStream_t)stream;
     if (cross_read_ok(*p)) return cross_read(*p, s);
+    if (cross_tc_ok(*p)) return cross_tc(*p, s);
     if (p->dtype == AIE_DT_F32) return cross_rows<float>(*p, s);
     return p->dtype == AIE_DT_F16 ? cross_rows<__half>(*p, s) : cross_rows<__nv_bfloat16>(*p, s);
 }

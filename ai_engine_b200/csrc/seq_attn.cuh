@@ -1,5 +1,6 @@
 // Attention on the tensor cores (tcgen05, f16 / bf16 operands, f32 sums):
-// whole packed prompts, and the shared prefix of a batch of streams.
+// whole packed prompts, the shared prefix of a batch of streams, and packed
+// tokens over states of another length.
 //
 //   S = Q K^T,  P = e^(scale (S - m)),  l = sum P,  O = P V,  out = O / l
 //
@@ -31,6 +32,12 @@
 // below 2^-14 would lose bits and those below 2^-25 vanish, which adds up over
 // a long context (one key 22.6 binary orders above 32768 equal ones: 0.0058
 // for 0.0051).  Exponents only: no instruction more.
+//
+// Tokens over states (CROSS): where there are fewer pairs of tiles than SMs, a
+// pair's steps are cut into parts of about as many as make one wave of blocks;
+// each part leaves (O / l, log2 of the weights' sum), which cross_join_kernel
+// joins as the shared prefix's pieces are.  Every block works the cut out from
+// the sequences' lengths, which the host does not know.
 //
 // Every wait is bounded (1 s); on expiry the block records an error code,
 // waits for its copies in flight, frees its tensor memory and returns.
@@ -177,7 +184,14 @@ struct AttnArgs {
     int out_bytes;            // what `out` is aligned to, in every row: 32, 16 or less
     int shared, max_len, page_size, pages, box_rows, splits, tiles_per_split;
     float scale_log2;
+    const int32_t *cu_k;      // states: the sequences' starts
+    int keys;                 // packed states
+    // splits: parts that there is room for
+    int capacity;             // blocks of a key head that run at once; 0: steps are not cut
 };
+
+constexpr int kAtPrompt = 0, kAtPaged = 1, kAtCross = 2;  // what attn_tc_kernel attends to
+constexpr int kAtLeast = 4;  // steps that a block is worth starting for: its start and end take about 3
 
 template <int DB>
 struct AttnSmem {
@@ -190,7 +204,7 @@ struct AttnSmem {
 struct AttnShared {
     uint64_t q_full, kv_full[8], kv_empty[8], s_full[2], p_full[2][2], o_full[2], drain;
     uint32_t tmem, abort;
-    int seq_first, seq_len, pair;
+    int seq_first, seq_len, pair, key_first, key_len, part, parts, per;
 };
 
 // What one block does: tile pair `pair` of tokens first .. first + len.
@@ -198,11 +212,100 @@ struct AttnWork {
     int first, len, pair, kvh, split;
 };
 
-template <typename T, int DB, bool PAGED>
+// A pair of tiles of tokens over states, and its share of their steps: part
+// `part` of `parts`, `per` steps each; base is the number of its first part.
+struct CrossWork {
+    int first, len, pair, key_first, key_len, part, parts, per;
+    long long base;
+};
+
+// By one warp: the pair with number `pair` among all, or the part with number
+// `unit` among all pairs' parts (the other is -1).  128 sequences at a time, 4 a
+// lane.  Only the lane that returns true has it.
+__device__ __forceinline__ bool cross_find(const AttnArgs &a, int unit, int pair, int lane, CrossWork &w)
+{
+    const int two = 2 * a.tokens_per_tile;
+    int start[4], len[4], key[4], key_len[4], pairs[4], steps[4];
+    auto load = [&](int s0) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int s = min(s0 + 4 * lane + i, a.seqs), next = min(s + 1, a.seqs);
+            start[i] = min(max(a.cu[s], 0), a.tokens);
+            len[i] = max(min(max(a.cu[next], 0), a.tokens) - start[i], 0);
+            key[i] = min(max(a.cu_k[s], 0), a.keys);
+            key_len[i] = max(min(max(a.cu_k[next], 0), a.keys) - key[i], 0);
+            pairs[i] = (len[i] + two - 1) / two;
+            steps[i] = (key_len[i] + kAtTile - 1) / kAtTile;
+        }
+    };
+    int per = 0x7fffffff;  // steps of a part
+    if (a.capacity) {
+        long long work = 0, n = 0;
+        for (int s0 = 0; s0 < a.seqs; s0 += 128) {
+            load(s0);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                work += (long long)pairs[i] * steps[i];
+                n += pairs[i];
+            }
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            work += __shfl_xor_sync(0xffffffffu, work, o);
+            n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
+        // a pair's last part is not full: room for one more each, where there is any
+        const long long room = a.capacity > 2 * n ? a.capacity - n : a.capacity;
+        per = (int)min(max((work + room - 1) / room, (long long)kAtLeast), 0x7fffffffll);
+    }
+    long long units_before = 0;
+    int pairs_before = 0;
+    for (int s0 = 0; s0 < a.seqs; s0 += 128) {
+        if (s0 || a.seqs > 128 || !a.capacity) load(s0);
+        int sum = 0, sum_units = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            sum += pairs[i];
+            sum_units += pairs[i] * max((steps[i] + per - 1ll) / per, 1ll);
+        }
+        int upto = sum, upto_units = sum_units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o), z = __shfl_up_sync(0xffffffffu, upto_units, o);
+            if (lane >= o) {
+                upto += y;
+                upto_units += z;
+            }
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, unit >= 0 ? unit < units_before + upto_units : pair < pairs_before + upto);
+        if (hit) {
+            if (lane != __ffs(hit) - 1) return false;
+            long long u = units_before + upto_units - sum_units;
+            int n = pairs_before + upto - sum;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int parts = (int)max((steps[i] + per - 1ll) / per, 1ll);
+                if (unit >= 0 ? unit >= u && unit < u + pairs[i] * parts : pair >= n && pair < n + pairs[i]) {
+                    const int in = unit >= 0 ? (int)(unit - u) : (pair - n) * parts;
+                    w = CrossWork{start[i], len[i], in / parts, key[i], key_len[i], in % parts, parts, per, u + in / parts * parts};
+                }
+                u += pairs[i] * parts;
+                n += pairs[i];
+            }
+            return true;
+        }
+        units_before += __shfl_sync(0xffffffffu, upto_units, 31);
+        pairs_before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    return false;
+}
+
+template <typename T, int DB, int MODE>
 __global__ void __launch_bounds__(kAtThreads, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const AttnArgs a)
 {
+    constexpr bool PAGED = MODE == kAtPaged, CROSS = MODE == kAtCross;
     using Sm = AttnSmem<DB>;
     extern __shared__ char smem_raw[];
     __shared__ AttnShared sh;
@@ -250,6 +353,22 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         w.pair = unit / a.splits;
         w.first = 0;
         w.len = a.tokens;
+    } else if constexpr (CROSS) {
+        if (warp == 0) {
+            if (lane == 0) sh.seq_len = 0;
+            __syncwarp();
+            CrossWork c;
+            if (cross_find(a, unit, -1, lane, c)) {
+                sh.seq_first = c.first;
+                sh.seq_len = c.len;
+                sh.pair = c.pair;
+                sh.key_first = c.key_first;
+                sh.key_len = c.key_len;
+                sh.part = c.part;
+                sh.parts = c.parts;
+                sh.per = c.per;
+            }
+        }
     } else {
         w.split = 0;
         if (warp == 0) {
@@ -301,6 +420,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         w.first = sh.seq_first;
         w.len = sh.seq_len;
         w.pair = sh.pair;
+        if constexpr (CROSS) w.split = sh.part;
         if (w.len == 0) {  // a block past the last pair
             if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
             return;
@@ -308,13 +428,15 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     }
     // keys seen by a tile's last token; `keys` also bounds the values that exist
     const int tok0 = w.pair * 2 * tpt;
-    const int keys = PAGED ? min(a.shared, a.max_len) : w.len;
-    const int step0 = PAGED ? w.split * a.tiles_per_split : 0;
+    const int keys = PAGED ? min(a.shared, a.max_len) : CROSS ? sh.key_len : w.len;
+    const int key_first = CROSS ? sh.key_first : w.first;
+    const int per_split = PAGED ? a.tiles_per_split : CROSS ? sh.per : 0, step0 = w.split * per_split;
+    const bool parts = PAGED || (CROSS && sh.parts > 1);  // a partial result, not the result
     auto steps_of = [&](int t) {
         const int first = tok0 + t * tpt, last = min(first + tpt, w.len);
-        const int seen = first >= w.len ? 0 : (!PAGED && a.causal) ? last : keys;
+        const int seen = first >= w.len ? 0 : (MODE == kAtPrompt && a.causal) ? last : keys;
         const int steps = (seen + kAtTile - 1) / kAtTile;
-        return PAGED ? max(min(steps, step0 + a.tiles_per_split), step0) : steps;
+        return MODE != kAtPrompt ? max(min(steps - step0, per_split), 0) + step0 : steps;
     };
     const int n0 = steps_of(0), n1 = steps_of(1), n = max(n0, n1);
     auto n_of = [&](int t) { return t ? n1 : n0; };
@@ -335,7 +457,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         int seen = keys;
         if constexpr (PAGED) {
             if (real) seen = min(seen, max(a.lens[tok], 0));
-        } else {
+        } else if constexpr (!CROSS) {
             if (a.causal) seen = min(tok + 1, keys);
         }
         const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * 128, to = ts + 256;
@@ -415,15 +537,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const float l = l2.x + l2.y;
         if (nt > step0 && ok) ok = __all_sync(0xffffffffu, wait(&sh.o_full[t], 0, 8));
         tc_fence_after();
-        if (ok && (nt > step0 || PAGED)) {
+        if (ok && (nt > step0 || MODE != kAtPrompt)) {
             // of this split's keys; scores of -inf alone (l is 0) count as none here
-            const bool none = nt <= step0 || seen <= step0 * kAtTile || (PAGED && l == 0.f);
+            const bool none = nt <= step0 || seen <= step0 * kAtTile || (parts && l == 0.f);
             const float r = none ? 0.f : 1.f / l;
-            const long long prow = PAGED ? ((long long)w.split * a.tokens + tok) * a.q_heads + head : 0;
+            const long long prow = PAGED   ? ((long long)w.split * a.tokens + tok) * a.q_heads + head
+                                   : CROSS ? (long long)blockIdx.x * (2 * kAtTile) + t * kAtTile + row
+                                           : 0;
             // 32 columns at a time out of tensor memory: a thread holds a row and
             // writes whole 32-byte sectors of it (16-byte pieces: 2 us a tile, so: 1)
-            const long long at = PAGED ? prow * a.d : (w.first + tok) * a.out_ts + head * a.out_hs;
-            if constexpr (PAGED) {
+            const long long at = parts ? prow * a.d : (w.first + tok) * a.out_ts + head * a.out_hs;
+            if (MODE != kAtPrompt && parts) {
                 // log2 of the weights' sum; -inf where nothing was seen
                 if (real) a.part_lse[prow] = none ? -INFINITY : fmaf(m, sl, log2f(l) - kWeightShift<T>);
             }
@@ -446,6 +570,9 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                         if (32 * c + i >= a.d) break;
                         if constexpr (PAGED) {
                             store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
+                        } else if (CROSS && parts) {
+                            store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
+                            if (32 * c + i + 8 < a.d) store32(a.part_o + at + 32 * c + i + 8, (const uint32_t *)&o[i + 8]);
                         } else {
                             T *dst = (T *)a.out + at + 32 * c + i;
                             uint32_t v[8];
@@ -517,7 +644,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                             (step * kAtTile + lane * rows) % a.page_size, page);
                     } else if (lane == 0) {
                         for (int b = 0; b < DB; b++)
-                            tma_load_3d(dst + b * kAtBlockBytes, tm, &sh.kv_full[st], b * 64, w.kvh, w.first + step * kAtTile);
+                            tma_load_3d(dst + b * kAtBlockBytes, tm, &sh.kv_full[st], b * 64, w.kvh, key_first + step * kAtTile);
                     }
                     issued = i + 1;
                 }
@@ -636,6 +763,55 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     }
 }
 
+// Pairs of tiles whose steps were cut: the parts' results joined, 32 rows a block.
+template <typename T>
+__global__ void __launch_bounds__(256) cross_join_kernel(const AttnArgs a)
+{
+    __shared__ CrossWork shared;
+    __shared__ int found;
+    behind_last_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int kvh = blockIdx.x % a.kv_heads, rows0 = blockIdx.x / a.kv_heads % 8 * 32, pair = blockIdx.x / a.kv_heads / 8;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    if (warp == 0) {
+        CrossWork c;
+        if (cross_find(a, -1, pair, lane, c)) {
+            shared = c;
+            found = 1;
+        }
+    }
+    __syncthreads();
+    // (the second only where cu is no list of starts, and parts are missing)
+    if (!found || shared.parts == 1 || shared.base + shared.parts > a.splits) return;
+    const CrossWork w = shared;
+    for (int i = rows0 + warp; i < rows0 + 32; i += 8) {
+        const int t = i / kAtTile, row = i % kAtTile, tok = (w.pair * 2 + t) * a.tokens_per_tile + row / a.group;
+        const int head = kvh * a.group + row % a.group;
+        if (row >= a.tokens_per_tile * a.group || tok >= w.len) continue;
+        auto at = [&](int part) { return ((w.base + part) * a.kv_heads + kvh) * (2 * kAtTile) + i; };
+        float top = -INFINITY;
+        for (int part = lane; part < w.parts; part += 32) top = fmaxf(top, a.part_lse[at(part)]);
+        top = warp_max(top);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float sum = 0.f;
+#pragma unroll 4
+        for (int part = 0; part < w.parts; part++) {
+            const float lse = a.part_lse[at(part)], f = lse == -INFINITY ? 0.f : ex2(lse - top);
+            sum += f;
+            if (lane * 4 < a.d) {
+                const float4 y = *(const float4 *)(a.part_o + at(part) * a.d + lane * 4);
+                x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+            }
+        }
+        const float f = 1.f / sum;
+        T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs + lane * 4;
+        if (lane * 4 < a.d) {
+            dst[0] = from_f32<T>(x.x * f); dst[1] = from_f32<T>(x.y * f); dst[2] = from_f32<T>(x.z * f); dst[3] = from_f32<T>(x.w * f);
+        }
+    }
+}
+
 // --------------------------------------------------------------- host ---
 
 // A [tokens][heads][d] tensor, or pages of it, as a tensor map with boxes of
@@ -662,11 +838,11 @@ static inline bool attn_map(CUtensorMap *tm, bool bf16, const void *p, uint32_t 
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DB, bool PAGED>
+template <typename T, int DB, int MODE>
 static cudaError_t attn_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
                                unsigned grid, cudaStream_t s)
 {
-    auto *fn = &attn_tc_kernel<T, DB, PAGED>;
+    auto *fn = &attn_tc_kernel<T, DB, MODE>;
     cudaError_t e = ensure_smem_attr((const void *)fn, AttnSmem<DB>::kBytes);
     if (e != cudaSuccess) return e;
     return launch_behind(fn, grid, kAtThreads, AttnSmem<DB>::kBytes, s, q, k, v, a);

@@ -486,7 +486,7 @@ static CrossPlan cross_plan(const aie_cross &p)
 extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p)
 {
     if (check_cross(p)) return 0;
-    if (cross_read_ok(*p)) return read_plan(p->seqs, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
+    if (cross_read_ok(*p)) return read_plan(false, p->seqs, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
     return cross_tc_ok(*p) ? cross_plan(*p).bytes : 64;
 }
 
@@ -497,7 +497,7 @@ static cudaError_t attn_cross_launch(const CUtensorMap &q, const CUtensorMap &k,
     cudaError_t e = a.d <= 64 ? attn_launch<T, 1, kAtCross>(q, k, v, a, (unsigned)w.grid, s)
                               : attn_launch<T, 2, kAtCross>(q, k, v, a, (unsigned)w.grid, s);
     if (e != cudaSuccess || !a.capacity) return e;
-    return launch_behind(cross_join_kernel<T>, (unsigned)(w.pairs * a.kv_heads * 8), 256, 0, s, a);
+    return launch_behind(cross_join_kernel<T>, (unsigned)(w.pairs * a.kv_heads * (2 * kAtTile / kJoinRows)), 32 * kJoinRows, 0, s, a);
 }
 
 static int cross_tc(const aie_cross &p, cudaStream_t s)
@@ -531,7 +531,7 @@ static int cross_tc(const aie_cross &p, cudaStream_t s)
 static int cross_read(const aie_cross &p, cudaStream_t s)
 {
     ReadArgs a = {};
-    const ReadPlan w = read_plan(p.seqs, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
+    const ReadPlan w = read_plan(false, p.seqs, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
     read_args(a, w, p.q, p.out, p.workspace);
     a.k = p.k.data; a.k_ts = p.k.token_stride; a.k_hs = p.k.head_stride;
     a.v = p.v.data; a.v_ts = p.v.token_stride; a.v_hs = p.v.head_stride;
@@ -628,7 +628,7 @@ static int check_kv4_step(const aie_kv4_step *p)
 
 static ReadPlan kv4_plan(const aie_kv4_step &p)
 {
-    return read_plan(p.batch, p.cache.kv_heads, p.q_heads / p.cache.kv_heads, p.cache.head_dim);
+    return read_plan(true, p.batch, p.cache.kv_heads, p.q_heads / p.cache.kv_heads, p.cache.head_dim);
 }
 
 extern "C" uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p) { return check_kv4_step(p) ? 0 : kv4_plan(*p).bytes; }

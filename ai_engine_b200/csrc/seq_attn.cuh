@@ -763,15 +763,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     }
 }
 
-// Pairs of tiles whose steps were cut: the parts' results joined, 32 rows a block.
+// Pairs of tiles whose steps were cut: the parts' results joined, a warp per row.
+constexpr int kJoinRows = 8;  // of a block
 template <typename T>
-__global__ void __launch_bounds__(256) cross_join_kernel(const AttnArgs a)
+__global__ void __launch_bounds__(32 * kJoinRows) cross_join_kernel(const AttnArgs a)
 {
     __shared__ CrossWork shared;
     __shared__ int found;
     behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int kvh = blockIdx.x % a.kv_heads, rows0 = blockIdx.x / a.kv_heads % 8 * 32, pair = blockIdx.x / a.kv_heads / 8;
+    const int kvh = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
+    const int i = unit % (2 * kAtTile / kJoinRows) * kJoinRows + warp, pair = unit / (2 * kAtTile / kJoinRows);
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
     if (warp == 0) {
@@ -782,33 +784,36 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const AttnArgs a)
         }
     }
     __syncthreads();
-    // (the second only where cu is no list of starts, and parts are missing)
+    // (the last only where cu is no list of starts, and parts are missing)
     if (!found || shared.parts == 1 || shared.base + shared.parts > a.splits) return;
     const CrossWork w = shared;
-    for (int i = rows0 + warp; i < rows0 + 32; i += 8) {
-        const int t = i / kAtTile, row = i % kAtTile, tok = (w.pair * 2 + t) * a.tokens_per_tile + row / a.group;
-        const int head = kvh * a.group + row % a.group;
-        if (row >= a.tokens_per_tile * a.group || tok >= w.len) continue;
-        auto at = [&](int part) { return ((w.base + part) * a.kv_heads + kvh) * (2 * kAtTile) + i; };
-        float top = -INFINITY;
-        for (int part = lane; part < w.parts; part += 32) top = fmaxf(top, a.part_lse[at(part)]);
-        top = warp_max(top);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        float sum = 0.f;
-#pragma unroll 4
-        for (int part = 0; part < w.parts; part++) {
-            const float lse = a.part_lse[at(part)], f = lse == -INFINITY ? 0.f : ex2(lse - top);
-            sum += f;
+    const int t = i / kAtTile, row = i % kAtTile, tok = (w.pair * 2 + t) * a.tokens_per_tile + row / a.group;
+    const int head = kvh * a.group + row % a.group;
+    if (row >= a.tokens_per_tile * a.group || tok >= w.len) return;
+    const long long first = (w.base * a.kv_heads + kvh) * (2 * kAtTile) + i, next = a.kv_heads * (2 * kAtTile);
+    float top = -INFINITY;
+    for (int part = lane; part < w.parts; part += 32) top = fmaxf(top, a.part_lse[first + part * next]);
+    top = warp_max(top);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float sum = 0.f;
+    const float *po = a.part_o + first * a.d + lane * 4;
+    for (int part0 = 0; part0 < w.parts; part0 += 32) {
+        const int n = min(w.parts - part0, 32);
+        const float lse = lane < n ? a.part_lse[first + (part0 + lane) * next] : -INFINITY, mine = lse == -INFINITY ? 0.f : ex2(lse - top);
+        sum += mine;
+#pragma unroll 8
+        for (int k = 0; k < n; k++) {
+            const float f = __shfl_sync(0xffffffffu, mine, k);
             if (lane * 4 < a.d) {
-                const float4 y = *(const float4 *)(a.part_o + at(part) * a.d + lane * 4);
+                const float4 y = *(const float4 *)(po + (part0 + k) * next * a.d);
                 x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
             }
         }
-        const float f = 1.f / sum;
-        T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs + lane * 4;
-        if (lane * 4 < a.d) {
-            dst[0] = from_f32<T>(x.x * f); dst[1] = from_f32<T>(x.y * f); dst[2] = from_f32<T>(x.z * f); dst[3] = from_f32<T>(x.w * f);
-        }
+    }
+    const float f = 1.f / warp_sum(sum);
+    T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs + lane * 4;
+    if (lane * 4 < a.d) {
+        dst[0] = from_f32<T>(x.x * f); dst[1] = from_f32<T>(x.y * f); dst[2] = from_f32<T>(x.z * f); dst[3] = from_f32<T>(x.w * f);
     }
 }
 

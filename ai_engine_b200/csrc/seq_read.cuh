@@ -24,8 +24,8 @@
 //
 // Rounding to fewer bits: the weights to 16 bits for the product with V (l sums
 // them unrounded; f16 weights 2^7 times as large, as in attn_tc_kernel), the
-// result, and over the 4-bit cache lo + code s to f16 for that product, by
-// 2^-12 of it, where the weights lose as much.
+// result, and over the 4-bit cache the weights times the scales to f16 for the
+// product with the codes.
 #pragma once
 #include "seq_kv4.cuh"
 #include "seq_step.cuh"
@@ -93,28 +93,26 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x)
     return y;
 }
 
-// (x & mask) | one, two halves at a time
-__device__ __forceinline__ uint32_t pick(uint32_t x, uint32_t mask, uint32_t one)
-{
-    uint32_t y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(one));
-    return y;
-}
-
-// Four codes of each half of a word as f16 pairs: code i of the lower half and of
-// the upper.  A code in an f16's fraction, four bits under 16 or eight under
-// 256, is that number plus the code.
+// The four codes of each half of a word as f16 pairs, code i of the lower half and
+// of the upper.  A code in the lowest bits of an f16 is that many times 2^-24, a
+// subnormal, which the products take as it is: exact, at one instruction a pair.
+// The odd ones stand four bits higher, 16 times as large.
 struct Codes {
-    uint32_t p[4];  // 256 + code 0, 16 + code 1, 256 + code 2, 16 + code 3
+    uint32_t p[4];
     __device__ __forceinline__ Codes(uint32_t w)
     {
-        const uint32_t lo = w << 2, hi = w >> 6;
-        p[0] = pick(lo, 0x003C003Cu, 0x5C005C00u);
-        p[1] = pick(lo, 0x03C003C0u, 0x4C004C00u);
-        p[2] = pick(hi, 0x003C003Cu, 0x5C005C00u);
-        p[3] = pick(hi, 0x03C003C0u, 0x4C004C00u);
+        p[0] = w & 0x000F000Fu;
+        p[1] = w & 0x00F000F0u;
+        p[2] = w >> 8 & 0x000F000Fu;
+        p[3] = w >> 8 & 0x00F000F0u;
     }
 };
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
+{
+    const __half2 y = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&y;
+}
 
 // N 32-bit words of shared memory from an address aligned to the whole of them.
 template <int N>
@@ -152,11 +150,17 @@ struct ReadTile {
     static constexpr uint32_t kStage = 2 * kSide + 2 * kPairs;
 };
 
+// Blocks of an SM.
+constexpr int read_blocks(bool kv4, int dc, int nt) { return nt == 1 && dc <= 4 ? 3 : 2; }
+
 // T: the operands' type, f16 in 4 bits.
 template <typename T, bool KV4, int DC, int NT, int STAGES>
-__global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
+__global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_kernel(const ReadArgs a)
 {
     using Tile = ReadTile<KV4, DC>;
+    // binary orders by which weights are held larger: in 4 bits they are also
+    // multiplied with scales below 8, and 2^8 2^4 8 is what f16 holds
+    constexpr float kShift = KV4 ? 4.f : kWeightShift<T>;
     constexpr int MT = Tile::kKeys / 16, OT = KV4 ? 2 * DC : DC;  // tiles of 16 keys; of 16 elements of V
     extern __shared__ __align__(16) char smem[];
     __shared__ long long scan[kRdThreads], warp_sum_[kRdWarps];
@@ -234,16 +238,17 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
 
     // ---- copies
     Place ahead = at;
-    long long page_at = 0;  // 4 bits: a lane's page (of 8 places of the tile), and the first place in it
-    int page_place = 0;
-    bool page_real = false;
+    // 4 bits: where a lane's 8 places of the tile (of lane & 3) have their codes and their pairs; -1: no such page
+    long long codes_at = 0, pairs_at = 0;
     auto look_up = [&] {
         if constexpr (KV4) {
             const int place = ahead.tile * Tile::kKeys + (lane & 3) * 8, i = fdiv(place, a.size);
             const int page = place < ahead.len ? a.table[(long long)ahead.s * a.table_stride + i] : -1;
-            page_real = page >= 0 && page < a.g.pages;
-            page_at = page_real ? page * a.g.page_stride + (ahead.head / a.zs) * a.g.block() : 0;
-            page_place = place - i * a.g.size;
+            const long long block = page * a.g.page_stride + (ahead.head / a.zs) * a.g.block();
+            const int in = place - i * a.g.size;
+            const bool real = page >= 0 && page < a.g.pages;
+            codes_at = real ? block + in * (16 * DC) : -1;
+            pairs_at = real ? block + (long long)a.g.size * (16 * DC) + in * (4 * DC) : -1;
         }
     };
     auto copy_tile = [&](int stage) {
@@ -252,37 +257,23 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
         if constexpr (KV4) {
 #pragma unroll
             for (int i = 0; i < DC; i++) {
-                const int c = i * 32 + lane, row = c / DC, piece = c - row * DC, eight = row >> 3;
-                const long long off = __shfl_sync(0xffffffffu, page_at, eight) +
-                                      (__shfl_sync(0xffffffffu, page_place, eight) + (row & 7)) * (16 * DC) + piece * 16;
-                const int n = __shfl_sync(0xffffffffu, (int)page_real, eight) && row < rows ? 16 : 0;
+                const int c = i * 32 + lane, row = c / DC, piece = c - row * DC, eight = c / (8 * DC);
+                const long long from = __shfl_sync(0xffffffffu, codes_at, eight);
+                const int n = from >= 0 && row < rows ? 16 : 0;
+                const long long off = n ? from + (c - eight * 8 * DC) * 16 : 0;
                 copy16(dst + row * Tile::kRow + piece * 16, a.g.k + off, n);
                 copy16(dst + Tile::kSide + row * Tile::kRow + piece * 16, a.g.v + off, n);
             }
-            // pairs: 16 bytes a lane, DC * 2 lanes to 8 places
-            const int eight = min(lane / (2 * DC), 3), in = lane * 16 - eight * 32 * DC;
-            const long long from = __shfl_sync(0xffffffffu, page_at, eight);
-            const int place = __shfl_sync(0xffffffffu, page_place, eight), real = __shfl_sync(0xffffffffu, (int)page_real, eight);
+            // pairs: 2 DC pieces to 8 places, one a lane
 #pragma unroll
             for (int i = 0; i < (DC + 3) / 4; i++) {
-                // heads of more than 128: another round of 32 lanes
-                const int c = i * 32 + lane;
-                if (DC > 4 || c < 8 * DC) {
-                    int e8 = eight, in_ = in, pl = place, re = real;
-                    long long fr = from;
-                    if constexpr (DC > 4) {
-                        e8 = min(c / (2 * DC), 3);
-                        in_ = c * 16 - e8 * 32 * DC;
-                        pl = __shfl_sync(0xffffffffu, page_place, e8);
-                        re = __shfl_sync(0xffffffffu, (int)page_real, e8);
-                        fr = __shfl_sync(0xffffffffu, page_at, e8);
-                    }
-                    if (c < 8 * DC) {
-                        const long long off = fr + (long long)a.g.size * (16 * DC) + pl * (4 * DC) + in_;
-                        const int n = re ? min(max((rows - e8 * 8) * 4 * DC - in_, 0), 16) : 0;
-                        copy16(dst + 2 * Tile::kSide + c * 16, a.g.k + off, n);
-                        copy16(dst + 2 * Tile::kSide + Tile::kPairs + c * 16, a.g.v + off, n);
-                    }
+                const int c = i * 32 + lane, eight = min(c / (2 * DC), 3), in = (c - eight * 2 * DC) * 16;
+                const long long from = __shfl_sync(0xffffffffu, pairs_at, eight);
+                if (c < 8 * DC) {
+                    const int n = from >= 0 ? min(max((rows - eight * 8) * 4 * DC - in, 0), 16) : 0;
+                    const long long off = n ? from + in : 0;
+                    copy16(dst + 2 * Tile::kSide + c * 16, a.g.k + off, n);
+                    copy16(dst + 2 * Tile::kSide + Tile::kPairs + c * 16, a.g.v + off, n);
                 }
             }
         } else {
@@ -315,10 +306,11 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
     // ---- products
     const int r = lane >> 2, c2 = (lane & 3) * 2;  // a lane's rows r, r + 8 and columns c2, c2 + 1 of a product
     const float sl = fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
-    uint32_t qb[NT][KV4 ? 2 * DC : DC][2];
-    float q_c[KV4 ? DC : 1][NT][2], q_sum[KV4 ? DC : 1][NT][2];  // 4 bits: what the codes' offsets add to a group, and its sum of q
-    float slq[NT][2];                                            // scale of a column's scores, in binary orders
+    uint32_t qb[NT][KV4 ? 2 * DC : DC][2], qs[NT][2];  // queries; 4 bits: each group's sum of them, in two f16
+    float slq[NT][2];                                  // scale of a column's scores, in binary orders
     float o[OT][NT][4], m[NT][2], l[NT][2];
+    float o_lo[KV4 ? NT : 1][4];  // 4 bits: the weighted sums of the groups' lo
+    int se = 0;                   // and 2^se .. 2^(se + 3), to which their scales go; o is in units of 2^(se - 24)
     bool fresh = true;
     int first_tile = 0, stage = 0;  // of the sequence's tiles; of the ring
     for (int i = 0; i < count; i++) {
@@ -352,30 +344,32 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
                     const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
 #pragma unroll
                     for (int g = 0; g < DC; g++) {
-                        float even = 0.f, odd = 0.f;
+                        float sum = 0.f;
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
-                            const float x = __half2float(__float2half_rn(f[g][e] * up));
-                            f[g][e] = x;
-                            if (e & 1) odd += x;
-                            else even += x;
+                            f[g][e] = __half2float(__float2half_rn(f[g][e] * up));
+                            sum += f[g][e];
                         }
+                        // element e + 4 is the same code of a word's upper half; odd codes are 16 times as large
 #pragma unroll
-                        for (int e = 0; e < 4; e++) qb[nt][2 * g + (e >> 1)][e & 1] = pack2<__half>(f[g][e], f[g][e + 4]);
-                        float cc = fmaf(256.f, even, 16.f * odd), su = even + odd;
-#pragma unroll
-                        for (int x = 1; x < 4; x <<= 1) {
-                            cc += __shfl_xor_sync(0xffffffffu, cc, x);
-                            su += __shfl_xor_sync(0xffffffffu, su, x);
+                        for (int e = 0; e < 4; e++) {
+                            const float x = e & 1 ? 0.0625f : 1.f;
+                            qb[nt][2 * g + (e >> 1)][e & 1] = pack2<__half>(f[g][e] * x, f[g][e + 4] * x);
                         }
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            q_c[g][nt][j] = __shfl_sync(0xffffffffu, cc, (c2 + j) * 4);
-                            q_sum[g][nt][j] = __shfl_sync(0xffffffffu, su, (c2 + j) * 4);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                        if (!(g & 3)) qs[nt][g >> 2] = 0u;
+                        if ((lane & 3) == (g & 3)) {
+                            const float hi = __half2float(__float2half_rn(sum));
+                            qs[nt][g >> 2] = pack2<__half>(hi, sum - hi);
                         }
                     }
+                    if (DC <= 4) qs[nt][1] = 0u;
 #pragma unroll
-                    for (int j = 0; j < 2; j++) slq[nt][j] = fmaxf(sl * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f);
+                    for (int j = 0; j < 2; j++)
+                        slq[nt][j] = fmaxf(sl * 0x1p24f * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f);
+                    o_lo[nt][0] = o_lo[nt][1] = o_lo[nt][2] = o_lo[nt][3] = 0.f;
+                    se = -100;  // none yet
                 } else {
                     const T *q = (const T *)a.q + qat;
 #pragma unroll
@@ -420,25 +414,39 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
             if constexpr (KV4) {
+                // S 2^-24 = sum over the groups of s (codes 2^-24) q, and of lo sum(q) 2^-24
                 const uint32_t *pk = (const uint32_t *)(st + 2 * Tile::kSide) + (mt * 16 + r) * DC;
                 uint32_t p0[DC], p1[DC];
                 shared_words<DC>(pk, p0);
                 shared_words<DC>(pk + 8 * DC, p1);
+                uint32_t low[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    // row r or r + 8, group lane & 3 or 4 further on
+                    const int g = (lane & 3) + (i >> 1) * 4;
+                    low[i] = g < DC ? __byte_perm(pk[(i & 1) * 8 * DC + g], 0, 0x3232) : 0u;
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    mma16816<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[mt][nt][j] *= 0x1p-24f;
+                }
 #pragma unroll
                 for (int g = 0; g < DC; g++) {
                     uint32_t w[2];
                     ldmatrix2(kt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
                     const Codes x0(w[0]), x1(w[1]);
-                    const float2 f0 = __half22float2(*(const __half2 *)&p0[g]), f1 = __half22float2(*(const __half2 *)&p1[g]);
+                    const float f0 = __half2float(__ushort_as_half((unsigned short)p0[g])), f1 = __half2float(__ushort_as_half((unsigned short)p1[g]));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float acc[4] = {-q_c[g][nt][0], -q_c[g][nt][1], -q_c[g][nt][0], -q_c[g][nt][1]};
+                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
                         mma16816<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
                         mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
-                            s[mt][nt][j] = fmaf(f0.x, acc[j], fmaf(f0.y, q_sum[g][nt][j], s[mt][nt][j]));
-                            s[mt][nt][2 + j] = fmaf(f1.x, acc[2 + j], fmaf(f1.y, q_sum[g][nt][j], s[mt][nt][2 + j]));
+                            s[mt][nt][j] = fmaf(f0, acc[j], s[mt][nt][j]);
+                            s[mt][nt][2 + j] = fmaf(f1, acc[2 + j], s[mt][nt][2 + j]);
                         }
                     }
                 }
@@ -486,6 +494,7 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
                     const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
                     m[nt][j] = x;
                     l[nt][j] *= f;
+                    if constexpr (KV4) o_lo[nt][j] *= f;
 #pragma unroll
                     for (int t = 0; t < OT; t++) {
                         o[t][nt][j] *= f;
@@ -498,7 +507,7 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
         for (int nt = 0; nt < NT; nt++) {
             float off[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], kWeightShift<T>);
+            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], kShift);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
                 float e[4];
@@ -511,37 +520,56 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
             }
         }
         // ---- values
+        uint32_t scale2 = 0;  // 2^-se, twice
+        if constexpr (KV4) {
+            // O = sum over the keys of (p s) codes, and of p lo.  The scales in f16 beside
+            // weights: brought to below 8 by a power of two that only moves when one is too large
+            uint32_t pv[DC];
+            shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
+            uint32_t most = 0;
+#pragma unroll
+            for (int g = 0; g < DC; g++) most = max(most, pv[g] & 0xffffu);
+            if (__any_sync(0xffffffffu, (int)(most >> 10) - 15 >= se + 3)) {
+                const int e = min(max((int)(__reduce_max_sync(0xffffffffu, most) >> 10) - 15, -14), 14);
+                const float f = se == -100 ? 1.f : __uint_as_float((uint32_t)(127 + se - e) << 23);
+                se = e;
+#pragma unroll
+                for (int t = 0; t < OT; t++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[t][nt][j] *= f;
+            }
+            scale2 = (uint32_t)(15 - se) * 0x04000400u;
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
             if constexpr (KV4) {
                 // (s, lo) of keys c2, c2 + 1 and of 8 further on, two keys to a register
                 const uint32_t *pv = (const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + (mt * 16 + c2) * DC;
-                uint32_t p0[DC], p1[DC], p2[DC], p3[DC];
+                uint32_t p0[DC], p1[DC], p2[DC], p3[DC], low[4] = {0u, 0u, 0u, 0u};
                 shared_words<DC>(pv, p0);
                 shared_words<DC>(pv + DC, p1);
                 shared_words<DC>(pv + 8 * DC, p2);
                 shared_words<DC>(pv + 9 * DC, p3);
+                if (r < DC) {  // row r: group r
+                    low[0] = __byte_perm(pv[r], pv[DC + r], 0x7632);
+                    low[2] = __byte_perm(pv[8 * DC + r], pv[9 * DC + r], 0x7632);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) mma16816<T>(o_lo[nt], low, pb[mt][nt][0], pb[mt][nt][1]);
 #pragma unroll
                 for (int g = 0; g < DC; g++) {
                     uint32_t w[2];
                     ldmatrix2_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
                     const Codes x0(w[0]), x1(w[1]);
-                    const uint32_t s0 = __byte_perm(p0[g], p1[g], 0x5410), l0 = __byte_perm(p0[g], p1[g], 0x7632);
-                    const uint32_t s1 = __byte_perm(p2[g], p3[g], 0x5410), l1 = __byte_perm(p2[g], p3[g], 0x7632);
-                    uint32_t v0[4], v1[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const __half2 less = __float2half2_rn(e & 1 ? -16.f : -256.f);
-                        const __half2 y0 = __hfma2(__hadd2(*(const __half2 *)&x0.p[e], less), *(const __half2 *)&s0, *(const __half2 *)&l0);
-                        const __half2 y1 = __hfma2(__hadd2(*(const __half2 *)&x1.p[e], less), *(const __half2 *)&s1, *(const __half2 *)&l1);
-                        v0[e] = *(const uint32_t *)&y0;
-                        v1[e] = *(const uint32_t *)&y1;
-                    }
-                    // rows r: elements 4 r + 0 (+ 2), rows r + 8: 4 r + 1 (+ 3)
+                    const uint32_t s0 = mul2(__byte_perm(p0[g], p1[g], 0x5410), scale2), s1 = mul2(__byte_perm(p2[g], p3[g], 0x5410), scale2);
+                    // rows r: elements 4 r + 0 (+ 2), rows r + 8: 4 r + 1 (+ 3), these 16 times as large
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        mma16816<T>(o[2 * g][nt], {v0[0], v0[1], v1[0], v1[1]}, pb[mt][nt][0], pb[mt][nt][1]);
-                        mma16816<T>(o[2 * g + 1][nt], {v0[2], v0[3], v1[2], v1[3]}, pb[mt][nt][0], pb[mt][nt][1]);
+                        const uint32_t b0 = mul2(pb[mt][nt][0], s0), b1 = mul2(pb[mt][nt][1], s1);
+                        mma16816<T>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
+                        mma16816<T>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
                     }
                 }
             } else {
@@ -570,6 +598,11 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
                     float sum = l[nt][j];
 #pragma unroll
                     for (int e = 4; e < 32; e <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
+                    float low[KV4 ? DC : 1];
+                    if constexpr (KV4) {
+#pragma unroll
+                        for (int g = 0; g < DC; g++) low[g] = __shfl_sync(0xffffffffu, o_lo[nt][j], g * 4 + (lane & 3));
+                    }
                     const int n = nt * 8 + c2 + j;
                     if (n >= heads) continue;
                     // of several parts, one with scores of -inf alone (the sum is 0) has no weight
@@ -577,13 +610,15 @@ __global__ void __launch_bounds__(kRdThreads) read_kernel(const ReadArgs a)
                     const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
-                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - kWeightShift<T>);
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - kShift);
 #pragma unroll
                     for (int t = 0; t < OT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int d = KV4 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 + e : t * 16 + e * 8 + r;
-                            const float x = o[t][nt][2 * e + j] * f;
+                            float x = o[t][nt][2 * e + j];
+                            if constexpr (KV4) x = fmaf(x, __uint_as_float((uint32_t)(127 + 24 + se - 4 * e) << 23), low[t >> 1]);
+                            x *= f;
                             if (!KV4 && d >= a.d) continue;
                             if (!whole) a.part_o[pat + d] = x;
                             else if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
@@ -660,16 +695,17 @@ struct ReadPlan {
     uint64_t lse_at, o_at, bytes;
 };
 
-constexpr int kRdBlocks = 2;  // of an SM
+// DC as the kernels are instantiated for it
+static int read_dc(bool kv4, uint32_t d) { return kv4 ? (int)d / 32 : d <= 64 ? 4 : d <= 128 ? 8 : 16; }
 
-static ReadPlan read_plan(uint32_t seqs, uint32_t kv_heads, uint32_t group, uint32_t d)
+static ReadPlan read_plan(bool kv4, uint32_t seqs, uint32_t kv_heads, uint32_t group, uint32_t d)
 {
     ReadPlan w;
     w.nt = group > 8 && d <= 128 ? 2 : 1;  // with heads of 256 the results of 16 would not fit the registers
     w.zs = (int)(group + 8 * w.nt - 1) / (8 * w.nt);
     w.heads = (int)kv_heads * w.zs;
     w.rows = (int)std::min<uint32_t>(group, 8 * w.nt);
-    w.workers = kRdBlocks * tc_sm_count() * kRdWarps;
+    w.workers = read_blocks(kv4, read_dc(kv4, d), w.nt) * tc_sm_count() * kRdWarps;
     const uint64_t parts = (uint64_t)w.workers + (uint64_t)w.heads * seqs;
     auto up = [](uint64_t x) { return (x + 31) / 32 * 32; };
     w.lse_at = up((seqs + 1ull) * 8);
@@ -681,8 +717,8 @@ static ReadPlan read_plan(uint32_t seqs, uint32_t kv_heads, uint32_t group, uint
 template <typename T, bool KV4, int DC, int NT>
 static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
 {
-    // the deepest ring with which kRdBlocks blocks fit an SM
-    constexpr uint32_t one = kRdWarps * ReadTile<KV4, DC>::kStage, room = (228 * 1024 / kRdBlocks - 1024 - 2048) / one;
+    // the deepest ring with which all blocks of an SM fit it
+    constexpr uint32_t one = kRdWarps * ReadTile<KV4, DC>::kStage, room = (228 * 1024 / read_blocks(KV4, DC, NT) - 1024 - 1280) / one;
     constexpr int stages = room > 6 ? 6 : room < 2 ? 2 : (int)room;
     auto *fn = &read_kernel<T, KV4, DC, NT, stages>;
     cudaError_t e = ensure_smem_attr((const void *)fn, stages * one);

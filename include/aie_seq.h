@@ -150,7 +150,7 @@ AIE_API int aie_prefix_attn(const aie_prefix *p, void *stream);
 
 /* A paged cache of keys and values in 4 bits.  Elements 32 g .. 32 g + 31 of a
  * head are a group with a scale s and a lowest value lo, both f16: its elements
- * are lo + code * s, codes 0 to 15.  The block of page p and head h is the
+ * are lo + code * s, codes 0 to 15, s finite and not negative.  The block of page p and head h is the
  * page_size * head_dim * 5 / 8 bytes at k + p * page_stride + h * (block bytes)
  * (v alike): first the codes, head_dim / 2 bytes a place, two to a byte, the even
  * element in the low half; then the groups' (s, lo) pairs, head_dim / 8 bytes a

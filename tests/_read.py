@@ -56,10 +56,12 @@ def read_cache(cache, head_dim):
 
 def kv4_attend(q, kp, vp, table, lens, scale=None):
     """One token of each stream over a 4-bit cache: the result and its bound.
-    Beyond _seq.attend's: queries in f16 with the largest at 2^8 or more (an
-    element loses at most 2^-33 of the largest), a group's products summed with
-    up to 256 times the queries' sizes beside them in f32, values rounded to f16
-    and f16 weights (2^-11 and its subnormals)."""
+    Beyond _seq.attend's: queries in f16 with the largest at 2^8 or more, odd ones
+    a 16th of that (an element loses at most 2^-29 of the largest); the scores as
+    a sum over codes and one over lowest values, in f32 and with the queries' sums
+    to 2^-22, so that each counts at its own size; weights in f16, then times
+    scales in f16 (2^-11 twice), over codes and lowest values that may cancel,
+    and their subnormals, which lose 2^-25 beside a largest weight of 2^4."""
     b, hq, d = q.shape
     hk, size = kp.shape[1], kp.shape[2]
     scale = d ** -0.5 if scale is None else scale
@@ -74,12 +76,13 @@ def kv4_attend(q, kp, vp, table, lens, scale=None):
             rows = slice(h * (hq // hk), (h + 1) * (hq // hk))
             seen = torch.full((hq // hk,), n, device=q.device)
             w, e = _seq.attend(q[i, rows], k, v, seen, scale, q.dtype)
-            # the offsets: 256 |q| over a group, 34 sums, times the group's scale; half a code's step at most
-            step = (kp.reshape(*kp.shape[:2], -1)[pages, h][:, size * d // 2:].contiguous().view(torch.float16)
-                               .double().reshape(-1, d // 32, 2)[:n, :, 0])
+            def parts(cache):  # 15 s and |lo| of each group of each place
+                pair = cache.reshape(*cache.shape[:2], -1)[pages, h][:, size * d // 2:].contiguous().view(torch.float16).double()
+                pair = pair.reshape(-1, d // 32, 2)[:n]
+                return 15 * pair[..., 0] + pair[..., 1].abs()
             qsum = q[i, rows].double().abs().unflatten(-1, (-1, 32)).sum(-1)
-            ds = abs(scale) * (34 * 2.0 ** -24 * 272 * (qsum @ step.T).amax(-1, keepdim=True)
-                               + 2.0 ** -33 * q[i, rows].double().abs().amax(-1, keepdim=True) * k.abs().sum(-1).max())
-            size_ = v.abs().amax(0)
-            want[i, rows], limit[i, rows] = w, e + (2 * ds + 2.0 ** -10) * size_ + 2.0 ** -23
+            ds = abs(scale) * (34 * 2.0 ** -24 * (qsum @ parts(kp).T).amax(-1, keepdim=True)
+                               + 2.0 ** -29 * q[i, rows].double().abs().amax(-1, keepdim=True) * k.abs().sum(-1).max())
+            size_ = parts(vp).amax(0).repeat_interleave(32)
+            want[i, rows], limit[i, rows] = w, e + (2 * ds + 2.0 ** -10) * size_ + n * 2.0 ** -28 * size_.max()
     return want, limit

@@ -114,6 +114,22 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
     return *(const uint32_t *)&y;
 }
 
+// c = a b
+template <typename T>
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+                     "{%10, %10, %10, %10};"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // N 32-bit words of shared memory from an address aligned to the whole of them.
 template <int N>
 __device__ __forceinline__ void shared_words(const uint32_t *p, uint32_t (&w)[N])
@@ -158,9 +174,12 @@ template <typename T, bool KV4, int DC, int NT, int STAGES>
 __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_kernel(const ReadArgs a)
 {
     using Tile = ReadTile<KV4, DC>;
-    // binary orders by which weights are held larger: in 4 bits they are also
-    // multiplied with scales below 8, and 2^8 2^4 8 is what f16 holds
-    constexpr float kShift = KV4 ? 4.f : kWeightShift<T>;
+    // Binary orders by which weights are held larger.  In 4 bits they are also
+    // multiplied with the groups' scales, below 2^(se + 3): 4 - se, so that 2^8 times
+    // both is what f16 holds, and se moves up only when a scale is too large.  (Values
+    // of a few units need no move; where they reach thousands, weights below 2^-5 of
+    // the largest begin to lose bits as subnormals.)
+    constexpr int kLeastScale = -3;
     constexpr int MT = Tile::kKeys / 16, OT = KV4 ? 2 * DC : DC;  // tiles of 16 keys; of 16 elements of V
     extern __shared__ __align__(16) char smem[];
     __shared__ long long scan[kRdThreads], warp_sum_[kRdWarps];
@@ -203,7 +222,9 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     // ---- where the warp's part begins
     struct Place {
         int s, head, tile, len;  // sequence; key head and block of query heads; tile of the sequence
+        long long head_at;       // 4 bits: the key head's blocks in a page; 16 bits: the key head
     } at;
+    auto head_at = [&](int head) { return (long long)(head / a.zs) * (KV4 ? a.g.block() : 1); };
     {
         at.head = (int)(begin / tiles);
         long long left = begin - at.head * tiles;
@@ -220,6 +241,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             left -= n;
         }
         at.tile = (int)left;
+        at.head_at = head_at(at.head);
     }
     auto advance = [&](Place &p) {
         if (++p.tile * Tile::kKeys < p.len) return;
@@ -227,7 +249,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         do {
             if (++p.s == a.seqs) {
                 p.s = 0;
-                p.head++;
+                p.head_at = head_at(++p.head);
             }
             p.len = read_len(a, p.s);
         } while (!p.len);
@@ -238,47 +260,48 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 
     // ---- copies
     Place ahead = at;
-    // 4 bits: where a lane's 8 places of the tile (of lane & 3) have their codes and their pairs; -1: no such page
-    long long codes_at = 0, pairs_at = 0;
+    // 4 bits: how many of a lane's 8 places of the tile (of lane & 3) exist, and where
+    // their codes and pairs are
+    long long codes_at = 0;
+    int pairs_in = 0, real = 0;  // pairs: from the codes on
     auto look_up = [&] {
         if constexpr (KV4) {
-            const int place = ahead.tile * Tile::kKeys + (lane & 3) * 8, i = fdiv(place, a.size);
+            const int place = ahead.tile * Tile::kKeys + (lane & 3) * 8, i = fdiv(place, a.size), in = place - i * a.g.size;
             const int page = place < ahead.len ? a.table[(long long)ahead.s * a.table_stride + i] : -1;
-            const long long block = page * a.g.page_stride + (ahead.head / a.zs) * a.g.block();
-            const int in = place - i * a.g.size;
-            const bool real = page >= 0 && page < a.g.pages;
-            codes_at = real ? block + in * (16 * DC) : -1;
-            pairs_at = real ? block + (long long)a.g.size * (16 * DC) + in * (4 * DC) : -1;
+            const bool exists = page >= 0 && page < a.g.pages;
+            real = exists ? min(ahead.len - place, 8) : 0;
+            codes_at = exists ? page * a.g.page_stride + ahead.head_at + in * (16 * DC) : 0;
+            pairs_in = exists ? (a.g.size - in) * (16 * DC) + in * (4 * DC) : 0;
         }
     };
     auto copy_tile = [&](int stage) {
         const uint32_t dst = ring_at + stage * Tile::kStage;
-        const int rows = ahead.len - ahead.tile * Tile::kKeys;  // that exist; the others are zeros
+        // keys that do not exist: zeros
         if constexpr (KV4) {
+            // 8 places' codes are 8 DC pieces of 16 bytes side by side, their pairs 2 DC
 #pragma unroll
             for (int i = 0; i < DC; i++) {
-                const int c = i * 32 + lane, row = c / DC, piece = c - row * DC, eight = c / (8 * DC);
-                const long long from = __shfl_sync(0xffffffffu, codes_at, eight);
-                const int n = from >= 0 && row < rows ? 16 : 0;
-                const long long off = n ? from + (c - eight * 8 * DC) * 16 : 0;
-                copy16(dst + row * Tile::kRow + piece * 16, a.g.k + off, n);
-                copy16(dst + Tile::kSide + row * Tile::kRow + piece * 16, a.g.v + off, n);
+                const int c = i * 32 + lane, row = c / DC, eight = c / (8 * DC);
+                const long long off = __shfl_sync(0xffffffffu, codes_at, eight) + (c - eight * 8 * DC) * 16;
+                const int n = (row & 7) < __shfl_sync(0xffffffffu, real, eight) ? 16 : 0;
+                const uint32_t to = dst + row * Tile::kRow + (c - row * DC) * 16;
+                copy16(to, a.g.k + off, n);
+                copy16(to + Tile::kSide, a.g.v + off, n);
             }
-            // pairs: 2 DC pieces to 8 places, one a lane
 #pragma unroll
             for (int i = 0; i < (DC + 3) / 4; i++) {
                 const int c = i * 32 + lane, eight = min(c / (2 * DC), 3), in = (c - eight * 2 * DC) * 16;
-                const long long from = __shfl_sync(0xffffffffu, pairs_at, eight);
+                const long long off = __shfl_sync(0xffffffffu, codes_at + pairs_in, eight) + in;
+                const int n = min(max(__shfl_sync(0xffffffffu, real, eight) * (4 * DC) - in, 0), 16);
                 if (c < 8 * DC) {
-                    const int n = from >= 0 ? min(max((rows - eight * 8) * 4 * DC - in, 0), 16) : 0;
-                    const long long off = n ? from + in : 0;
                     copy16(dst + 2 * Tile::kSide + c * 16, a.g.k + off, n);
                     copy16(dst + 2 * Tile::kSide + Tile::kPairs + c * 16, a.g.v + off, n);
                 }
             }
         } else {
+            const int rows = ahead.len - ahead.tile * Tile::kKeys;
             const long long key = min(max(a.cu[ahead.s], 0), a.keys) + (long long)ahead.tile * Tile::kKeys;
-            const int kvh = ahead.head / a.zs;
+            const int kvh = (int)ahead.head_at;
             const T *k = (const T *)a.k + key * a.k_ts + kvh * a.k_hs, *v = (const T *)a.v + key * a.v_ts + kvh * a.v_hs;
 #pragma unroll
             for (int i = 0; i < DC; i++) {
@@ -310,7 +333,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     float slq[NT][2];                                  // scale of a column's scores, in binary orders
     float o[OT][NT][4], m[NT][2], l[NT][2];
     float o_lo[KV4 ? NT : 1][4];  // 4 bits: the weighted sums of the groups' lo
-    int se = 0;                   // and 2^se .. 2^(se + 3), to which their scales go; o is in units of 2^(se - 24)
+    int se = kLeastScale;         // their scales are below 2^(se + 3)
     bool fresh = true;
     int first_tile = 0, stage = 0;  // of the sequence's tiles; of the ring
     for (int i = 0; i < count; i++) {
@@ -369,7 +392,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     for (int j = 0; j < 2; j++)
                         slq[nt][j] = fmaxf(sl * 0x1p24f * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f);
                     o_lo[nt][0] = o_lo[nt][1] = o_lo[nt][2] = o_lo[nt][3] = 0.f;
-                    se = -100;  // none yet
+                    se = kLeastScale;
                 } else {
                     const T *q = (const T *)a.q + qat;
 #pragma unroll
@@ -411,8 +434,6 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         float s[MT][NT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) s[mt][nt][0] = s[mt][nt][1] = s[mt][nt][2] = s[mt][nt][3] = 0.f;
             if constexpr (KV4) {
                 // S 2^-24 = sum over the groups of s (codes 2^-24) q, and of lo sum(q) 2^-24
                 const uint32_t *pk = (const uint32_t *)(st + 2 * Tile::kSide) + (mt * 16 + r) * DC;
@@ -428,7 +449,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
-                    mma16816<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
+                    mma16816_first<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[mt][nt][j] *= 0x1p-24f;
                 }
@@ -440,8 +461,8 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const float f0 = __half2float(__ushort_as_half((unsigned short)p0[g])), f1 = __half2float(__ushort_as_half((unsigned short)p1[g]));
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma16816<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
+                        float acc[4];
+                        mma16816_first<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
                         mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
 #pragma unroll
                         for (int j = 0; j < 2; j++) {
@@ -456,7 +477,10 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     uint32_t w[4];
                     ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (2 * k + (lane >> 4)) * 16, w);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (k) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                        else mma16816_first<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                    }
                 }
             }
         }
@@ -471,6 +495,27 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         if (mt * 16 + r + (j >> 1) * 8 >= here) s[mt][nt][j] = -INFINITY;
         }
         // ---- weights
+        if constexpr (KV4) {
+            uint32_t pv[DC], most = 0;
+            shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
+#pragma unroll
+            for (int g = 0; g < DC; g++) most = max(most, pv[g] & 0xffffu);
+            if (__any_sync(0xffffffffu, (int)(most >> 10) - 15 >= se + 3)) {
+                const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 10) - 15, 14);
+                const float f = __uint_as_float((uint32_t)(127 + se - e) << 23);
+                se = e;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (j < 2) l[nt][j] *= f;
+                        o_lo[nt][j] *= f;
+#pragma unroll
+                        for (int t = 0; t < OT; t++) o[t][nt][j] *= f;
+                    }
+            }
+        }
+        const float shift = KV4 ? (float)(4 - se) : kWeightShift<T>;
         float top[NT][2];
         bool grow = false;
 #pragma unroll
@@ -507,7 +552,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         for (int nt = 0; nt < NT; nt++) {
             float off[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], kShift);
+            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], shift);
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
                 float e[4];
@@ -520,32 +565,11 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             }
         }
         // ---- values
-        uint32_t scale2 = 0;  // 2^-se, twice
-        if constexpr (KV4) {
-            // O = sum over the keys of (p s) codes, and of p lo.  The scales in f16 beside
-            // weights: brought to below 8 by a power of two that only moves when one is too large
-            uint32_t pv[DC];
-            shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
-            uint32_t most = 0;
-#pragma unroll
-            for (int g = 0; g < DC; g++) most = max(most, pv[g] & 0xffffu);
-            if (__any_sync(0xffffffffu, (int)(most >> 10) - 15 >= se + 3)) {
-                const int e = min(max((int)(__reduce_max_sync(0xffffffffu, most) >> 10) - 15, -14), 14);
-                const float f = se == -100 ? 1.f : __uint_as_float((uint32_t)(127 + se - e) << 23);
-                se = e;
-#pragma unroll
-                for (int t = 0; t < OT; t++)
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int j = 0; j < 4; j++) o[t][nt][j] *= f;
-            }
-            scale2 = (uint32_t)(15 - se) * 0x04000400u;
-        }
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
             if constexpr (KV4) {
-                // (s, lo) of keys c2, c2 + 1 and of 8 further on, two keys to a register
+                // O = sum over the keys of (p s) codes, and of p lo.  (s, lo) of keys c2, c2 + 1
+                // and of 8 further on, two keys to a register
                 const uint32_t *pv = (const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + (mt * 16 + c2) * DC;
                 uint32_t p0[DC], p1[DC], p2[DC], p3[DC], low[4] = {0u, 0u, 0u, 0u};
                 shared_words<DC>(pv, p0);
@@ -563,7 +587,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     uint32_t w[2];
                     ldmatrix2_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
                     const Codes x0(w[0]), x1(w[1]);
-                    const uint32_t s0 = mul2(__byte_perm(p0[g], p1[g], 0x5410), scale2), s1 = mul2(__byte_perm(p2[g], p3[g], 0x5410), scale2);
+                    const uint32_t s0 = __byte_perm(p0[g], p1[g], 0x5410), s1 = __byte_perm(p2[g], p3[g], 0x5410);
                     // rows r: elements 4 r + 0 (+ 2), rows r + 8: 4 r + 1 (+ 3), these 16 times as large
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
@@ -610,14 +634,14 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
-                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - kShift);
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - shift);
 #pragma unroll
                     for (int t = 0; t < OT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int d = KV4 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 + e : t * 16 + e * 8 + r;
                             float x = o[t][nt][2 * e + j];
-                            if constexpr (KV4) x = fmaf(x, __uint_as_float((uint32_t)(127 + 24 + se - 4 * e) << 23), low[t >> 1]);
+                            if constexpr (KV4) x = fmaf(x, e ? 0x1p20f : 0x1p24f, low[t >> 1]);
                             x *= f;
                             if (!KV4 && d >= a.d) continue;
                             if (!whole) a.part_o[pat + d] = x;

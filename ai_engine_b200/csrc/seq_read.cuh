@@ -101,10 +101,24 @@ struct Codes {
     uint32_t p[4];
     __device__ __forceinline__ Codes(uint32_t w)
     {
+        const uint32_t high = __byte_perm(w, 0, 0x4341);  // codes 2 and 3, in each half's lower byte
         p[0] = w & 0x000F000Fu;
         p[1] = w & 0x00F000F0u;
-        p[2] = w >> 8 & 0x000F000Fu;
-        p[3] = w >> 8 & 0x00F000F0u;
+        p[2] = high & 0x000F000Fu;
+        p[3] = high & 0x00F000F0u;
+    }
+};
+
+// The same with the odd ones still on top of the even: p[1] is code 0 + 16 code 1.
+// For a sum over them from which that over the even ones can be taken away.
+struct StackedCodes {
+    uint32_t p[4];
+    __device__ __forceinline__ StackedCodes(uint32_t w)
+    {
+        p[1] = w & 0x00FF00FFu;
+        p[3] = __byte_perm(w, 0, 0x4341);
+        p[0] = w & 0x000F000Fu;
+        p[2] = p[3] & 0x000F000Fu;
     }
 };
 
@@ -260,18 +274,22 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 
     // ---- copies
     Place ahead = at;
-    // 4 bits: how many of a lane's 8 places of the tile (of lane & 3) exist, and where
-    // their codes and pairs are
-    long long codes_at = 0;
-    int pairs_in = 0, real = 0;  // pairs: from the codes on
+    // 4 bits: four lanes to 8 places of the tile (the lane's are those of lane & 3), eight
+    // lanes to a piece of every one of them: how many exist, and where their codes
+    // and pairs are
+    const int in8 = lane >> 2;
+    const uint8_t *codes_at = nullptr, *pairs_at = nullptr;
+    const long long v_from_k = a.g.v - a.g.k;
+    int real = 0;
     auto look_up = [&] {
         if constexpr (KV4) {
             const int place = ahead.tile * Tile::kKeys + (lane & 3) * 8, i = fdiv(place, a.size), in = place - i * a.g.size;
             const int page = place < ahead.len ? a.table[(long long)ahead.s * a.table_stride + i] : -1;
             const bool exists = page >= 0 && page < a.g.pages;
             real = exists ? min(ahead.len - place, 8) : 0;
-            codes_at = exists ? page * a.g.page_stride + ahead.head_at + in * (16 * DC) : 0;
-            pairs_in = exists ? (a.g.size - in) * (16 * DC) + in * (4 * DC) : 0;
+            const uint8_t *block = a.g.k + ahead.head_at + (exists ? page * a.g.page_stride : 0);
+            codes_at = block + in * (16 * DC) + in8 * 16;
+            pairs_at = block + a.g.size * (16 * DC) + in * (4 * DC) + in8 * 16;
         }
     };
     auto copy_tile = [&](int stage) {
@@ -279,23 +297,20 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         // keys that do not exist: zeros
         if constexpr (KV4) {
             // 8 places' codes are 8 DC pieces of 16 bytes side by side, their pairs 2 DC
+            const uint32_t codes_to = dst + (lane & 3) * 8 * Tile::kRow, pairs_to = dst + 2 * Tile::kSide + ((lane & 3) * 2 * DC + in8) * 16;
 #pragma unroll
             for (int i = 0; i < DC; i++) {
-                const int c = i * 32 + lane, row = c / DC, eight = c / (8 * DC);
-                const long long off = __shfl_sync(0xffffffffu, codes_at, eight) + (c - eight * 8 * DC) * 16;
-                const int n = (row & 7) < __shfl_sync(0xffffffffu, real, eight) ? 16 : 0;
-                const uint32_t to = dst + row * Tile::kRow + (c - row * DC) * 16;
-                copy16(to, a.g.k + off, n);
-                copy16(to + Tile::kSide, a.g.v + off, n);
+                const int c = i * 8 + in8, row = c / DC, n = row < real ? 16 : 0;
+                const uint32_t to = codes_to + row * Tile::kRow + (c - row * DC) * 16;
+                copy16(to, codes_at + i * 128, n);
+                copy16(to + Tile::kSide, codes_at + v_from_k + i * 128, n);
             }
 #pragma unroll
             for (int i = 0; i < (DC + 3) / 4; i++) {
-                const int c = i * 32 + lane, eight = min(c / (2 * DC), 3), in = (c - eight * 2 * DC) * 16;
-                const long long off = __shfl_sync(0xffffffffu, codes_at + pairs_in, eight) + in;
-                const int n = min(max(__shfl_sync(0xffffffffu, real, eight) * (4 * DC) - in, 0), 16);
-                if (c < 8 * DC) {
-                    copy16(dst + 2 * Tile::kSide + c * 16, a.g.k + off, n);
-                    copy16(dst + 2 * Tile::kSide + Tile::kPairs + c * 16, a.g.v + off, n);
+                const int n = min(max(real * (4 * DC) - (i * 8 + in8) * 16, 0), 16);
+                if (i * 8 + in8 < 2 * DC) {
+                    copy16(pairs_to + i * 128, pairs_at + i * 128, n);
+                    copy16(pairs_to + Tile::kPairs + i * 128, pairs_at + v_from_k + i * 128, n);
                 }
             }
         } else {
@@ -331,6 +346,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     const float sl = fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
     uint32_t qb[NT][KV4 ? 2 * DC : DC][2], qs[NT][2];  // queries; 4 bits: each group's sum of them, in two f16
     float slq[NT][2];                                  // scale of a column's scores, in binary orders
+    float off[NT][2], most_s[NT][2];                   // weights are 2^(slq s + off); scores above that move m
     float o[OT][NT][4], m[NT][2], l[NT][2];
     float o_lo[KV4 ? NT : 1][4];  // 4 bits: the weighted sums of the groups' lo
     int se = kLeastScale;         // their scales are below 2^(se + 3)
@@ -407,8 +423,8 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                 }
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    m[nt][j] = -INFINITY;
-                    l[nt][j] = 0.f;
+                    m[nt][j] = most_s[nt][j] = -INFINITY;
+                    l[nt][j] = off[nt][j] = 0.f;
                 }
 #pragma unroll
                 for (int x = 0; x < OT; x++) o[x][nt][0] = o[x][nt][1] = o[x][nt][2] = o[x][nt][3] = 0.f;
@@ -430,71 +446,6 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         const char *const st = ring + stage * Tile::kStage;
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         const uint32_t kt = smem_u32(st), vt = kt + Tile::kSide;
-        // ---- scores: keys r and r + 8 of each 16, query heads c2 and c2 + 1
-        float s[MT][NT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            if constexpr (KV4) {
-                // S 2^-24 = sum over the groups of s (codes 2^-24) q, and of lo sum(q) 2^-24
-                const uint32_t *pk = (const uint32_t *)(st + 2 * Tile::kSide) + (mt * 16 + r) * DC;
-                uint32_t p0[DC], p1[DC];
-                shared_words<DC>(pk, p0);
-                shared_words<DC>(pk + 8 * DC, p1);
-                uint32_t low[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // row r or r + 8, group lane & 3 or 4 further on
-                    const int g = (lane & 3) + (i >> 1) * 4;
-                    low[i] = g < DC ? __byte_perm(pk[(i & 1) * 8 * DC + g], 0, 0x3232) : 0u;
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    mma16816_first<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) s[mt][nt][j] *= 0x1p-24f;
-                }
-#pragma unroll
-                for (int g = 0; g < DC; g++) {
-                    uint32_t w[2];
-                    ldmatrix2(kt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
-                    const Codes x0(w[0]), x1(w[1]);
-                    const float f0 = __half2float(__ushort_as_half((unsigned short)p0[g])), f1 = __half2float(__ushort_as_half((unsigned short)p1[g]));
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float acc[4];
-                        mma16816_first<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
-                        mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
-#pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            s[mt][nt][j] = fmaf(f0, acc[j], s[mt][nt][j]);
-                            s[mt][nt][2 + j] = fmaf(f1, acc[2 + j], s[mt][nt][2 + j]);
-                        }
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < DC; k++) {
-                    uint32_t w[4];
-                    ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (2 * k + (lane >> 4)) * 16, w);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (k) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
-                        else mma16816_first<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
-                    }
-                }
-            }
-        }
-        const int here = at.len - at.tile * Tile::kKeys;
-        if (here < Tile::kKeys) {
-#pragma unroll
-            for (int mt = 0; mt < MT; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (mt * 16 + r + (j >> 1) * 8 >= here) s[mt][nt][j] = -INFINITY;
-        }
-        // ---- weights
         if constexpr (KV4) {
             uint32_t pv[DC], most = 0;
             shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
@@ -503,6 +454,11 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             if (__any_sync(0xffffffffu, (int)(most >> 10) - 15 >= se + 3)) {
                 const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 10) - 15, 14);
                 const float f = __uint_as_float((uint32_t)(127 + se - e) << 23);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    off[nt][0] += (float)(se - e);
+                    off[nt][1] += (float)(se - e);
+                }
                 se = e;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -515,95 +471,166 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     }
             }
         }
-        const float shift = KV4 ? (float)(4 - se) : kWeightShift<T>;
-        float top[NT][2];
-        bool grow = false;
+        {
+            const int here = at.len - at.tile * Tile::kKeys;
+            // ---- scores: keys r and r + 8 of each 16, query heads c2 and c2 + 1
+            float s[MT][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+            for (int mt = 0; mt < MT; mt++) {
+                if constexpr (KV4) {
+                    // S 2^-24 = sum over the groups of s (codes 2^-24) q, and of lo sum(q) 2^-24
+                    const uint32_t *pk = (const uint32_t *)(st + 2 * Tile::kSide) + (mt * 16 + r) * DC;
+                    uint32_t p0[DC], p1[DC];
+                    shared_words<DC>(pk, p0);
+                    shared_words<DC>(pk + 8 * DC, p1);
+                    uint32_t low[4];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                float x = m[nt][j];
+                    for (int i = 0; i < 4; i++) {
+                        // row r or r + 8, group lane & 3 or 4 further on
+                        const int g = (lane & 3) + (i >> 1) * 4;
+                        low[i] = g < DC ? __byte_perm(pk[(i & 1) * 8 * DC + g], 0, 0x3232) : 0u;
+                    }
 #pragma unroll
-                for (int mt = 0; mt < MT; mt++) x = max3(x, s[mt][nt][j], s[mt][nt][2 + j]);
-                top[nt][j] = x;
-                grow |= (x - m[nt][j]) * slq[nt][j] > 8.f;  // as in attn_tc_kernel: smaller steps leave m
+                    for (int nt = 0; nt < NT; nt++) {
+                        mma16816_first<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) s[mt][nt][j] *= 0x1p-24f;
+                    }
+                    uint32_t w[4];
+#pragma unroll
+                    for (int g = 0; g < DC; g++) {
+                        // of 16 keys, two groups at a time
+                        if (g + 1 < DC && !(g & 1)) ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (g + (lane >> 4)) * 16, w);
+                        else if (!(g & 1)) ldmatrix2(kt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, *(uint32_t(*)[2])w);
+                        const Codes x0(w[(g & 1) * 2]), x1(w[(g & 1) * 2 + 1]);
+                        const float f0 = __half2float(__ushort_as_half((unsigned short)p0[g])), f1 = __half2float(__ushort_as_half((unsigned short)p1[g]));
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            float acc[4];
+                            mma16816_first<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
+                            mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                s[mt][nt][j] = fmaf(f0, acc[j], s[mt][nt][j]);
+                                s[mt][nt][2 + j] = fmaf(f1, acc[2 + j], s[mt][nt][2 + j]);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < DC; k++) {
+                        uint32_t w[4];
+                        ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (2 * k + (lane >> 4)) * 16, w);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            if (k) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                            else mma16816_first<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                        }
+                    }
+                }
             }
-        if (__any_sync(0xffffffffu, grow)) {
+            if (here < Tile::kKeys) {
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int j = 0; j < 4; j++)
+                            if (mt * 16 + r + (j >> 1) * 8 >= here) s[mt][nt][j] = -INFINITY;
+            }
+            // ---- weights
+            float top[NT][2];
+            bool grow = false;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    float x = top[nt][j];
+                    float x = m[nt][j];
 #pragma unroll
-                    for (int e = 4; e < 32; e <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
-                    const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
-                    m[nt][j] = x;
-                    l[nt][j] *= f;
-                    if constexpr (KV4) o_lo[nt][j] *= f;
-#pragma unroll
-                    for (int t = 0; t < OT; t++) {
-                        o[t][nt][j] *= f;
-                        o[t][nt][2 + j] *= f;
-                    }
+                    for (int mt = 0; mt < MT; mt++) x = max3(x, s[mt][nt][j], s[mt][nt][2 + j]);
+                    top[nt][j] = x;
+                    grow |= x > most_s[nt][j];
                 }
-        }
-        uint32_t pb[MT][NT][2];
+            if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            float off[2];
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int j = 0; j < 2; j++) off[j] = m[nt][j] == -INFINITY ? 0.f : fmaf(-m[nt][j], slq[nt][j], shift);
+                    for (int j = 0; j < 2; j++) {
+                        float x = top[nt][j];
+#pragma unroll
+                        for (int e = 4; e < 32; e <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
+                        const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
+                        if (x != -INFINITY) {
+                            m[nt][j] = x;
+                            off[nt][j] = fmaf(-x, slq[nt][j], KV4 ? (float)(4 - se) : kWeightShift<T>);
+                            // as in attn_tc_kernel: steps of up to 8 binary orders leave m
+                            most_s[nt][j] = x + __fdividef(8.f, slq[nt][j]);
+                        }
+                        l[nt][j] *= f;
+                        if constexpr (KV4) o_lo[nt][j] *= f;
+#pragma unroll
+                        for (int t = 0; t < OT; t++) {
+                            o[t][nt][j] *= f;
+                            o[t][nt][2 + j] *= f;
+                        }
+                    }
+            }
+            uint32_t pb[NT][MT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int mt = 0; mt < MT; mt++) {
+                    float e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) e[j] = ex2(fmaf(s[mt][nt][j], slq[nt][j & 1], off[nt][j & 1]));
+                    l[nt][0] += e[0] + e[2];
+                    l[nt][1] += e[1] + e[3];
+                    pb[nt][mt][0] = transpose8x8(pack2<T>(e[0], e[1]));
+                    pb[nt][mt][1] = transpose8x8(pack2<T>(e[2], e[3]));
+                }
+            // ---- values
 #pragma unroll
             for (int mt = 0; mt < MT; mt++) {
-                float e[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) e[j] = ex2(fmaf(s[mt][nt][j], slq[nt][j & 1], off[j & 1]));
-                l[nt][0] += e[0] + e[2];
-                l[nt][1] += e[1] + e[3];
-                pb[mt][nt][0] = transpose8x8(pack2<T>(e[0], e[1]));
-                pb[mt][nt][1] = transpose8x8(pack2<T>(e[2], e[3]));
-            }
-        }
-        // ---- values
-#pragma unroll
-        for (int mt = 0; mt < MT; mt++) {
-            if constexpr (KV4) {
-                // O = sum over the keys of (p s) codes, and of p lo.  (s, lo) of keys c2, c2 + 1
-                // and of 8 further on, two keys to a register
-                const uint32_t *pv = (const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + (mt * 16 + c2) * DC;
-                uint32_t p0[DC], p1[DC], p2[DC], p3[DC], low[4] = {0u, 0u, 0u, 0u};
-                shared_words<DC>(pv, p0);
-                shared_words<DC>(pv + DC, p1);
-                shared_words<DC>(pv + 8 * DC, p2);
-                shared_words<DC>(pv + 9 * DC, p3);
-                if (r < DC) {  // row r: group r
-                    low[0] = __byte_perm(pv[r], pv[DC + r], 0x7632);
-                    low[2] = __byte_perm(pv[8 * DC + r], pv[9 * DC + r], 0x7632);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) mma16816<T>(o_lo[nt], low, pb[mt][nt][0], pb[mt][nt][1]);
-#pragma unroll
-                for (int g = 0; g < DC; g++) {
-                    uint32_t w[2];
-                    ldmatrix2_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, w);
-                    const Codes x0(w[0]), x1(w[1]);
-                    const uint32_t s0 = __byte_perm(p0[g], p1[g], 0x5410), s1 = __byte_perm(p2[g], p3[g], 0x5410);
-                    // rows r: elements 4 r + 0 (+ 2), rows r + 8: 4 r + 1 (+ 3), these 16 times as large
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        const uint32_t b0 = mul2(pb[mt][nt][0], s0), b1 = mul2(pb[mt][nt][1], s1);
-                        mma16816<T>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
-                        mma16816<T>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
+                if constexpr (KV4) {
+                    // O = sum over the keys of (p s) codes, and of p lo.  (s, lo) of keys c2, c2 + 1
+                    // and of 8 further on, two keys to a register
+                    const uint32_t *pv = (const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + (mt * 16 + c2) * DC;
+                    uint32_t p0[DC], p1[DC], p2[DC], p3[DC], low[4] = {0u, 0u, 0u, 0u};
+                    shared_words<DC>(pv, p0);
+                    shared_words<DC>(pv + DC, p1);
+                    shared_words<DC>(pv + 8 * DC, p2);
+                    shared_words<DC>(pv + 9 * DC, p3);
+                    if (r < DC) {  // row r: group r
+                        low[0] = __byte_perm(pv[r], pv[DC + r], 0x7632);
+                        low[2] = __byte_perm(pv[8 * DC + r], pv[9 * DC + r], 0x7632);
                     }
-                }
-            } else {
 #pragma unroll
-                for (int t = 0; t < DC; t++) {
-                    // as stored: keys 0-7 and 8-15 by elements 0-7, then 8-15
+                    for (int nt = 0; nt < NT; nt++) mma16816<T>(o_lo[nt], low, pb[nt][mt][0], pb[nt][mt][1]);
                     uint32_t w[4];
-                    ldmatrix4_t(vt + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * Tile::kRow + (2 * t + (lane >> 3 & 1)) * 16, w);
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816<T>(o[t][nt], w, pb[mt][nt][0], pb[mt][nt][1]);
+                    for (int g = 0; g < DC; g++) {
+                        // of 16 keys, two groups at a time
+                        if (g + 1 < DC && !(g & 1)) ldmatrix4_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + (g + (lane >> 4)) * 16, w);
+                        else if (!(g & 1)) ldmatrix2_t(vt + (mt * 16 + (lane & 15)) * Tile::kRow + g * 16, *(uint32_t(*)[2])w);
+                        const StackedCodes x0(w[(g & 1) * 2]), x1(w[(g & 1) * 2 + 1]);
+                        const uint32_t s0 = __byte_perm(p0[g], p1[g], 0x5410), s1 = __byte_perm(p2[g], p3[g], 0x5410);
+                        // rows r: elements 4 r + 0 (+ 2), rows r + 8: these and 16 times 4 r + 1 (+ 3)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            const uint32_t b0 = mul2(pb[nt][mt][0], s0), b1 = mul2(pb[nt][mt][1], s1);
+                            mma16816<T>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
+                            mma16816<T>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < DC; t++) {
+                        // as stored: keys 0-7 and 8-15 by elements 0-7, then 8-15
+                        uint32_t w[4];
+                        ldmatrix4_t(vt + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * Tile::kRow + (2 * t + (lane >> 3 & 1)) * 16, w);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) mma16816<T>(o[t][nt], w, pb[nt][mt][0], pb[nt][mt][1]);
+                    }
                 }
             }
         }
@@ -634,14 +661,14 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
-                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(m[nt][j], slq[nt][j], log2f(sum) - shift);
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : log2f(sum) - off[nt][j];
 #pragma unroll
                     for (int t = 0; t < OT; t++)
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
                             const int d = KV4 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 + e : t * 16 + e * 8 + r;
                             float x = o[t][nt][2 * e + j];
-                            if constexpr (KV4) x = fmaf(x, e ? 0x1p20f : 0x1p24f, low[t >> 1]);
+                            if constexpr (KV4) x = fmaf(e ? x - o[t][nt][j] : x, e ? 0x1p20f : 0x1p24f, low[t >> 1]);
                             x *= f;
                             if (!KV4 && d >= a.d) continue;
                             if (!whole) a.part_o[pat + d] = x;

@@ -486,7 +486,7 @@ static CrossPlan cross_plan(const aie_cross &p)
 extern "C" uint64_t aie_cross_attn_workspace(const aie_cross *p)
 {
     if (check_cross(p)) return 0;
-    if (cross_read_ok(*p)) return read_plan(false, p->seqs, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
+    if (cross_read_ok(*p)) return read_plan(false, p->seqs, p->keys, p->kv_heads, p->q_heads / p->kv_heads, p->head_dim).bytes;
     return cross_tc_ok(*p) ? cross_plan(*p).bytes : 64;
 }
 
@@ -531,7 +531,8 @@ static int cross_tc(const aie_cross &p, cudaStream_t s)
 static int cross_read(const aie_cross &p, cudaStream_t s)
 {
     ReadArgs a = {};
-    const ReadPlan w = read_plan(false, p.seqs, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
+    const ReadPlan w = read_plan(false, p.seqs, p.keys, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
+    if (w.tiles > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^35 (state, key head) pairs in one call");
     read_args(a, w, p.q, p.out, p.workspace);
     a.k = p.k.data; a.k_ts = p.k.token_stride; a.k_hs = p.k.head_stride;
     a.v = p.v.data; a.v_ts = p.v.token_stride; a.v_hs = p.v.head_stride;
@@ -628,7 +629,7 @@ static int check_kv4_step(const aie_kv4_step *p)
 
 static ReadPlan kv4_plan(const aie_kv4_step &p)
 {
-    return read_plan(true, p.batch, p.cache.kv_heads, p.q_heads / p.cache.kv_heads, p.cache.head_dim);
+    return read_plan(true, p.batch, (uint64_t)p.batch * p.max_len, p.cache.kv_heads, p.q_heads / p.cache.kv_heads, p.cache.head_dim);
 }
 
 extern "C" uint64_t aie_kv4_attn_workspace(const aie_kv4_step *p) { return check_kv4_step(p) ? 0 : kv4_plan(*p).bytes; }
@@ -637,8 +638,7 @@ static int kv4_step(const aie_kv4_step &p, cudaStream_t s)
 {
     ReadArgs a = {};
     const ReadPlan w = kv4_plan(p);
-    if ((uint64_t)p.batch * w.heads * (p.max_len / 32 + 1ull) / w.workers > 0x7ffffff0ull)
-        return fail(AIE_E_UNSUPPORTED, "too many places in one call");
+    if (w.tiles > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^36 (place, key head) pairs in one call");
     read_args(a, w, p.q, p.out, p.workspace);
     a.g = kv4_geom(p.cache); a.size = make_fastdiv(a.g.size);
     a.table = p.table; a.lens = p.lens; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;

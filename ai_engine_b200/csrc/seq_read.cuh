@@ -52,9 +52,10 @@ struct ReadArgs {
     int zs, heads;           // blocks of a group's query heads; key heads times those
     int rows;                // query heads of a block that are kept
     int bf16;
+    int q_vec, o_vec;        // bytes that q and out are aligned to, in every row
     float scale;
     // workspace
-    long long *before;       // [seqs + 1]: tiles of the sequences before
+    unsigned *before;        // [seqs + 1]: tiles of the sequences before
     float *part_lse, *part_o;
     int workers;
 };
@@ -67,7 +68,7 @@ __device__ __forceinline__ int read_len(const ReadArgs &a, int s)
 }
 
 // Tiles a warp takes of `total`.
-__device__ __forceinline__ long long read_share(long long total, int workers) { return max((total + workers - 1) / workers, 1ll); }
+__device__ __forceinline__ unsigned read_share(unsigned total, unsigned workers) { return max((total + workers - 1) / workers, 1u); }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, int bytes)
 {
@@ -128,6 +129,12 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
     return *(const uint32_t *)&y;
 }
 
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b)
+{
+    const __half2 y = __hmax2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&y;
+}
+
 // c = a b
 template <typename T>
 __device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -180,6 +187,20 @@ struct ReadTile {
     static constexpr uint32_t kStage = 2 * kSide + 2 * kPairs;
 };
 
+// Four neighbouring elements of a result.
+__device__ __forceinline__ void read_store4(const ReadArgs &a, long long at, const float (&x)[4])
+{
+    unsigned short *out = (unsigned short *)a.out + at;
+    uint2 y;
+    if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(x[0], x[1]), pack2<__nv_bfloat16>(x[2], x[3]));
+    else y = make_uint2(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]));
+    if (a.o_vec >= 8) *(uint2 *)out = y;
+    else {
+        out[0] = (unsigned short)y.x; out[1] = (unsigned short)(y.x >> 16);
+        out[2] = (unsigned short)y.y; out[3] = (unsigned short)(y.y >> 16);
+    }
+}
+
 // Blocks of an SM.
 constexpr int read_blocks(bool kv4, int dc, int nt) { return nt == 1 && dc <= 4 ? 3 : 2; }
 
@@ -196,27 +217,27 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     constexpr int kLeastScale = -3;
     constexpr int MT = Tile::kKeys / 16, OT = KV4 ? 2 * DC : DC;  // tiles of 16 keys; of 16 elements of V
     extern __shared__ __align__(16) char smem[];
-    __shared__ long long scan[kRdThreads], warp_sum_[kRdWarps];
+    __shared__ unsigned scan[kRdThreads], warp_sums[kRdWarps];
     behind_last_launch();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     // ---- tiles before each thread's sequences, and in all
     const int per = (a.seqs + kRdThreads - 1) / kRdThreads, s_from = tid * per, s_to = min(s_from + per, a.seqs);
-    long long mine = 0;
+    unsigned mine = 0;
     for (int s = s_from; s < s_to; s++) mine += (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys;
-    long long upto = mine;
+    unsigned upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += y;
     }
-    if (lane == 31) warp_sum_[warp] = upto;
+    if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
-    long long tiles = 0, base = upto - mine;
+    unsigned tiles = 0, base = upto - mine;
 #pragma unroll
     for (int i = 0; i < kRdWarps; i++) {
-        if (i < warp) base += warp_sum_[i];
-        tiles += warp_sum_[i];
+        if (i < warp) base += warp_sums[i];
+        tiles += warp_sums[i];
     }
     scan[tid] = base;
     if (blockIdx.x == 0) {  // for the joining launch
@@ -227,10 +248,11 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         if (tid == 0) a.before[a.seqs] = tiles;
     }
     __syncthreads();
-    const long long total = tiles * a.heads, share = read_share(total, a.workers);
+    const unsigned total = tiles * a.heads, share = read_share(total, a.workers);
     const int worker = blockIdx.x * kRdWarps + warp;
-    const long long begin = worker * share;
-    if (begin >= total) return;
+    const unsigned long long first_of = (unsigned long long)worker * share;
+    if (first_of >= total) return;
+    const unsigned begin = (unsigned)first_of;
     const int count = (int)min(share, total - begin);
 
     // ---- where the warp's part begins
@@ -241,7 +263,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     auto head_at = [&](int head) { return (long long)(head / a.zs) * (KV4 ? a.g.block() : 1); };
     {
         at.head = (int)(begin / tiles);
-        long long left = begin - at.head * tiles;
+        unsigned left = begin - at.head * tiles;
         // the last thread whose sequences begin at or before it
         int t = 0;
 #pragma unroll
@@ -250,7 +272,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         left -= scan[t];
         for (at.s = t * per;; at.s++) {
             at.len = read_len(a, at.s);
-            const int n = (at.len + Tile::kKeys - 1) / Tile::kKeys;
+            const unsigned n = (at.len + Tile::kKeys - 1) / Tile::kKeys;
             if (left < n) break;
             left -= n;
         }
@@ -269,8 +291,40 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         } while (!p.len);
     };
 
+    const int r = lane >> 2, c2 = (lane & 3) * 2;  // a lane's rows r, r + 8 and columns c2, c2 + 1 of a product
     char *const ring = smem + warp * (STAGES * Tile::kStage);
     const uint32_t ring_at = smem_u32(ring);
+
+    // ---- the queries of a sequence, as they come: of head r the elements 32 g + 8 (lane & 3)
+    // .. + 7 of each group, or 16 k + c2, + 1 and + 8, + 9 of each step
+    uint32_t raw[NT][KV4 ? 4 * DC : 2 * DC];
+    auto load_q = [&] {
+        const int row0 = at.head % a.zs * (8 * NT), heads = min(a.group - row0, 8 * NT);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const bool real = nt * 8 + r < heads;
+            const unsigned short *q = (const unsigned short *)a.q + (long long)at.s * a.q_ts +
+                                      (long long)(at.head / a.zs * a.group + row0 + (real ? nt * 8 + r : 0)) * a.q_hs;
+            auto two = [&](int d) { return a.q_vec >= 4 ? *(const uint32_t *)(q + d) : (uint32_t)q[d] | (uint32_t)q[d + 1] << 16; };
+            if constexpr (KV4) {
+#pragma unroll
+                for (int g = 0; g < DC; g++) {
+                    const int d = g * 32 + (lane & 3) * 8;
+                    uint4 x;
+                    if (a.q_vec >= 16) x = *(const uint4 *)(q + d);
+                    else x = make_uint4(two(d), two(d + 2), two(d + 4), two(d + 6));
+                    raw[nt][g * 4] = real ? x.x : 0u;
+                    raw[nt][g * 4 + 1] = real ? x.y : 0u;
+                    raw[nt][g * 4 + 2] = real ? x.z : 0u;
+                    raw[nt][g * 4 + 3] = real ? x.w : 0u;
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 2 * DC; k++) raw[nt][k] = real && k * 8 + c2 < a.d ? two(k * 8 + c2) : 0u;  // head_dim is even
+            }
+        }
+    };
+    load_q();
 
     // ---- copies
     Place ahead = at;
@@ -342,7 +396,6 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     }
 
     // ---- products
-    const int r = lane >> 2, c2 = (lane & 3) * 2;  // a lane's rows r, r + 8 and columns c2, c2 + 1 of a product
     const float sl = fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
     uint32_t qb[NT][KV4 ? 2 * DC : DC][2], qs[NT][2];  // queries; 4 bits: each group's sum of them, in two f16
     float slq[NT][2];                                  // scale of a column's scores, in binary orders
@@ -356,23 +409,21 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         if (fresh) {
             fresh = false;
             first_tile = at.tile;
-            const int kvh = at.head / a.zs, row0 = at.head % a.zs * (8 * NT), heads = min(a.group - row0, 8 * NT);
+            if (i) load_q();
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-                const int n = nt * 8 + r;
-                const long long qat = (long long)at.s * a.q_ts + (long long)(kvh * a.group + row0 + n) * a.q_hs;
                 if constexpr (KV4) {
                     float f[DC][8], top = 0.f;
 #pragma unroll
                     for (int g = 0; g < DC; g++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const long long x = qat + g * 32 + (lane & 3) * 8 + e;
-                            f[g][e] = n >= heads ? 0.f
-                                      : a.bf16   ? __bfloat162float(((const __nv_bfloat16 *)a.q)[x])
-                                                 : __half2float(((const __half *)a.q)[x]);
-                            f[g][e] *= sign;
-                            top = fmaxf(top, fabsf(f[g][e]));
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t x = raw[nt][g * 4 + e];
+                            const float2 y = a.bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u))
+                                                    : __half22float2(*(const __half2 *)&x);
+                            f[g][2 * e] = y.x * sign;
+                            f[g][2 * e + 1] = y.y * sign;
+                            top = fmaxf(top, fmaxf(fabsf(f[g][2 * e]), fabsf(f[g][2 * e + 1])));
                         }
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -410,15 +461,11 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     o_lo[nt][0] = o_lo[nt][1] = o_lo[nt][2] = o_lo[nt][3] = 0.f;
                     se = kLeastScale;
                 } else {
-                    const T *q = (const T *)a.q + qat;
 #pragma unroll
-                    for (int k = 0; k < DC; k++)
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int d = k * 16 + e * 8 + c2;
-                            const bool real = n < heads && d < a.d;  // d is even
-                            qb[nt][k][e] = real ? pack2<T>(sign * to_f32(q[d]), sign * to_f32(q[d + 1])) : 0u;
-                        }
+                    for (int k = 0; k < 2 * DC; k++) {
+                        const T *x = (const T *)&raw[nt][k];
+                        qb[nt][k >> 1][k & 1] = pack2<T>(sign * to_f32(x[0]), sign * to_f32(x[1]));
+                    }
                     slq[nt][0] = slq[nt][1] = fmaxf(sl, 1e-37f);
                 }
 #pragma unroll
@@ -450,9 +497,10 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             uint32_t pv[DC], most = 0;
             shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
 #pragma unroll
-            for (int g = 0; g < DC; g++) most = max(most, pv[g] & 0xffffu);
-            if (__any_sync(0xffffffffu, (int)(most >> 10) - 15 >= se + 3)) {
-                const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 10) - 15, 14);
+            for (int g = 0; g < DC; g++) most = max2(most, pv[g]);  // of the lower halves
+            most <<= 16;
+            if (__any_sync(0xffffffffu, most >= (uint32_t)(se + 3 + 15) << 26)) {
+                const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 26) - 15, 14);
                 const float f = __uint_as_float((uint32_t)(127 + se - e) << 23);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
@@ -662,19 +710,33 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
                         a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : log2f(sum) - off[nt][j];
+                    if constexpr (KV4) {
+                        // four neighbouring elements of each group
 #pragma unroll
-                    for (int t = 0; t < OT; t++)
+                        for (int g = 0; g < DC; g++) {
+                            float x[4];
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            const int d = KV4 ? (t >> 1) * 32 + r * 4 + (t & 1) * 2 + e : t * 16 + e * 8 + r;
-                            float x = o[t][nt][2 * e + j];
-                            if constexpr (KV4) x = fmaf(e ? x - o[t][nt][j] : x, e ? 0x1p20f : 0x1p24f, low[t >> 1]);
-                            x *= f;
-                            if (!KV4 && d >= a.d) continue;
-                            if (!whole) a.part_o[pat + d] = x;
-                            else if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
-                            else ((__half *)a.out)[oat + d] = __float2half_rn(x);
+                            for (int e = 0; e < 4; e++) {
+                                const float *t = o[2 * g + (e >> 1)][nt];
+                                x[e] = f * fmaf(e & 1 ? t[2 + j] - t[j] : t[j], e & 1 ? 0x1p20f : 0x1p24f, low[g]);
+                            }
+                            const int d = g * 32 + r * 4;
+                            if (!whole) *(float4 *)(a.part_o + pat + d) = make_float4(x[0], x[1], x[2], x[3]);
+                            else read_store4(a, oat + d, x);
                         }
+                    } else {
+#pragma unroll
+                        for (int t = 0; t < OT; t++)
+#pragma unroll
+                            for (int e = 0; e < 2; e++) {
+                                const int d = t * 16 + e * 8 + r;
+                                if (d >= a.d) continue;
+                                const float x = o[t][nt][2 * e + j] * f;
+                                if (!whole) a.part_o[pat + d] = x;
+                                else if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
+                                else ((__half *)a.out)[oat + d] = __float2half_rn(x);
+                            }
+                    }
                 }
             fresh = true;
         }
@@ -687,7 +749,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 struct JoinArgs {
     void *out;
     long long o_ts, o_hs;
-    const long long *before;
+    const unsigned *before;
     const float *part_lse, *part_o;
     int seqs, hq, group, d, zs, heads, rows, bf16, workers;
 };
@@ -695,39 +757,57 @@ struct JoinArgs {
 __global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
 {
     __shared__ float sums[kRdWarps][256], weights[kRdWarps];
-    behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int s = blockIdx.x / a.hq, h = blockIdx.x % a.hq, kvh = h / a.group, in = h % a.group;
     const int head = kvh * a.zs + in / a.rows, row = in % a.rows;
-    const long long tiles = a.before[a.seqs], from = a.before[s], n = a.before[s + 1] - from;
-    const long long share = read_share(tiles * a.heads, a.workers), at = head * tiles + from;
-    const long long first = at / share, last = n ? (at + n - 1) / share : first - 1;
     const long long oat = (long long)s * a.o_ts + (long long)h * a.o_hs;
+    behind_last_launch();
+    const unsigned tiles = a.before[a.seqs], from = a.before[s], n = a.before[s + 1] - from;
     auto store = [&](int d, float x) {
         if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
         else ((__half *)a.out)[oat + d] = __float2half_rn(x);
     };
-    if (first == last) return;
     if (n == 0) {
         for (int d = threadIdx.x; d < a.d; d += kRdThreads) store(d, 0.f);
         return;
     }
-    const int parts = (int)(last - first + 1);
-    const long long id = first + (long long)head * a.seqs + s;
-    const float *lse = a.part_lse + id * a.rows + row, *po = a.part_o + (id * a.rows + row) * a.d;
+    const unsigned share = read_share(tiles * a.heads, a.workers), at = head * tiles + from, first = at / share;
+    const int parts = (int)((at + n - 1) / share - first + 1);
+    if (parts == 1) return;
+    const long long id = (long long)first + (long long)head * a.seqs + s, next = (long long)a.rows * a.d;
+    const float *lse = a.part_lse + id * a.rows + row, *po = a.part_o + (id * a.rows + row) * a.d + lane * 4;
+    // a warp every fourth part, a lane four neighbouring elements (of 128 at a time);
+    // the first on their way before the weights are known
+    constexpr int kFirst = 2;
+    float4 y[kFirst][2];
+#pragma unroll
+    for (int i = 0; i < kFirst; i++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (warp + i * kRdWarps < parts && k * 128 + lane * 4 < a.d)
+                y[i][k] = *(const float4 *)(po + (warp + i * kRdWarps) * next + k * 128);
     float top = -INFINITY;
     for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[(long long)i * a.rows]);
     top = warp_max(top);
-    // a warp every fourth part, a lane four neighbouring elements (of 128 at a time)
     float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     float sum = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < parts; i += kRdWarps) {
+    auto add = [&](int i, const float4 (&z)[2]) {
         const float w = lse[(long long)i * a.rows], f = w == -INFINITY ? 0.f : ex2(w - top);
         sum += f;
 #pragma unroll
         for (int k = 0; k < 2; k++)
-            if (k * 128 + lane * 4 < a.d) add_scaled(x[k], f, *(const float4 *)(po + (long long)i * a.rows * a.d + k * 128 + lane * 4));
+            if (k * 128 + lane * 4 < a.d) add_scaled(x[k], f, z[k]);
+    };
+#pragma unroll
+    for (int i = 0; i < kFirst; i++)
+        if (warp + i * kRdWarps < parts) add(warp + i * kRdWarps, y[i]);
+#pragma unroll 4
+    for (int i = warp + kFirst * kRdWarps; i < parts; i += kRdWarps) {
+        float4 z[2];
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+            if (k * 128 + lane * 4 < a.d) z[k] = *(const float4 *)(po + i * next + k * 128);
+        add(i, z);
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) *(float4 *)&sums[warp][k * 128 + lane * 4] = x[k];
@@ -743,13 +823,14 @@ __global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
 // the workspace.
 struct ReadPlan {
     int nt, zs, heads, rows, workers;
-    uint64_t lse_at, o_at, bytes;
+    uint64_t tiles, lse_at, o_at, bytes;  // tiles: at most
 };
 
 // DC as the kernels are instantiated for it
 static int read_dc(bool kv4, uint32_t d) { return kv4 ? (int)d / 32 : d <= 64 ? 4 : d <= 128 ? 8 : 16; }
 
-static ReadPlan read_plan(bool kv4, uint32_t seqs, uint32_t kv_heads, uint32_t group, uint32_t d)
+// most: as many keys as all sequences have together, or more.
+static ReadPlan read_plan(bool kv4, uint32_t seqs, uint64_t most, uint32_t kv_heads, uint32_t group, uint32_t d)
 {
     ReadPlan w;
     w.nt = group > 8 && d <= 128 ? 2 : 1;  // with heads of 256 the results of 16 would not fit the registers
@@ -757,9 +838,10 @@ static ReadPlan read_plan(bool kv4, uint32_t seqs, uint32_t kv_heads, uint32_t g
     w.heads = (int)kv_heads * w.zs;
     w.rows = (int)std::min<uint32_t>(group, 8 * w.nt);
     w.workers = read_blocks(kv4, read_dc(kv4, d), w.nt) * tc_sm_count() * kRdWarps;
+    w.tiles = (most / (kv4 ? 32 : 16) + seqs) * w.heads;
     const uint64_t parts = (uint64_t)w.workers + (uint64_t)w.heads * seqs;
     auto up = [](uint64_t x) { return (x + 31) / 32 * 32; };
-    w.lse_at = up((seqs + 1ull) * 8);
+    w.lse_at = up((seqs + 1ull) * 4);
     w.o_at = up(w.lse_at + parts * w.rows * 4);
     w.bytes = w.o_at + parts * w.rows * d * 4 + 32;
     return w;
@@ -787,7 +869,12 @@ static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const 
     a.out = out.data; a.o_ts = out.token_stride; a.o_hs = out.head_stride;
     a.zs = w.zs; a.heads = w.heads; a.rows = w.rows; a.workers = w.workers;
     char *ws = (char *)(((uintptr_t)workspace + 31) / 32 * 32);
-    a.before = (long long *)ws;
+    a.before = (unsigned *)ws;
+    auto vec = [](const aie_heads &h) {
+        const uint64_t bits = (uintptr_t)h.data | 2 * h.token_stride | 2 * h.head_stride;
+        return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
+    };
+    a.q_vec = vec(q); a.o_vec = vec(out);
     a.part_lse = (float *)(ws + w.lse_at);
     a.part_o = (float *)(ws + w.o_at);
 }

@@ -162,13 +162,6 @@ __device__ __forceinline__ float ex2(float x)
     return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c)
-{
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
 // ------------------------------------------------------------- kernel ---
 
 struct AttnArgs {

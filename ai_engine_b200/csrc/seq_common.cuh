@@ -91,6 +91,13 @@ static cudaError_t launch_behind(void (*fn)(P...), dim3 grid, unsigned threads, 
     return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll

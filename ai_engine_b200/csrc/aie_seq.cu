@@ -468,18 +468,23 @@ static bool cross_tc_ok(const aie_cross &p)
 // No more pairs of tiles than whole ones, and one that is not whole per
 // sequence.  Where they fill the SMs less than twice, their steps are cut.
 struct CrossPlan {
+    bool few;
     int capacity;
-    uint64_t pairs, grid, bytes;
+    uint64_t pairs, grid, rows, bytes;  // rows of a partial result
 };
 
 static CrossPlan cross_plan(const aie_cross &p)
 {
     CrossPlan w = {};
-    const int tpt = kAtTile / (int)(p.q_heads / p.kv_heads), sms = tc_sm_count();
-    w.pairs = p.tokens / (2 * tpt) + std::min(p.seqs, p.tokens);
-    if (w.pairs * p.kv_heads < 2ull * sms) w.capacity = std::max(1, sms / (int)p.kv_heads);
+    const uint32_t tpt = kAtTile / (p.q_heads / p.kv_heads), sms = (uint32_t)tc_sm_count();
+    auto pairs = [&](uint32_t tokens) { return p.tokens / tokens + (uint64_t)std::min(p.seqs, p.tokens); };
+    // no more tokens a sequence than a tile holds: pairs of the same rows
+    w.few = p.tokens <= (uint64_t)tpt * p.seqs && pairs(tpt) * p.kv_heads < 2 * sms;
+    w.pairs = pairs(w.few ? tpt : 2 * tpt);
+    if (w.pairs * p.kv_heads < 2 * sms) w.capacity = (int)std::max(1u, sms / p.kv_heads);
     w.grid = (w.pairs + w.capacity) * p.kv_heads;
-    w.bytes = 64 + (w.capacity ? w.grid * 2 * kAtTile * (p.head_dim + 1) * 4 : 0);
+    w.rows = (w.few ? 1 : 2) * kAtTile;
+    w.bytes = 64 + (w.capacity ? w.grid * w.rows * (p.head_dim + 1) * 4 : 0);
     return w;
 }
 
@@ -494,10 +499,14 @@ template <typename T>
 static cudaError_t attn_cross_launch(const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, const AttnArgs &a,
                                      const CrossPlan &w, cudaStream_t s)
 {
-    cudaError_t e = a.d <= 64 ? attn_launch<T, 1, kAtCross>(q, k, v, a, (unsigned)w.grid, s)
-                              : attn_launch<T, 2, kAtCross>(q, k, v, a, (unsigned)w.grid, s);
-    if (e != cudaSuccess || !a.capacity) return e;
-    return launch_behind(cross_join_kernel<T>, (unsigned)(w.pairs * a.kv_heads * (2 * kAtTile / kJoinRows)), 32 * kJoinRows, 0, s, a);
+    const unsigned grid = (unsigned)w.grid, rows = (unsigned)(w.pairs * a.kv_heads * w.rows / kJoinRows);
+    cudaError_t e;
+    if (w.few) {
+        e = a.d <= 64 ? attn_launch<T, 1, kAtFew>(q, k, v, a, grid, s) : attn_launch<T, 2, kAtFew>(q, k, v, a, grid, s);
+        return e != cudaSuccess ? e : launch_behind(cross_join_kernel<T, true>, rows, 32 * kJoinRows, 0, s, a);
+    }
+    e = a.d <= 64 ? attn_launch<T, 1, kAtCross>(q, k, v, a, grid, s) : attn_launch<T, 2, kAtCross>(q, k, v, a, grid, s);
+    return e != cudaSuccess || !a.capacity ? e : launch_behind(cross_join_kernel<T, false>, rows, 32 * kJoinRows, 0, s, a);
 }
 
 static int cross_tc(const aie_cross &p, cudaStream_t s)
@@ -510,19 +519,20 @@ static int cross_tc(const aie_cross &p, cudaStream_t s)
     a.out_ts = p.out.token_stride; a.out_hs = p.out.head_stride;
     char *ws = (char *)(((uintptr_t)p.workspace + 31) / 32 * 32);
     a.part_o = (float *)ws;
-    a.part_lse = (float *)(ws + (w.capacity ? w.grid * 2 * kAtTile * p.head_dim * 4 : 0));
+    a.part_lse = (float *)(ws + (w.capacity ? w.grid * w.rows * p.head_dim * 4 : 0));
     a.tokens = (int)p.tokens; a.seqs = (int)p.seqs; a.keys = (int)p.keys; a.capacity = w.capacity;
     a.splits = (int)(w.grid / p.kv_heads);
     a.kv_heads = (int)p.kv_heads; a.q_heads = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads);
     a.d = (int)p.head_dim; a.tokens_per_tile = kAtTile / a.group;
+    a.pair_tokens = (w.few ? 1 : 2) * a.tokens_per_tile;
     a.out_bytes = out_bytes(p.out, p.head_dim);
     a.scale_log2 = p.scale * 1.4426950408889634f;
     const bool bf16 = p.dtype == AIE_DT_BF16;
     CUtensorMap q, k, v;
     if (!attn_map(&q, bf16, p.q.data, p.head_dim, p.q_heads, p.q.head_stride, p.tokens, p.q.token_stride, 0, 0, a.group,
                   a.tokens_per_tile) ||
-        !attn_map(&k, bf16, p.k.data, p.head_dim, p.kv_heads, p.k.head_stride, p.keys, p.k.token_stride, 0, 0, 1, kAtTile) ||
-        !attn_map(&v, bf16, p.v.data, p.head_dim, p.kv_heads, p.v.head_stride, p.keys, p.v.token_stride, 0, 0, 1, kAtTile))
+        !attn_map(&k, bf16, p.k.data, p.head_dim, p.kv_heads, p.k.head_stride, p.keys, p.k.token_stride, 0, 0, 1, kCrossBox) ||
+        !attn_map(&v, bf16, p.v.data, p.head_dim, p.kv_heads, p.v.head_stride, p.keys, p.v.token_stride, 0, 0, 1, kCrossBox))
         return fail(AIE_E_CUDA, "cuTensorMapEncodeTiled failed");
     return launched(bf16 ? attn_cross_launch<__nv_bfloat16>(q, k, v, a, w, s) : attn_cross_launch<__half>(q, k, v, a, w, s),
                     "cross attention");

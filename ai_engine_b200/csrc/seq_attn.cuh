@@ -39,6 +39,12 @@
 // joins as the shared prefix's pieces are.  Every block works the cut out from
 // the sequences' lengths, which the host does not know.
 //
+// Where sequences have no more tokens than fill one tile (FEW), both tiles are the
+// same rows, and take the steps in turn: a step's chain of scores, exponentials
+// and products is 1.7 us long, and nothing else would hide it.  (Short questions
+// about long clips, 12 steps a block: 15.6 us for the steps, which is 5.7 TB/s,
+// against 24 with one tile, or with half of every step's keys for each.)
+//
 // Every wait is bounded (1 s); on expiry the block records an error code,
 // waits for its copies in flight, frees its tensor memory and returns.
 #pragma once
@@ -173,6 +179,7 @@ struct AttnArgs {
     float *part_o, *part_lse; // shared prefix: [split][row][d] and [split][row], row = stream * q_heads + head
     int tokens, seqs;         // prompts: packed tokens; shared prefix: streams
     int kv_heads, q_heads, group, d, tokens_per_tile;
+    int pair_tokens;          // states: tokens of a pair of tiles, that of one where both are the same rows
     int causal;
     int out_bytes;            // what `out` is aligned to, in every row: 32, 16 or less
     int shared, max_len, page_size, pages, box_rows, splits, tiles_per_split;
@@ -183,13 +190,14 @@ struct AttnArgs {
     int capacity;             // blocks of a key head that run at once; 0: steps are not cut
 };
 
-constexpr int kAtPrompt = 0, kAtPaged = 1, kAtCross = 2;  // what attn_tc_kernel attends to
+constexpr int kAtPrompt = 0, kAtPaged = 1, kAtCross = 2, kAtFew = 3;  // what attn_tc_kernel attends to
+constexpr int kCrossBox = 32;  // states of a copy
 constexpr int kAtLeast = 4;  // steps that a block is worth starting for: its start and end take about 3
 
-template <int DB>
+template <int DB, bool FEW>
 struct AttnSmem {
-    static constexpr int kStages = DB == 2 ? 5 : 8;
-    static constexpr uint32_t kQ = 2 * DB * kAtBlockBytes;
+    static constexpr int kStages = DB == 2 ? (FEW ? 6 : 5) : 8;
+    static constexpr uint32_t kQ = (FEW ? 1 : 2) * DB * kAtBlockBytes;
     static constexpr uint32_t kStage = DB * kAtBlockBytes;
     static constexpr uint32_t kBytes = kQ + kStages * kStage + 1024 /* alignment */;
 };
@@ -217,7 +225,7 @@ struct CrossWork {
 // lane.  Only the lane that returns true has it.
 __device__ __forceinline__ bool cross_find(const AttnArgs &a, int unit, int pair, int lane, CrossWork &w)
 {
-    const int two = 2 * a.tokens_per_tile;
+    const int two = a.pair_tokens;
     int start[4], len[4], key[4], key_len[4], pairs[4], steps[4];
     auto load = [&](int s0) {
 #pragma unroll
@@ -298,8 +306,9 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const AttnArgs a)
 {
-    constexpr bool PAGED = MODE == kAtPaged, CROSS = MODE == kAtCross;
-    using Sm = AttnSmem<DB>;
+    constexpr bool PAGED = MODE == kAtPaged, FEW = MODE == kAtFew, CROSS = MODE == kAtCross || FEW;
+    constexpr int kTurns = FEW ? 2 : 1;  // tiles that take the steps in turn
+    using Sm = AttnSmem<DB, FEW>;
     extern __shared__ char smem_raw[];
     __shared__ AttnShared sh;
     char *smem = (char *)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -420,18 +429,18 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         }
     }
     // keys seen by a tile's last token; `keys` also bounds the values that exist
-    const int tok0 = w.pair * 2 * tpt;
+    const int tok0 = w.pair * (FEW ? 1 : 2) * tpt;
     const int keys = PAGED ? min(a.shared, a.max_len) : CROSS ? sh.key_len : w.len;
     const int key_first = CROSS ? sh.key_first : w.first;
     const int per_split = PAGED ? a.tiles_per_split : CROSS ? sh.per : 0, step0 = w.split * per_split;
     const bool parts = PAGED || (CROSS && sh.parts > 1);  // a partial result, not the result
     auto steps_of = [&](int t) {
-        const int first = tok0 + t * tpt, last = min(first + tpt, w.len);
+        const int first = tok0 + (FEW ? 0 : t * tpt), last = min(first + tpt, w.len);
         const int seen = first >= w.len ? 0 : (MODE == kAtPrompt && a.causal) ? last : keys;
         const int steps = (seen + kAtTile - 1) / kAtTile;
         return MODE != kAtPrompt ? max(min(steps - step0, per_split), 0) + step0 : steps;
     };
-    const int n0 = steps_of(0), n1 = steps_of(1), n = max(n0, n1);
+    const int n0 = steps_of(0), n1 = FEW && n0 - step0 < 2 ? step0 : steps_of(1), n = max(n0, n1);
     auto n_of = [&](int t) { return t ? n1 : n0; };
     volatile uint32_t *abort = &sh.abort;
     auto wait = [&](uint64_t *bar, uint32_t parity, uint32_t site) {
@@ -445,7 +454,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kAtRowRegs));
         // ---- rows
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
-        const int tok = tok0 + t * tpt + row / a.group, head = w.kvh * a.group + row % a.group;
+        const int tok = tok0 + (FEW ? 0 : t * tpt) + row / a.group, head = w.kvh * a.group + row % a.group;
         const bool real = row < tpt * a.group && tok < w.len;
         int seen = keys;
         if constexpr (PAGED) {
@@ -459,40 +468,40 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         float2 l2 = make_float2(0.f, 0.f);
         bool ok = true;
         const int nt = n_of(t);
-        for (int j = step0; j < nt; j++) {
-            ok = wait(&sh.s_full[t], (j - step0) & 1, 7);
+        for (int j = step0 + (FEW ? t : 0); j < nt; j += kTurns) {
+            ok = wait(&sh.s_full[t], ((j - step0) / kTurns) & 1, 7);
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
             tc_fence_after();
-            float s[128];
+            float s[kAtTile];
 #pragma unroll
-            for (int i = 0; i < 4; i++) tmem_ld32(ts + 32 * i, s + 32 * i);
+            for (int i = 0; i < kAtTile / 32; i++) tmem_ld32(ts + 32 * i, s + 32 * i);
 #pragma unroll
-            for (int i = 0; i < 4; i++) tmem_wait_ld32(s + 32 * i);
+            for (int i = 0; i < kAtTile / 32; i++) tmem_wait_ld32(s + 32 * i);
             const int here = seen - j * kAtTile;
             if (__any_sync(0xffffffffu, here < kAtTile)) {
 #pragma unroll
-                for (int i = 0; i < 128; i++) s[i] = i < here ? s[i] : -INFINITY;
+                for (int i = 0; i < kAtTile; i++) s[i] = i < here ? s[i] : -INFINITY;
             }
             float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-            for (int i = 4; i < 124; i += 8) {
+            for (int i = 4; i < kAtTile - 4; i += 8) {
                 mx[0] = max3(mx[0], s[i], s[i + 1]);
                 mx[1] = max3(mx[1], s[i + 2], s[i + 3]);
                 mx[2] = max3(mx[2], s[i + 4], s[i + 5]);
                 mx[3] = max3(mx[3], s[i + 6], s[i + 7]);
             }
-            mx[0] = max3(mx[0], s[124], s[125]);
-            mx[1] = max3(mx[1], s[126], s[127]);
+            mx[0] = max3(mx[0], s[kAtTile - 4], s[kAtTile - 3]);
+            mx[1] = max3(mx[1], s[kAtTile - 2], s[kAtTile - 1]);
             const float top = fmaxf(max3(mx[0], mx[1], mx[2]), fmaxf(mx[3], m));
             // -inf - -inf is NaN: not greater, nothing to move
             const bool grow = (top - m) * sl > 8.f;
             if (__any_sync(0xffffffffu, grow)) {
                 const float f = grow ? ex2((m - top) * sl) : 1.f;  // from -inf: 0
                 if (grow) m = top;
-                if (j > step0) {
+                if (j >= step0 + kTurns) {
                     l2.x *= f;
                     l2.y *= f;
 #pragma unroll
@@ -509,7 +518,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             const float off = m == -INFINITY ? 0.f : fmaf(-m, sl, kWeightShift<T>);
             const float2 sl2 = make_float2(sl, sl), off2 = make_float2(off, off);
 #pragma unroll
-            for (int c = 0; c < 2; c++) {
+            for (int c = 0; c < kAtTile / 64; c++) {
                 uint32_t p[32];
 #pragma unroll
                 for (int i = 0; i < 32; i++) {
@@ -530,59 +539,104 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const float l = l2.x + l2.y;
         if (nt > step0 && ok) ok = __all_sync(0xffffffffu, wait(&sh.o_full[t], 0, 8));
         tc_fence_after();
-        if (ok && (nt > step0 || MODE != kAtPrompt)) {
-            // of this split's keys; scores of -inf alone (l is 0) count as none here
-            const bool none = nt <= step0 || seen <= step0 * kAtTile || (parts && l == 0.f);
-            const float r = none ? 0.f : 1.f / l;
-            const long long prow = PAGED   ? ((long long)w.split * a.tokens + tok) * a.q_heads + head
-                                   : CROSS ? (long long)blockIdx.x * (2 * kAtTile) + t * kAtTile + row
-                                           : 0;
-            // 32 columns at a time out of tensor memory: a thread holds a row and
-            // writes whole 32-byte sectors of it (16-byte pieces: 2 us a tile, so: 1)
-            const long long at = parts ? prow * a.d : (w.first + tok) * a.out_ts + head * a.out_hs;
-            if (MODE != kAtPrompt && parts) {
-                // log2 of the weights' sum; -inf where nothing was seen
-                if (real) a.part_lse[prow] = none ? -INFINITY : fmaf(m, sl, log2f(l) - kWeightShift<T>);
+        // of this split's keys; scores of -inf alone (l is 0) count as none here
+        const bool none = nt <= step0 || seen <= (step0 + (FEW ? t : 0)) * kAtTile || ((parts || FEW) && l == 0.f);
+        const float r = none ? 0.f : 1.f / l;
+        const float lse = none ? -INFINITY : fmaf(m, sl, log2f(l) - kWeightShift<T>);  // log2 of the weights' sum
+        const long long prow = PAGED   ? ((long long)w.split * a.tokens + tok) * a.q_heads + head
+                               : FEW   ? (long long)blockIdx.x * kAtTile + row
+                               : CROSS ? (long long)blockIdx.x * (2 * kAtTile) + t * kAtTile + row
+                                       : 0;
+        const long long at = parts ? prow * a.d : (w.first + tok) * a.out_ts + head * a.out_hs;
+        // 32 columns at a time out of tensor memory: a thread holds a row and
+        // writes whole 32-byte sectors of it (16-byte pieces: 2 us a tile, so: 1)
+        auto fetch = [&](int c, float (&o)[32]) {
+            if (nt > step0) {
+                tmem_ld32(to + 32 * c, o);
+                tmem_wait_ld32(o);
             }
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = none ? 0.f : o[i] * r;
+        };
+        auto put = [&](int c, float (&o)[32]) {
+#pragma unroll
+            for (int i = 0; i < 32; i += PAGED ? 8 : 16) {
+                if (32 * c + i >= a.d) break;
+                if constexpr (PAGED) {
+                    store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
+                } else if (CROSS && parts) {
+                    store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
+                    if (32 * c + i + 8 < a.d) store32(a.part_o + at + 32 * c + i + 8, (const uint32_t *)&o[i + 8]);
+                } else {
+                    T *dst = (T *)a.out + at + 32 * c + i;
+                    uint32_t v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
+                    if (a.out_bytes == 32) store32(dst, v);
+                    else if (a.out_bytes == 16) {
+                        ((uint4 *)dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
+                        if (32 * c + i + 8 < a.d) ((uint4 *)dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (32 * c + i + e < a.d) dst[e] = from_f32<T>(o[i + e]);
+                    }
+                }
+            }
+        };
+        if constexpr (FEW) {
+            // a row's two results become one: the other tile's thread gets half of the
+            // columns, by way of the ring, which is free once all products are done
+            constexpr int kPad = 32 * DB + 4;
+            float *const halves = (float *)skv, *const lses = halves + 2 * kAtTile * kPad;
+            if (ok && n_of(1 - t) > step0) ok = __all_sync(0xffffffffu, wait(&sh.o_full[1 - t], 0, 8));
+            tc_fence_after();
+            if (ok) {
+                lses[t * kAtTile + row] = lse;
+#pragma unroll 1
+                for (int c = 0; c < DB; c++) {
+                    float o[32];
+                    fetch((1 - t) * DB + c, o);
+                    float4 *const to_ = (float4 *)(halves + (t * kAtTile + row) * kPad + 32 * c);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) to_[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (ok) {
+                const float other = lses[(1 - t) * kAtTile + row], top = fmaxf(lse, other);
+                const float w0 = lse == -INFINITY ? 0.f : ex2(lse - top), w1 = other == -INFINITY ? 0.f : ex2(other - top), sum = w0 + w1;
+                // no keys: zeros; keys with scores of -inf alone: NaN, or a part without weight
+                const float f = sum == 0.f && (parts || !keys) ? 0.f : 1.f / sum;
+                if (parts && t == 0 && real) a.part_lse[prow] = sum == 0.f ? -INFINITY : top + log2f(sum);
+#pragma unroll 1
+                for (int c = t * DB; c < t * DB + DB; c++) {
+                    float o[32];
+                    fetch(c, o);
+                    const float4 *const from = (const float4 *)(halves + ((1 - t) * kAtTile + row) * kPad + 32 * (c - t * DB));
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float4 x = from[i];
+                        o[4 * i] = f * fmaf(w0, o[4 * i], w1 * x.x);
+                        o[4 * i + 1] = f * fmaf(w0, o[4 * i + 1], w1 * x.y);
+                        o[4 * i + 2] = f * fmaf(w0, o[4 * i + 2], w1 * x.z);
+                        o[4 * i + 3] = f * fmaf(w0, o[4 * i + 3], w1 * x.w);
+                    }
+                    if (real) put(c, o);
+                    __syncwarp();
+                }
+            }
+        } else if (ok && (nt > step0 || MODE != kAtPrompt)) {
+            if (MODE != kAtPrompt && parts && real) a.part_lse[prow] = lse;
             bool nan = false;
 #pragma unroll 1
             for (int c = 0; c < 2 * DB; c++) {
                 float o[32];
-                if (nt > step0) {
-                    tmem_ld32(to + 32 * c, o);
-                    tmem_wait_ld32(o);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = none ? 0.f : o[i] * r;
+                fetch(c, o);
                 if (PAGED && seen < keys)
 #pragma unroll
                     for (int i = 0; i < 32; i++) nan |= o[i] != o[i];
-                if (real) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += PAGED ? 8 : 16) {
-                        if (32 * c + i >= a.d) break;
-                        if constexpr (PAGED) {
-                            store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
-                        } else if (CROSS && parts) {
-                            store32(a.part_o + at + 32 * c + i, (const uint32_t *)&o[i]);
-                            if (32 * c + i + 8 < a.d) store32(a.part_o + at + 32 * c + i + 8, (const uint32_t *)&o[i + 8]);
-                        } else {
-                            T *dst = (T *)a.out + at + 32 * c + i;
-                            uint32_t v[8];
-#pragma unroll
-                            for (int e = 0; e < 8; e++) v[e] = pack2<T>(o[i + 2 * e], o[i + 2 * e + 1]);
-                            if (a.out_bytes == 32) store32(dst, v);
-                            else if (a.out_bytes == 16) {
-                                ((uint4 *)dst)[0] = make_uint4(v[0], v[1], v[2], v[3]);
-                                if (32 * c + i + 8 < a.d) ((uint4 *)dst)[1] = make_uint4(v[4], v[5], v[6], v[7]);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 16; e++)
-                                    if (32 * c + i + e < a.d) dst[e] = from_f32<T>(o[i + e]);
-                            }
-                        }
-                    }
-                }
+                if (real) put(c, o);
                 __syncwarp();
             }
             // A stream that ends in the prefix, and a result of NaN: values that it does
@@ -597,7 +651,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             if (n > step0) {
                 if (lane == 0) {
                     const uint32_t q_bytes = (uint32_t)tpt * a.group * 128 * DB;
-                    const int tiles = n1 > step0 ? 2 : 1;
+                    const int tiles = !FEW && n1 > step0 ? 2 : 1;
                     mbar_expect_tx(&sh.q_full, q_bytes * tiles);
                     for (int t = 0; t < tiles; t++)
                         for (int b = 0; b < DB; b++)
@@ -615,9 +669,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 int page = 0, next = 0;
                 if constexpr (PAGED) next = page_of(step0);
                 int issued = 0;
-                for (int i = 0; i < 2 * (n - step0); i++) {
-                    const int st = i % Sm::kStages, round = i / Sm::kStages, step = step0 + i / 2;
-                    const CUtensorMap *tm = i & 1 ? &tm_v : &tm_k;
+                for (int i = 0; i < 2 * (n - step0) + (FEW ? 1 : 0); i++) {
+                    // (FEW: K of two steps, then V of both; an odd last step has no second)
+                    const int st = i % Sm::kStages, round = i / Sm::kStages, step = step0 + (FEW ? i / 4 * 2 + (i & 1) : i / 2);
+                    if (FEW && step >= n) continue;
+                    const CUtensorMap *tm = (FEW ? i & 2 : i & 1) ? &tm_v : &tm_k;
                     char *dst = skv + st * Sm::kStage;
                     int go = 1;
                     if (lane == 0) {
@@ -635,6 +691,11 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                             for (int b = 0; b < DB; b++)
                                 tma_load_4d(dst + b * kAtBlockBytes + lane * rows * 128, tm, &sh.kv_full[st], b * 64, w.kvh,
                                             (step * kAtTile + lane * rows) % a.page_size, page);
+                    } else if constexpr (CROSS) {
+                        // four lanes to 64 elements of 128 states (texts over clips: 589 us, 600 with one)
+                        if (lane < DB * (kAtTile / kCrossBox))
+                            tma_load_3d(dst + lane % DB * kAtBlockBytes + lane / DB * (kCrossBox * 128), tm, &sh.kv_full[st], lane % DB * 64,
+                                        w.kvh, key_first + step * kAtTile + lane / DB * kCrossBox);
                     } else if (lane == 0) {
                         for (int b = 0; b < DB; b++)
                             tma_load_3d(dst + b * kAtBlockBytes, tm, &sh.kv_full[st], b * 64, w.kvh, key_first + step * kAtTile);
@@ -645,7 +706,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 if (*abort && lane == 0) {
                     mbar_wait(&sh.q_full, 0);
                     for (int i = max(issued - Sm::kStages, 0); i < issued; i++)
-                        mbar_wait(&sh.kv_full[i % Sm::kStages], (i / Sm::kStages) & 1);
+                        if (!FEW || step0 + i / 4 * 2 + (i & 1) < n) mbar_wait(&sh.kv_full[i % Sm::kStages], (i / Sm::kStages) & 1);
                 }
                 __syncwarp();
             }
@@ -656,7 +717,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 const uint64_t qd0 = smem_desc_sw128(smem_u32(sq)), kd0 = smem_desc_sw128(smem_u32(skv)),
                                vd0 = smem_desc_mn_sw128(smem_u32(skv));
                 auto s_mma = [&](int t, uint32_t k) {
-                    const uint64_t qd = qd0 + t * (DB * kAtBlockBytes >> 4), kd = kd0 + k * (Sm::kStage >> 4);
+                    const uint64_t qd = qd0 + (FEW ? 0 : t * (DB * kAtBlockBytes >> 4)), kd = kd0 + k * (Sm::kStage >> 4);
 #pragma unroll
                     for (int i = 0; i < 4 * DB; i++) {
                         const uint32_t off = ((i / 4) * kAtBlockBytes + (i % 4) * 32) >> 4;
@@ -673,14 +734,38 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                    !first || i > 0);
                 };
                 bool ok = wait(&sh.q_full, 0, 2) && wait(&sh.kv_full[0], 0, 3);
-                if (ok) {
+                if constexpr (FEW) {
+                    // step i by tile i % 2: its K is copy 4 (i / 2) + i % 2, its V two further on
+                    const int steps = n - step0;
+                    for (int i = 0; ok && i < min(steps, 2); i++) {
+                        if (i && !(ok = wait(&sh.kv_full[i], 0, 3))) break;
+                        tc_fence_after();
+                        s_mma(i, i);
+                        mma_commit(&sh.kv_empty[i]);
+                    }
+                    for (int i = 0; ok && i < steps; i++) {
+                        const int t = i & 1, iv = 2 * (i & ~1) + 2 + t, ik = iv + 2;
+                        const uint32_t par = (i >> 1) & 1;
+                        if (!(ok = wait(&sh.p_full[t][0], par, 6))) break;
+                        tc_fence_after();
+                        o_mma(t, iv % Sm::kStages, 0, i < 2);
+                        if (!(ok = wait(&sh.p_full[t][1], par, 6))) break;
+                        tc_fence_after();
+                        o_mma(t, iv % Sm::kStages, 1, false);
+                        mma_commit(&sh.kv_empty[iv % Sm::kStages]);
+                        if (i + 2 < steps) {
+                            s_mma(t, ik % Sm::kStages);
+                            mma_commit(&sh.kv_empty[ik % Sm::kStages]);
+                        } else mma_commit(&sh.o_full[t]);
+                    }
+                } else if (ok) {
                     tc_fence_after();
                     if (n0 > step0) s_mma(0, 0);
                     if (n1 > step0) s_mma(1, 0);
                     mma_commit(&sh.kv_empty[0]);
                 }
                 uint32_t vj = 1, kj = 2 % Sm::kStages, v_old = 0, k_old = 0;  // ring places of V(j), K(j + 1)
-                for (int j = step0; ok && j < n; j++) {
+                for (int j = step0; !FEW && ok && j < n; j++) {
                     const uint32_t par = (j - step0) & 1;
                     if (j < n0) {
                         if (!(ok = wait(&sh.p_full[0][0], par, 6))) break;
@@ -725,7 +810,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             // wait costs the issuing thread about 200 cycles even when there
             // is nothing to wait for, so it makes as few as it can.)
             for (int j = step0; j < n; j++) {
-                const int iv = 2 * (j - step0) + 1, ik = iv + 1;
+                const int turn = (j - step0) % kTurns, iv = FEW ? 2 * (j - step0 - turn) + 2 + turn : 2 * (j - step0) + 1, ik = FEW ? iv + 2 : iv + 1;
                 bool ok = wait(&sh.kv_full[iv % Sm::kStages], (iv / Sm::kStages) & 1, 4);
                 // values behind the last key may be anything, and 0 times them NaN: zeros
                 const int real = keys - j * kAtTile;
@@ -736,12 +821,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                             *(uint4 *)(skv + iv % Sm::kStages * Sm::kStage + b * kAtBlockBytes + i * 16) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                if (ok && j + 1 < n) ok = wait(&sh.kv_full[ik % Sm::kStages], (ik / Sm::kStages) & 1, 5);
+                if (ok && j + kTurns < n) ok = wait(&sh.kv_full[ik % Sm::kStages], (ik / Sm::kStages) & 1, 5);
                 // one arrival per step
-                for (int t = 0; t < 2 && ok && j > step0; t++)
-                    if (j - 1 < n_of(t)) ok = wait(&sh.p_full[t][0], (j - 1 - step0) & 1, 11);
+                if constexpr (FEW) {
+                    if (ok && j >= step0 + 2) ok = wait(&sh.p_full[turn][0], ((j - step0) / 2 - 1) & 1, 11);
+                } else {
+                    for (int t = 0; t < 2 && ok && j > step0; t++)
+                        if (j - 1 < n_of(t)) ok = wait(&sh.p_full[t][0], (j - 1 - step0) & 1, 11);
+                }
                 if (!__all_sync(0xffffffffu, ok)) break;
-                if (lane == 0) {
+                if (FEW && lane == 0) mbar_arrive(&sh.p_full[turn][0]);
+                else if (lane == 0) {
                     if (j < n0) mbar_arrive(&sh.p_full[0][0]);
                     if (j < n1) mbar_arrive(&sh.p_full[1][0]);
                 }
@@ -758,7 +848,7 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
 // Pairs of tiles whose steps were cut: the parts' results joined, a warp per row.
 constexpr int kJoinRows = 8;  // of a block
-template <typename T>
+template <typename T, bool FEW>
 __global__ void __launch_bounds__(32 * kJoinRows) cross_join_kernel(const AttnArgs a)
 {
     __shared__ CrossWork shared;
@@ -766,7 +856,8 @@ __global__ void __launch_bounds__(32 * kJoinRows) cross_join_kernel(const AttnAr
     behind_last_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int kvh = blockIdx.x % a.kv_heads, unit = blockIdx.x / a.kv_heads;
-    const int i = unit % (2 * kAtTile / kJoinRows) * kJoinRows + warp, pair = unit / (2 * kAtTile / kJoinRows);
+    constexpr int kRows = FEW ? kAtTile : 2 * kAtTile;
+    const int i = unit % (kRows / kJoinRows) * kJoinRows + warp, pair = unit / (kRows / kJoinRows);
     if (threadIdx.x == 0) found = 0;
     __syncthreads();
     if (warp == 0) {
@@ -780,31 +871,32 @@ __global__ void __launch_bounds__(32 * kJoinRows) cross_join_kernel(const AttnAr
     // (the last only where cu is no list of starts, and parts are missing)
     if (!found || shared.parts == 1 || shared.base + shared.parts > a.splits) return;
     const CrossWork w = shared;
-    const int t = i / kAtTile, row = i % kAtTile, tok = (w.pair * 2 + t) * a.tokens_per_tile + row / a.group;
+    const int t = i / kAtTile, row = i % kAtTile, tok = w.pair * a.pair_tokens + t * a.tokens_per_tile + row / a.group;
     const int head = kvh * a.group + row % a.group;
     if (row >= a.tokens_per_tile * a.group || tok >= w.len) return;
-    const long long first = (w.base * a.kv_heads + kvh) * (2 * kAtTile) + i, next = a.kv_heads * (2 * kAtTile);
+    T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs + lane * 4;
+    const long long first = (w.base * a.kv_heads + kvh) * kRows + i, next = a.kv_heads * kRows;
+    const int parts = w.parts;
+    auto at = [&](int part) { return first + part * next; };
     float top = -INFINITY;
-    for (int part = lane; part < w.parts; part += 32) top = fmaxf(top, a.part_lse[first + part * next]);
+    for (int part = lane; part < parts; part += 32) top = fmaxf(top, a.part_lse[at(part)]);
     top = warp_max(top);
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     float sum = 0.f;
-    const float *po = a.part_o + first * a.d + lane * 4;
-    for (int part0 = 0; part0 < w.parts; part0 += 32) {
-        const int n = min(w.parts - part0, 32);
-        const float lse = lane < n ? a.part_lse[first + (part0 + lane) * next] : -INFINITY, mine = lse == -INFINITY ? 0.f : ex2(lse - top);
+    for (int part0 = 0; part0 < parts; part0 += 32) {
+        const int n = min(parts - part0, 32);
+        const float lse = lane < n ? a.part_lse[at(part0 + lane)] : -INFINITY, mine = lse == -INFINITY ? 0.f : ex2(lse - top);
         sum += mine;
 #pragma unroll 8
         for (int k = 0; k < n; k++) {
             const float f = __shfl_sync(0xffffffffu, mine, k);
             if (lane * 4 < a.d) {
-                const float4 y = *(const float4 *)(po + (part0 + k) * next * a.d);
+                const float4 y = *(const float4 *)(a.part_o + at(part0 + k) * a.d + lane * 4);
                 x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
             }
         }
     }
     const float f = 1.f / warp_sum(sum);
-    T *dst = (T *)a.out + (w.first + tok) * a.out_ts + head * a.out_hs + lane * 4;
     if (lane * 4 < a.d) {
         dst[0] = from_f32<T>(x.x * f); dst[1] = from_f32<T>(x.y * f); dst[2] = from_f32<T>(x.z * f); dst[3] = from_f32<T>(x.w * f);
     }
@@ -841,9 +933,9 @@ static cudaError_t attn_launch(const CUtensorMap &q, const CUtensorMap &k, const
                                unsigned grid, cudaStream_t s)
 {
     auto *fn = &attn_tc_kernel<T, DB, MODE>;
-    cudaError_t e = ensure_smem_attr((const void *)fn, AttnSmem<DB>::kBytes);
+    cudaError_t e = ensure_smem_attr((const void *)fn, AttnSmem<DB, MODE == kAtFew>::kBytes);
     if (e != cudaSuccess) return e;
-    return launch_behind(fn, grid, kAtThreads, AttnSmem<DB>::kBytes, s, q, k, v, a);
+    return launch_behind(fn, grid, kAtThreads, AttnSmem<DB, MODE == kAtFew>::kBytes, s, q, k, v, a);
 }
 
 }  // namespace aie

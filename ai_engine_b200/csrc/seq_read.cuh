@@ -129,6 +129,13 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b)
     return *(const uint32_t *)&y;
 }
 
+// a b - y
+__device__ __forceinline__ uint32_t lost2(uint32_t a, uint32_t b, uint32_t y)
+{
+    const __half2 z = __hfma2(*(const __half2 *)&a, *(const __half2 *)&b, __hneg2(*(const __half2 *)&y));
+    return *(const uint32_t *)&z;
+}
+
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b)
 {
     const __half2 y = __hmax2(*(const __half2 *)&a, *(const __half2 *)&b);
@@ -668,6 +675,10 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                             const uint32_t b0 = mul2(pb[nt][mt][0], s0), b1 = mul2(pb[nt][mt][1], s1);
                             mma16816<T>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
                             mma16816<T>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
+                            // what p s lost in f16 (exactly f16 again), times the middle code, to the lo of
+                            // row g: else lo + code s, which cancel, would not lose the same
+                            const uint32_t middle = r == g ? 0x47804780u : 0u;
+                            mma16816<T>(o_lo[nt], {middle, 0u, middle, 0u}, lost2(pb[nt][mt][0], s0, b0), lost2(pb[nt][mt][1], s1, b1));
                         }
                     }
                 } else {

@@ -8,6 +8,13 @@ pages back.  Projections are plain matrix products; everything else of a
 layer is ``attention`` and ``pages``.
 
     python -m ai_engine_b200.decoder [streams] [prompt tokens] [steps]
+
+A second one reads frames: each stream's prompt is a coarse clip and a text,
+whose tokens stand on three axes (time, row, column); the cache is held in 4
+bits; and every layer also attends to the states that an encoder has made of
+the clip's frames, which have a length of their own.
+
+    python -m ai_engine_b200.decoder frames [streams] [frames] [steps]
 """
 from __future__ import annotations
 
@@ -113,7 +120,131 @@ class StreamDecoder:
         return int(self.state.status.item())
 
 
+def grid(frames: int, height: int, width: int, device="cuda") -> torch.Tensor:
+    """Positions [frames * height * width, 3] of a clip's tokens: time, row, column."""
+    i = torch.arange(frames * height * width, dtype=torch.int32, device=device)
+    return torch.stack([i // (height * width), i // width % height, i % width], 1).contiguous()
+
+
+class FrameDecoder:
+    """Layers of x += attention(x) wo over a 4-bit cache, then x += attention of
+    x to the frames' states.  A stream a row, all of them in every call; heads of
+    a multiple of 32."""
+
+    def __init__(self, layers: int, dim: int, q_heads: int, kv_heads: int, head_dim: int, *, streams: int, pages_: int,
+                 page_size: int = 16, max_len: int = 4096, dtype=torch.bfloat16, device="cuda", seed: int = 0):
+        self.dim, self.hq, self.hk, self.d, self.streams = dim, q_heads, kv_heads, head_dim, streams
+        width = -(-max_len // page_size)
+        self.page_size, self.max_len, self.dtype, self.device = page_size, width * page_size, dtype, torch.device(device)
+        g = torch.Generator(device).manual_seed(seed)
+
+        def weight(*shape):
+            return (torch.randn(shape, generator=g, device=device) * shape[0] ** -0.5).to(dtype)
+        heads = (q_heads + 2 * kv_heads) * head_dim
+        self.wqkv = [weight(dim, heads) for _ in range(layers)]
+        self.wo = [weight(q_heads * head_dim, dim) for _ in range(layers)]
+        self.wq, self.wkv = ([weight(dim, n * head_dim) for _ in range(layers)] for n in (q_heads, 2 * kv_heads))
+        self.wx = [weight(q_heads * head_dim, dim) for _ in range(layers)]
+        self.norms = [1.0 + 0.1 * torch.randn(2, head_dim, generator=g, device=device) for _ in range(layers)]
+        self.table = angles(self.max_len, head_dim, device=device)
+        # a quarter of a head's pairs for time, the rest for rows and columns
+        pairs = head_dim // 2
+        axis = torch.arange(pairs, device=device) >= pairs // 4
+        self.axis = (axis.int() + (torch.arange(pairs, device=device) >= pairs - (pairs - pairs // 4) // 2).int()).to(torch.uint8)
+        self.kv = pages.new_cache4(layers, pages_, page_size, kv_heads, head_dim, device)
+        self.state = pages.new_state(pages_, streams, width, device)
+        self.rows = torch.arange(streams, dtype=torch.int32, device=device)
+        self.states, self.starts, self.begun = [], None, False
+
+    def _starts(self, lens: Sequence[int]) -> torch.Tensor:
+        cu = [0]
+        for n in lens:
+            cu.append(cu[-1] + n)
+        return torch.tensor(cu, dtype=torch.int32, device=self.device)
+
+    def watch(self, states: torch.Tensor, lens: Sequence[int]) -> None:
+        """The encoder's states of all streams' frames, packed [states, dim]:
+        lens[s] of them are stream s's (none is possible)."""
+        if len(lens) != self.streams or sum(lens) != states.shape[0]:
+            raise ValueError(f"{len(lens)} lengths, {sum(lens)} in all, for {states.shape[0]} states of {self.streams} streams")
+        kv = [(states @ w).view(-1, 2, self.hk, self.d) for w in self.wkv]
+        self.states, self.starts = [(x[:, 0], x[:, 1]) for x in kv], self._starts(lens)
+
+    def _watching(self) -> None:
+        if self.starts is None:
+            raise ValueError("the streams have nothing to watch yet")
+
+    def _layer(self, i: int, x: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, attend, cu) -> torch.Tensor:
+        qkv = (x @ self.wqkv[i]).view(x.shape[0], self.hq + 2 * self.hk, self.d)
+        q, k, v = qkv.split([self.hq, self.hk, self.hk], 1)
+        q, k = attention.qk_norm_rope(q, k, positions, self.table, pair_axis=self.axis, q_weight=self.norms[i][0],
+                                      k_weight=self.norms[i][1], q_out=q, k_out=k)
+        attention.kv4_file(k, v, self.kv[i, 0], self.kv[i, 1], slots)
+        x = x + attend(i, q, k, v).reshape(x.shape[0], -1) @ self.wo[i]
+        q = (x @ self.wq[i]).view(x.shape[0], self.hq, self.d)
+        o = attention.cross_attention(q, *self.states[i], self.starts, cu_q=cu)
+        return x + o.reshape(x.shape[0], -1) @ self.wx[i]
+
+    def prompt(self, x: torch.Tensor, positions: torch.Tensor, lens: Sequence[int]) -> torch.Tensor:
+        """All streams' prompts, packed [tokens, dim], each lens[s] tokens at
+        positions [tokens, 3]; the rows are empty.  Each part of a prompt is
+        attended as it is, not as the cache holds it."""
+        if len(lens) != self.streams or sum(lens) != x.shape[0]:
+            raise ValueError(f"{len(lens)} lengths, {sum(lens)} in all, for {x.shape[0]} tokens of {self.streams} streams")
+        self._watching()
+        if self.begun:
+            raise ValueError("the rows hold tokens already")
+        self.begun = True
+        cu = self._starts(lens)
+        slots = pages.grow(self.state, self.page_size, self.rows, cu[1:] - cu[:-1], x.shape[0])
+        for i in range(len(self.wqkv)):
+            x = self._layer(i, x, positions, slots, lambda _, q, k, v: attention.prompt_attention(q, k, v, cu), cu)
+        return x
+
+    def step(self, x: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
+        """One token for each stream [streams, dim], at positions [streams, 3]."""
+        self._watching()
+        self.begun = True
+        slots = pages.grow(self.state, self.page_size, self.rows, torch.ones_like(self.rows), self.streams)
+
+        def attend(i, q, k, v):
+            return attention.kv4_attention(q, self.kv[i, 0], self.kv[i, 1], self.state.table, self.state.lens, max_len=self.max_len)
+        for i in range(len(self.wqkv)):
+            x = self._layer(i, x, positions, slots, attend, None)
+        return x
+
+    def status(self) -> int:
+        """What the cache's calls could not do (waits for the device)."""
+        return int(self.state.status.item())
+
+
+def frames_main(argv: List[str]) -> None:
+    streams, frames, steps = (int(v) for v in (argv + ["16", "32", "64"][len(argv):]))
+    coarse, text = grid(frames, 5, 9), 40  # a clip of 5 x 9 tokens a frame, and a text behind it
+    n = coarse.shape[0] + text
+    m = FrameDecoder(4, 1024, 16, 4, 128, streams=streams, pages_=streams * -(-(n + steps) // 16) + 8, max_len=n + steps)
+    g = torch.Generator("cuda").manual_seed(1)
+
+    def rand(tokens):
+        return torch.randn(tokens, 1024, generator=g, device="cuda").bfloat16()
+    m.watch(rand(streams * frames * 180), [frames * 180] * streams)  # 10 x 18 states a frame
+    after = max(frames, 9) + torch.arange(text + steps, dtype=torch.int32, device="cuda")[:, None].expand(-1, 3)
+    m.prompt(rand(streams * n), torch.cat([coarse, after[:text]]).repeat(streams, 1), [n] * streams)
+    x = rand(streams)
+    m.step(x, after[text:text + 1].repeat(streams, 1))
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    for i in range(1, steps):
+        x = m.step(x, after[text + i:text + i + 1].repeat(streams, 1))
+    b.record()
+    b.synchronize()
+    print(f"{streams} streams, {frames} frames each: {a.elapsed_time(b) / max(1, steps - 1) * 1e3:.0f} us a step of 4 layers over "
+          f"{n} tokens in 4 bits and {frames * 180} states; status {m.status()}")
+
+
 def main(argv: List[str]) -> None:
+    if argv[:1] == ["frames"]:
+        return frames_main(argv[1:])
     streams, prompt, steps = (int(v) for v in (argv + ["32", "2000", "64"][len(argv):]))
     need = -(-prompt // 16) + streams * (steps // 16 + 2) + 8
     m = StreamDecoder(4, 1024, 16, 4, 128, streams=streams, pages_=need, max_len=prompt + steps + 1)

@@ -121,3 +121,9 @@ def test_python_refuses_host_tensors(lib):
         attention.kv4_attention(q, kv[0, 0], kv[0, 1], i.view(1, 4), i[:1])
     with pytest.raises(TypeError):
         attention.qk_norm_rope(q, q, i, torch.zeros(4, 64), pair_axis=torch.zeros(32, dtype=torch.uint8))
+
+
+def test_grid_of_a_clip():
+    from ai_engine_b200 import decoder
+    p = decoder.grid(2, 2, 3, device="cpu")
+    assert p.dtype == torch.int32 and p.tolist() == [[t, r, c] for t in range(2) for r in range(2) for c in range(3)]

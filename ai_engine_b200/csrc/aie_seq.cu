@@ -543,11 +543,12 @@ static int cross_read(const aie_cross &p, cudaStream_t s)
     ReadArgs a = {};
     const ReadPlan w = read_plan(false, p.seqs, p.keys, p.kv_heads, p.q_heads / p.kv_heads, p.head_dim);
     if (w.tiles > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^35 (state, key head) pairs in one call");
+    a.seqs = (int)p.seqs;
     read_args(a, w, p.q, p.out, p.workspace);
     a.k = p.k.data; a.k_ts = p.k.token_stride; a.k_hs = p.k.head_stride;
     a.v = p.v.data; a.v_ts = p.v.token_stride; a.v_hs = p.v.head_stride;
     a.cu = p.cu_k; a.keys = (int)p.keys;
-    a.seqs = (int)p.seqs; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
+    a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
     a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
     return launched(a.bf16 ? read16_launch<__nv_bfloat16>(a, w.nt, s) : read16_launch<__half>(a, w.nt, s), "cross attention");
 }
@@ -649,10 +650,11 @@ static int kv4_step(const aie_kv4_step &p, cudaStream_t s)
     ReadArgs a = {};
     const ReadPlan w = kv4_plan(p);
     if (w.tiles > 0x7fffffffull) return fail(AIE_E_UNSUPPORTED, "more than 2^36 (place, key head) pairs in one call");
+    a.seqs = (int)p.batch;
     read_args(a, w, p.q, p.out, p.workspace);
     a.g = kv4_geom(p.cache); a.size = make_fastdiv(a.g.size);
     a.table = p.table; a.lens = p.lens; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
-    a.seqs = (int)p.batch; a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads); a.d = a.g.d;
+    a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads); a.d = a.g.d;
     a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
     cudaError_t e;
     switch (a.d / 32) {

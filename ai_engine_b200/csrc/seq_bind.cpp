@@ -415,7 +415,7 @@ void check_kv4(const at::Tensor &t, const char *name, int device)
 aie_kv4 cache4(const at::Tensor &k, const at::Tensor &v, int device)
 {
     check_kv4(k, "k_pages", device);
-    check_kv4(v, "v_pages", device);
+    check_kv4(v, "v_pages", (int)k.get_device());
     if (k.sizes() != v.sizes() || k.strides() != v.strides())
         refuse(PyExc_ValueError, "k_pages and v_pages must have the same shape and strides");
     return {k.data_ptr(), v.data_ptr(), k.stride(0), u32(k.size(0), "pages"), u32(k.size(2), "page_size"), u32(k.size(1), "kv_heads"),

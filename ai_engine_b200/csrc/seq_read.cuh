@@ -58,6 +58,7 @@ struct ReadArgs {
     unsigned *before;        // [seqs + 1]: tiles of the sequences before
     float *part_lse, *part_o;
     int workers;
+    unsigned parts_each;     // host: of a sequence and head, where its share is like the others'
 };
 
 __device__ __forceinline__ int read_len(const ReadArgs &a, int s)
@@ -756,7 +757,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 }
 
 // Sequences whose tiles more than one warp took, and those without any: a block
-// per sequence and query head.
+// per sequence and query head, of more warps where there are more parts.
 struct JoinArgs {
     void *out;
     long long o_ts, o_hs;
@@ -765,9 +766,12 @@ struct JoinArgs {
     int seqs, hq, group, d, zs, heads, rows, bf16, workers;
 };
 
-__global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
+template <int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
 {
-    __shared__ float sums[kRdWarps][256], weights[kRdWarps];
+    constexpr bool MANY = WARPS > 4;
+    extern __shared__ float weight[];  // MANY: of each part
+    __shared__ float sums[WARPS][256], tops[WARPS], totals[WARPS];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int s = blockIdx.x / a.hq, h = blockIdx.x % a.hq, kvh = h / a.group, in = h % a.group;
     const int head = kvh * a.zs + in / a.rows, row = in % a.rows;
@@ -779,7 +783,7 @@ __global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
         else ((__half *)a.out)[oat + d] = __float2half_rn(x);
     };
     if (n == 0) {
-        for (int d = threadIdx.x; d < a.d; d += kRdThreads) store(d, 0.f);
+        for (int d = threadIdx.x; d < a.d; d += 32 * WARPS) store(d, 0.f);
         return;
     }
     const unsigned share = read_share(tiles * a.heads, a.workers), at = head * tiles + from, first = at / share;
@@ -787,7 +791,7 @@ __global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
     if (parts == 1) return;
     const long long id = (long long)first + (long long)head * a.seqs + s, next = (long long)a.rows * a.d;
     const float *lse = a.part_lse + id * a.rows + row, *po = a.part_o + (id * a.rows + row) * a.d + lane * 4;
-    // a warp every fourth part, a lane four neighbouring elements (of 128 at a time);
+    // a warp every WARPS-th part, a lane four neighbouring elements (of 128 at a time);
     // the first on their way before the weights are known
     constexpr int kFirst = 2;
     float4 y[kFirst][2];
@@ -795,37 +799,80 @@ __global__ void __launch_bounds__(kRdThreads) read_join_kernel(const JoinArgs a)
     for (int i = 0; i < kFirst; i++)
 #pragma unroll
         for (int k = 0; k < 2; k++)
-            if (warp + i * kRdWarps < parts && k * 128 + lane * 4 < a.d)
-                y[i][k] = *(const float4 *)(po + (warp + i * kRdWarps) * next + k * 128);
-    float top = -INFINITY;
-    for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[(long long)i * a.rows]);
-    top = warp_max(top);
+            if (warp + i * WARPS < parts && k * 128 + lane * 4 < a.d)
+                y[i][k] = *(const float4 *)(po + (warp + i * WARPS) * next + k * 128);
+    float top = -INFINITY, sum = 0.f;
     float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-    float sum = 0.f;
-    auto add = [&](int i, const float4 (&z)[2]) {
-        const float w = lse[(long long)i * a.rows], f = w == -INFINITY ? 0.f : ex2(w - top);
-        sum += f;
+    auto weigh = [&](float w) { return w == -INFINITY ? 0.f : ex2(w - top); };
+    auto add = [&](float f, const float4 (&z)[2]) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
             if (k * 128 + lane * 4 < a.d) add_scaled(x[k], f, z[k]);
     };
-#pragma unroll
-    for (int i = 0; i < kFirst; i++)
-        if (warp + i * kRdWarps < parts) add(warp + i * kRdWarps, y[i]);
-#pragma unroll 4
-    for (int i = warp + kFirst * kRdWarps; i < parts; i += kRdWarps) {
-        float4 z[2];
+    auto load = [&](int i, float4 (&z)[2]) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
             if (k * 128 + lane * 4 < a.d) z[k] = *(const float4 *)(po + i * next + k * 128);
-        add(i, z);
+    };
+    if constexpr (MANY) {
+        // the weights first, by all threads
+        for (int i = threadIdx.x; i < parts; i += 32 * WARPS) {
+            const float w = lse[(long long)i * a.rows];
+            weight[i] = w;
+            top = fmaxf(top, w);
+        }
+        top = warp_max(top);
+        if (lane == 0) tops[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) top = fmaxf(top, tops[i]);
+        for (int i = threadIdx.x; i < parts; i += 32 * WARPS) {
+            weight[i] = weigh(weight[i]);
+            sum += weight[i];
+        }
+        sum = warp_sum(sum);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kFirst; i++)
+            if (warp + i * WARPS < parts) add(weight[warp + i * WARPS], y[i]);
+#pragma unroll 8
+        for (int i = warp + kFirst * WARPS; i < parts; i += WARPS) {
+            float4 z[2];
+            load(i, z);
+            add(weight[i], z);
+        }
+    } else {
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[(long long)i * a.rows]);
+        top = warp_max(top);
+#pragma unroll
+        for (int i = 0; i < kFirst; i++)
+            if (warp + i * WARPS < parts) {
+                const float f = weigh(lse[(long long)(warp + i * WARPS) * a.rows]);
+                sum += f;
+                add(f, y[i]);
+            }
+#pragma unroll 4
+        for (int i = warp + kFirst * WARPS; i < parts; i += WARPS) {
+            float4 z[2];
+            load(i, z);
+            const float f = weigh(lse[(long long)i * a.rows]);
+            sum += f;
+            add(f, z);
+        }
     }
+    if (lane == 0) totals[warp] = sum;
 #pragma unroll
     for (int k = 0; k < 2; k++) *(float4 *)&sums[warp][k * 128 + lane * 4] = x[k];
-    if (lane == 0) weights[warp] = sum;
     __syncthreads();
-    const float all = 1.f / (weights[0] + weights[1] + weights[2] + weights[3]);
-    for (int d = threadIdx.x; d < a.d; d += kRdThreads) store(d, (sums[0][d] + sums[1][d] + sums[2][d] + sums[3][d]) * all);
+    float all = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; i++) all += totals[i];
+    for (int d = threadIdx.x; d < a.d; d += 32 * WARPS) {
+        float z = 0.f;
+#pragma unroll
+        for (int i = 0; i < WARPS; i++) z += sums[i][d];
+        store(d, z / all);
+    }
 }
 
 // --------------------------------------------------------------- host ---
@@ -871,7 +918,14 @@ static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
     if (e != cudaSuccess) return e;
     const JoinArgs j{a.out, a.o_ts, a.o_hs, a.before, a.part_lse, a.part_o, a.seqs, a.hq, a.group, a.d, a.zs, a.heads, a.rows, a.bf16,
                      a.workers};
-    return launch_behind(read_join_kernel, (unsigned)((long long)a.seqs * a.hq), kRdThreads, 0, s, j);
+    // warps a row, by its parts: with two each (256 streams of up to 1900 places in 4 bits)
+    // 87.4 us a call of two warps, 91.3 of four; with three (96 of 5000) 83.4 and 81.5; with
+    // 600 (one of 9682 states) 14.8 of sixteen, 21 of eight, 31 of four; with 15, 14.4 of
+    // four and 15.5 of sixteen
+    const unsigned rows = (unsigned)((long long)a.seqs * a.hq);
+    if (a.parts_each <= 2) return launch_behind(read_join_kernel<2>, rows, 64, 0, s, j);
+    if (a.parts_each <= 24) return launch_behind(read_join_kernel<4>, rows, 128, 0, s, j);
+    return launch_behind(read_join_kernel<16>, rows, 512, (a.workers + 2) * 4, s, j);
 }
 
 static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const aie_heads &out, void *workspace)
@@ -879,6 +933,7 @@ static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const 
     a.q = q.data; a.q_ts = q.token_stride; a.q_hs = q.head_stride;
     a.out = out.data; a.o_ts = out.token_stride; a.o_hs = out.head_stride;
     a.zs = w.zs; a.heads = w.heads; a.rows = w.rows; a.workers = w.workers;
+    a.parts_each = (unsigned)(std::min<uint64_t>(w.workers, w.tiles) / ((uint64_t)w.heads * a.seqs)) + 1;
     char *ws = (char *)(((uintptr_t)workspace + 31) / 32 * 32);
     a.before = (unsigned *)ws;
     auto vec = [](const aie_heads &h) {

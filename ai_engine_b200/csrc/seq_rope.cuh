@@ -26,13 +26,12 @@ struct RopeArgs {
     int axes;             // positions of a token
 };
 
-// The cosines and sines of pair i of token t: its own row of the table where the
-// positions have axes.
-template <typename T>
+// The table's row for a token's position (along an axis), nullptr outside it.
+template <bool AXES, typename T>
 __device__ __forceinline__ const float *rope_angles(const RopeArgs<T> &a, int t, int axis)
 {
-    if (axis >= a.axes) return nullptr;
-    const int pos = a.pos[(long long)t * a.axes + axis];
+    if (AXES && axis >= a.axes) return nullptr;
+    const int pos = a.pos[AXES ? (long long)t * a.axes + axis : t];
     return pos >= 0 && pos < a.max_pos ? a.cs + (long long)pos * a.rot : nullptr;
 }
 
@@ -90,14 +89,14 @@ __global__ void __launch_bounds__(128) rope_row_kernel(RopeArgs<T> a)
     T *o1 = key ? (a.ko.p ? a.ko.at(t, h) : nullptr) : a.qo.at(t, h);
     T *o2 = key ? rope_slot(a.kp, a.pg, a.slots, t, h) : nullptr;
     const int half = a.rot >> 1;
-    const float *cs = !AXES && a.rot ? rope_angles(a, t, 0) : nullptr;
+    const float *cs = !AXES && a.rot ? rope_angles<AXES>(a, t, 0) : nullptr;
     for (int i = lane; i < a.d; i += 32) {
         float v = y[i];
         if (i < a.rot) {
             const int f = a.interleaved ? i >> 1 : (i < half ? i : i - half);
             const bool first = a.interleaved ? !(i & 1) : i < half;
             const float other = y[a.interleaved ? i ^ 1 : (first ? i + half : i - half)];
-            if constexpr (AXES) cs = rope_angles(a, t, a.axis[f]);
+            if constexpr (AXES) cs = rope_angles<AXES>(a, t, a.axis[f]);
             if (cs) {
                 const float c = cs[f], s = cs[half + f];
                 v = first ? v * c - other * s : v * c + other * s;
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
             uint2 ax = make_uint2(0, 0);  // their axes
             if constexpr (AXES) ax = *(const uint2 *)(a.axis + lane * 8);
             if (!AXES || (ax.x == ax.y && ax.x == (ax.x & 255) * 0x01010101u)) {
-                if (const float *cs = rope_angles(a, t, ax.x & 255)) {
+                if (const float *cs = rope_angles<AXES>(a, t, ax.x & 255)) {
                     load8f(cs + lane * 8, c);
                     load8f(cs + lane * 8 + half, sn);
                 } else {
@@ -279,7 +278,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
             } else {
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const float *cs = rope_angles(a, t, ((k < 4 ? ax.x : ax.y) >> 8 * (k & 3)) & 255);
+                    const float *cs = rope_angles<AXES>(a, t, ((k < 4 ? ax.x : ax.y) >> 8 * (k & 3)) & 255);
                     c[k] = cs ? cs[lane * 8 + k] : __int_as_float(0x7fffffff);
                     sn[k] = cs ? cs[lane * 8 + k + half] : __int_as_float(0x7fffffff);
                 }

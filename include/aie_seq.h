@@ -106,9 +106,10 @@ AIE_API int aie_prompt_attn(const aie_prompt *p, void *stream);
  * Both lists (device, [seqs + 1], not decreasing, within 0 .. tokens and 0 ..
  * keys) are read on the device.  A sequence without states gives zeros; tokens
  * of no sequence are left unwritten.  Values of other sequences, infinities and
- * NaN among them, never reach a result.
- * workspace: aie_cross_attn_workspace(p) bytes, 16-byte aligned, its contents
- * unspecified before and after; calls that may overlap need one each. */
+ * NaN among them, never reach a result.  out overlaps no input.
+ * workspace: aie_cross_attn_workspace(p) bytes (p as in the call, apart from
+ * these two), 16-byte aligned, its contents unspecified before and after; calls
+ * that may overlap need one each. */
 typedef struct aie_cross {
     aie_heads q, k, v, out;
     const int32_t *cu_q, *cu_k;
@@ -189,7 +190,7 @@ AIE_API int aie_kv4_load(const aie_kv4_rows *p, void *stream);
  * count as max_len.  table and lens are read on the device.  Page numbers
  * outside the cache are never read from; the stream's result is then
  * unspecified.  Places from lens[b] on, whatever they hold, never reach stream
- * b's result.
+ * b's result.  out overlaps no input.
  * workspace: aie_kv4_attn_workspace(p) bytes, 16-byte aligned, its contents
  * unspecified before and after; calls that may overlap need one each. */
 typedef struct aie_kv4_step {

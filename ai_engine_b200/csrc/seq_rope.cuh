@@ -169,16 +169,50 @@ __device__ __forceinline__ Vec8<T> pack8(const float *f)
     return v;
 }
 
-__device__ __forceinline__ void load8f(const float *p, float *f)
+// A piece of 8 elements, or of 4 16-bit ones.
+template <typename T, int N>
+struct Piece : Vec8<T> {
+    __device__ __forceinline__ void load(const T *p) { *(Vec8<T> *)this = load8(p); }
+    __device__ __forceinline__ void store(T *p) const { store8(p, *this); }
+    __device__ __forceinline__ void unpack(float *f) const { unpack8<T>(*this, f); }
+    __device__ __forceinline__ void pack(const float *f) { *(Vec8<T> *)this = pack8<T>(f); }
+};
+template <typename T>
+struct Piece<T, 4> {
+    static_assert(sizeof(T) == 2, "16-bit elements");
+    uint2 u;
+    __device__ __forceinline__ void load(const T *p)
+    {
+        asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(u.x), "=r"(u.y) : "l"(p));
+    }
+    __device__ __forceinline__ void store(T *p) const { *(uint2 *)p = u; }
+    __device__ __forceinline__ void unpack(float *f) const
+    {
+        const uint32_t w[2] = {u.x, u.y};
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const float2 y = std::is_same<T, __half>::value ? __half22float2(*(const __half2 *)&w[i])
+                                                            : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+            f[2 * i] = y.x;
+            f[2 * i + 1] = y.y;
+        }
+    }
+    __device__ __forceinline__ void pack(const float *f) { u = make_uint2(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3])); }
+};
+
+template <int N>
+__device__ __forceinline__ void load_floats(const float *p, float *f)
 {
-    const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+        const float4 a = *(const float4 *)(p + i);
+        f[i] = a.x; f[i + 1] = a.y; f[i + 2] = a.z; f[i + 3] = a.w;
+    }
 }
 
 // Heads in whole 16-element pieces, everything 16-byte aligned: LPR lanes per
-// head (a power of two, at least d / 16), each with two pieces of 8 elements
-// that the rotation pairs with each other, so that it needs no exchange: with
+// head (a power of two, at least d / 2 N), each with two pieces of N = 8 elements
+// (4 for heads that allow no more) that the rotation pairs with each other, so that it needs no exchange: with
 // halves, elements i and i + rot / 2; interleaved or not rotated, neighbours.
 // A lane keeps its pieces' weights and its token's angles in registers for
 // HPT heads of the token, whose loads are all in flight at once.
@@ -197,7 +231,7 @@ struct RopeVec {
     float inv_d;
 };
 
-template <typename T, int LPR, int HPT, bool INTERLEAVED, bool AXES>
+template <typename T, int LPR, int HPT, bool INTERLEAVED, bool AXES, int N>
 __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(const RopeArgs<T> a, const RopeVec g)
 {
     behind_last_launch();
@@ -211,21 +245,21 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
     const unsigned per = key ? g.k_units : g.q_units;
     const int t = (int)(unit / per), h0 = (int)(unit - (unsigned)t * per) * HPT;
     const int n = min(HPT, (key ? a.hk : a.hq) - h0);
-    const bool on = lane * 16 < a.d;
+    const bool on = lane * (2 * N) < a.d;
     // the lane's pieces: elements e0 and e0 + gap on
     const int half = a.rot >> 1;
-    const bool turn = !value && lane * 16 < a.rot;
-    const int e0 = !INTERLEAVED && turn ? lane * 8 : lane * 16, gap = !INTERLEAVED && turn ? half : 8;
+    const bool turn = !value && lane * (2 * N) < a.rot;
+    const int e0 = !INTERLEAVED && turn ? lane * N : lane * (2 * N), gap = !INTERLEAVED && turn ? half : N;
 
     const HeadsOf<T> &src = value ? a.v : key ? a.k : a.q;
-    Vec8<T> x[HPT][2];
+    Piece<T, N> x[HPT][2];
     if (on) {
         const T *p = src.at(t, h0) + e0;
 #pragma unroll
         for (int i = 0; i < HPT; i++)
             if (i < n) {
-                x[i][0] = load8(p);
-                x[i][1] = load8(p + gap);
+                x[i][0].load(p);
+                x[i][1].load(p + gap);
                 p += src.hs;
             }
     }
@@ -246,8 +280,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
 #pragma unroll
         for (int i = 0; i < HPT; i++)
             if (on && page && i < n) {
-                store8(page, x[i][0]);
-                store8(page + gap, x[i][1]);
+                x[i][0].store(page);
+                x[i][1].store(page + gap);
                 page += a.pg.hs;
             }
         return;
@@ -255,47 +289,48 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
     // y0 = r (x0 a0 + x1 b0), y1 = r (x1 a1 + x0 b1): weight and angle in one
     // factor, the same for all heads of the token.  Two elements to a register pair.
     const float *w = key ? a.wk : a.wq;
-    float2 a0[4], a1[4], b0[4], b1[4];
+    float2 a0[N / 2], a1[N / 2], b0[N / 2], b1[N / 2];
     if (on) {
-        float c[8], sn[8], w0[8], w1[8];
+        float c[N], sn[N], w0[N], w1[N];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
+        for (int k = 0; k < N; k++) {
             c[k] = w0[k] = w1[k] = 1.f;
             sn[k] = 0.f;
         }
         if (turn) {
-            // angles: e0 .. e0 + 7 of the halves, or of the eight neighbouring pairs
+            // angles: e0 .. e0 + N - 1 of the halves, or of the N neighbouring pairs
             uint2 ax = make_uint2(0, 0);  // their axes
-            if constexpr (AXES) ax = *(const uint2 *)(a.axis + lane * 8);
+            if constexpr (AXES && N == 8) ax = *(const uint2 *)(a.axis + lane * N);
+            else if constexpr (AXES) ax.x = ax.y = *(const uint32_t *)(a.axis + lane * N);
             if (!AXES || (ax.x == ax.y && ax.x == (ax.x & 255) * 0x01010101u)) {
                 if (const float *cs = rope_angles<AXES>(a, t, ax.x & 255)) {
-                    load8f(cs + lane * 8, c);
-                    load8f(cs + lane * 8 + half, sn);
+                    load_floats<N>(cs + lane * N, c);
+                    load_floats<N>(cs + lane * N + half, sn);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < 8; k++) c[k] = sn[k] = __int_as_float(0x7fffffff);
+                    for (int k = 0; k < N; k++) c[k] = sn[k] = __int_as_float(0x7fffffff);
                 }
             } else {
 #pragma unroll
-                for (int k = 0; k < 8; k++) {
+                for (int k = 0; k < N; k++) {
                     const float *cs = rope_angles<AXES>(a, t, ((k < 4 ? ax.x : ax.y) >> 8 * (k & 3)) & 255);
-                    c[k] = cs ? cs[lane * 8 + k] : __int_as_float(0x7fffffff);
-                    sn[k] = cs ? cs[lane * 8 + k + half] : __int_as_float(0x7fffffff);
+                    c[k] = cs ? cs[lane * N + k] : __int_as_float(0x7fffffff);
+                    sn[k] = cs ? cs[lane * N + k + half] : __int_as_float(0x7fffffff);
                 }
             }
         }
         if (w) {
-            load8f(w + e0, w0);
-            load8f(w + e0 + gap, w1);
+            load_floats<N>(w + e0, w0);
+            load_floats<N>(w + e0 + gap, w1);
         }
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < N / 2; k++) {
             const int i = 2 * k, j = i + 1;
             if (INTERLEAVED && turn) {  // pairs (i, j) of either piece; b goes with the pair swapped
                 a0[k] = make_float2(w0[i] * c[k], w0[j] * c[k]);
                 b0[k] = make_float2(-w0[j] * sn[k], w0[i] * sn[k]);
-                a1[k] = make_float2(w1[i] * c[k + 4], w1[j] * c[k + 4]);
-                b1[k] = make_float2(-w1[j] * sn[k + 4], w1[i] * sn[k + 4]);
+                a1[k] = make_float2(w1[i] * c[k + N / 2], w1[j] * c[k + N / 2]);
+                b1[k] = make_float2(-w1[j] * sn[k + N / 2], w1[i] * sn[k + N / 2]);
             } else {
                 a0[k] = make_float2(w0[i] * c[i], w0[j] * c[j]);
                 b0[k] = make_float2(-w1[i] * sn[i], -w1[j] * sn[j]);
@@ -309,17 +344,17 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
 #pragma unroll
     for (int i = 0; i < HPT; i++) {
         if (i >= n) break;
-        float2 f0[4], f1[4];
+        float2 f0[N / 2], f1[N / 2];
         float r = 1.f;
         if (on) {
-            unpack8(x[i][0], (float *)f0);
-            unpack8(x[i][1], (float *)f1);
+            x[i][0].unpack((float *)f0);
+            x[i][1].unpack((float *)f1);
         }
         if (w) {
             float2 sum = make_float2(0.f, 0.f);
             if (on)
 #pragma unroll
-                for (int k = 0; k < 4; k++) sum = __ffma2_rn(f0[k], f0[k], __ffma2_rn(f1[k], f1[k], sum));
+                for (int k = 0; k < N / 2; k++) sum = __ffma2_rn(f0[k], f0[k], __ffma2_rn(f1[k], f1[k], sum));
             float total = sum.x + sum.y;
 #pragma unroll
             for (int o = LPR / 2; o; o >>= 1) total += __shfl_xor_sync(mask, total, o);
@@ -328,7 +363,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
         if (!on) continue;
         const float2 r2 = make_float2(r, r);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < N / 2; k++) {
             const float2 p = f0[k], q = f1[k];
             float2 y0 = __fmul2_rn(p, a0[k]), y1 = __fmul2_rn(q, a1[k]);
             if (turn) {
@@ -338,31 +373,37 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) rope_vec_kernel(con
             f0[k] = __fmul2_rn(y0, r2);
             f1[k] = __fmul2_rn(y1, r2);
         }
-        const Vec8<T> y0 = pack8<T>((const float *)f0), y1 = pack8<T>((const float *)f1);
+        Piece<T, N> y0, y1;
+        y0.pack((const float *)f0);
+        y1.pack((const float *)f1);
         if (out) {
-            store8(out, y0);
-            store8(out + gap, y1);
+            y0.store(out);
+            y1.store(out + gap);
             out += dst.hs;
         }
         if (page) {
-            store8(page, y0);
-            store8(page + gap, y1);
+            y0.store(page);
+            y1.store(page + gap);
             page += a.pg.hs;
         }
     }
 }
 
+// Pieces of n elements.
 template <typename T>
-static bool rope_vec_ok(const RopeArgs<T> &a)
+static bool rope_vec_ok(const RopeArgs<T> &a, int n)
 {
-    const long long unit = 16 / sizeof(T);
-    auto ok = [&](const HeadsOf<T> &h) { return !h.p || ((uintptr_t)h.p % 16 == 0 && h.ts % unit == 0 && h.hs % unit == 0); };
-    auto ptr = [](const void *p) { return (uintptr_t)p % 16 == 0; };
-    return a.d % 16 == 0 && a.rot % 16 == 0 && (unsigned long long)a.tokens * (a.hq + 2 * a.hk) < 1ull << 32 && ok(a.q) && ok(a.k) && ok(a.v) && ok(a.qo) && ok(a.ko) && ptr(a.kp) && ptr(a.vp) &&
-           (!a.kp || (a.pg.ps % unit == 0 && a.pg.ts % unit == 0 && a.pg.hs % unit == 0)) && ptr(a.wq) && ptr(a.wk) && ptr(a.cs) && (uintptr_t)a.axis % 8 == 0;
+    const int bytes = std::min(16, n * (int)sizeof(T));
+    const long long unit = bytes / (int)sizeof(T);
+    auto ok = [&](const HeadsOf<T> &h) { return !h.p || ((uintptr_t)h.p % bytes == 0 && h.ts % unit == 0 && h.hs % unit == 0); };
+    auto ptr = [](const void *p, int b) { return (uintptr_t)p % b == 0; };
+    return a.d % (2 * n) == 0 && a.rot % (2 * n) == 0 && (unsigned long long)a.tokens * (a.hq + 2 * a.hk) < 1ull << 32 && ok(a.q) &&
+           ok(a.k) && ok(a.v) && ok(a.qo) && ok(a.ko) && ptr(a.kp, bytes) && ptr(a.vp, bytes) &&
+           (!a.kp || (a.pg.ps % unit == 0 && a.pg.ts % unit == 0 && a.pg.hs % unit == 0)) && ptr(a.wq, 16) && ptr(a.wk, 16) && ptr(a.cs, 16) &&
+           ptr(a.axis, n);
 }
 
-template <typename T, int LPR, int HPT>
+template <typename T, int LPR, int HPT, int N = 8>
 static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
 {
     RopeVec g;
@@ -374,8 +415,8 @@ static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
     g.slots32 = (unsigned long long)a.pg.pages * a.pg.size <= 0xffffffffull;
     g.inv_d = 1.0f / (float)a.d;
     const unsigned grid = (unsigned)(((unsigned long long)g.end * LPR + kRopeThreads - 1) / kRopeThreads);
-    auto *fn = a.axis ? (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, true> : rope_vec_kernel<T, LPR, HPT, false, true>)
-                      : (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, false> : rope_vec_kernel<T, LPR, HPT, false, false>);
+    auto *fn = a.axis ? (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, true, N> : rope_vec_kernel<T, LPR, HPT, false, true, N>)
+                      : (a.interleaved ? rope_vec_kernel<T, LPR, HPT, true, false, N> : rope_vec_kernel<T, LPR, HPT, false, false, N>);
     return launch_behind(fn, grid, kRopeThreads, 0, s, a, g);
 }
 
@@ -393,10 +434,15 @@ static cudaError_t rope_vec_launch(const RopeArgs<T> &a, cudaStream_t s)
 template <typename T>
 static cudaError_t rope_launch(const RopeArgs<T> &a, cudaStream_t s)
 {
-    if (rope_vec_ok(a)) {
+    if (rope_vec_ok(a, 8)) {
         if (a.d <= 64) return rope_vec_launch<T, 4>(a, s);
         if (a.d <= 128) return rope_vec_launch<T, 8>(a, s);
         return rope_vec_launch<T, 32>(a, s);
+    }
+    if constexpr (sizeof(T) == 2) {
+        // heads or rotations in multiples of 8 only, or rows aligned to 8 bytes: pieces of 4
+        // (2345 tokens of 32 + 8 heads of 80, 40 rotated, filed: 18 us; a warp a head: 51)
+        if (a.d <= 128 && rope_vec_ok(a, 4)) return a.d <= 64 ? rope_vec_launch<T, 8, 2, 4>(a, s) : rope_vec_launch<T, 16, 2, 4>(a, s);
     }
     const long long units = (long long)a.tokens * (a.hq + a.hk + (a.vp ? a.hk : 0));
     return launch_behind(a.axis ? rope_row_kernel<T, true> : rope_row_kernel<T, false>, (unsigned)((units + 3) / 4), 128, 0, s, a);

@@ -59,6 +59,33 @@ def test_axes(cuda_ok, dt, tokens, hq, hk, d, rot, axes, kind, interleaved):
     _seq.check_norm_rope(ko, *_seq.norm_rope(k, wk, at, own, rot, interleaved, 1e-5))
 
 
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("d, rot, off", [(80, 40, 0), (24, 8, 0), (72, 40, 0), (120, 56, 0), (8, 8, 0), (128, 24, 0), (64, 64, 4), (80, 40, 4), (80, 40, 2)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("kind", [None, "sorted", "turns"])
+def test_pieces_of_four(cuda_ok, dt, d, rot, off, interleaved, kind):
+    """Heads and rotations in multiples of 8, rows aligned to 8 bytes and less;
+    with one position a token too, filed."""
+    t, hq, hk, size, n = 37, 6, 3, 8, 6
+    raw = _rand((t * (hq + 2 * hk) * d + off,), dt, 5, 2.0)
+    x = raw[off:].view(t, hq + 2 * hk, d)
+    q, k, v = x[:, :hq], x[:, hq:hq + hk], x[:, hq + hk:]
+    wq, wk, table = _rand((d,), F32, 3), _rand((d,), F32, 4), _table(50, rot)
+    axis = _axes(rot // 2, 3, kind or "even")
+    pos = torch.randint(0, 50, (t, 3), device="cuda", dtype=torch.int32)
+    if kind is None:
+        pos[:, 1], pos[:, 2] = pos[:, 0], pos[:, 0]
+    own, at = _own_table(table, pos, axis)
+    pages = torch.zeros(2, n, size, hk, d, dtype=dt, device="cuda")
+    slots = torch.randperm(n * size, device="cuda")[:t]
+    qo, ko = attention.qk_norm_rope(q, k, pos[:, 0].contiguous() if kind is None else pos, table, pair_axis=axis if kind else None,
+                                    q_weight=wq, k_weight=wk, interleaved=interleaved, v=v, k_pages=pages[0], v_pages=pages[1],
+                                    slots=slots)
+    _seq.check_norm_rope(qo, *_seq.norm_rope(q, wq, at, own, rot, interleaved, 1e-6))
+    _seq.check_norm_rope(ko, *_seq.norm_rope(k, wk, at, own, rot, interleaved, 1e-6))
+    assert torch.equal(pages[0, slots // size, slots % size], ko) and torch.equal(pages[1, slots // size, slots % size], v)
+
+
 @pytest.mark.parametrize("dt", [F16, F32])
 @pytest.mark.parametrize("off", [0, 1])
 def test_one_axis_is_the_plain_call(cuda_ok, dt, off):

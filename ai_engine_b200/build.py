@@ -1,8 +1,10 @@
 """In-tree build of the CUDA library ``ai_engine_b200/libaie_conv.so``.
 
-Two translation units, compiled for sm_100a only and side by side: the conv
-path (``csrc/aie_conv.cu``, which includes the ``k_*.cuh`` kernels) and the
-sequence operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels).  Beside
+Translation units, compiled for sm_100a only and side by side: the conv path
+(``csrc/aie_conv.cu``, which includes the ``k_*.cuh`` kernels), the sequence
+operators (``csrc/aie_seq.cu``, the ``seq_*.cuh`` kernels) and, for the time they
+take, the one-token kernels over states and the 4-bit cache
+(``csrc/aie_read*.cu``).  Beside
 it ``_seqcall.so``, the sequence operators' binding on torch tensors
 (``csrc/seq_bind.cpp``), which is linked against it; where torch or Python's
 headers are missing it is left out, with a message (the C ABI needs neither).
@@ -25,7 +27,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libaie_conv.so")
-UNITS = ("aie_conv", "aie_seq")
+UNITS = ("aie_conv", "aie_seq", "aie_read16", "aie_read4_f16", "aie_read4_bf16")
 OBJ = os.path.join(HERE, "_build")
 BIND = os.path.join(HERE, "_seqcall.so")
 BIND_SRC = os.path.join(CSRC, "seq_bind.cpp")

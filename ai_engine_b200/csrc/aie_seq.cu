@@ -550,7 +550,7 @@ static int cross_read(const aie_cross &p, cudaStream_t s)
     a.cu = p.cu_k; a.keys = (int)p.keys;
     a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
     a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
-    return launched(a.bf16 ? read16_launch<__nv_bfloat16>(a, w.nt, s) : read16_launch<__half>(a, w.nt, s), "cross attention");
+    return launched(read16_run(a, w.nt, s), "cross attention");
 }
 
 template <typename T>
@@ -656,17 +656,7 @@ static int kv4_step(const aie_kv4_step &p, cudaStream_t s)
     a.table = p.table; a.lens = p.lens; a.max_len = (int)p.max_len; a.table_stride = (int)p.table_stride;
     a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.cache.kv_heads); a.d = a.g.d;
     a.bf16 = p.dtype == AIE_DT_BF16; a.scale = p.scale;
-    cudaError_t e;
-    switch (a.d / 32) {
-    case 1: e = read4_launch<1>(a, w.nt, s); break;
-    case 2: e = read4_launch<2>(a, w.nt, s); break;
-    case 3: e = read4_launch<3>(a, w.nt, s); break;
-    case 4: e = read4_launch<4>(a, w.nt, s); break;
-    case 5: e = read4_launch<5>(a, w.nt, s); break;
-    case 6: e = read4_launch<6>(a, w.nt, s); break;
-    case 7: e = read4_launch<7>(a, w.nt, s); break;
-    default: e = read4_launch<8>(a, w.nt, s); break;
-    }
+    const cudaError_t e = a.bf16 ? read4_run_bf16(a, w.nt, s) : read4_run_f16(a, w.nt, s);
     return launched(e, "attention over 4 bits");
 }
 

@@ -55,11 +55,11 @@ __device__ __forceinline__ Vec8<T> read8(const T *p, int vec)
 
 // Next to a border between two codes, where f32 may be on the wrong side, and
 // wherever codes have to be kept within 0 .. 15.
-__device__ __noinline__ uint32_t kv4_code64(float x, float lo, float s)
+static __device__ __noinline__ uint32_t kv4_code64(float x, float lo, float s)
 {
     return s > 0.f ? (uint32_t)fmin(fmax(rint(((double)x - (double)lo) / (double)s), 0.0), 15.0) : 0u;
 }
-__device__ __noinline__ float kv4_scale64(float hi, float lo) { return (float)fmax(((double)hi - (double)lo) / 15.0, 0.0); }
+static __device__ __noinline__ float kv4_scale64(float hi, float lo) { return (float)fmax(((double)hi - (double)lo) / 15.0, 0.0); }
 
 __device__ __forceinline__ __half lower(__half2 x) { return __low2half(x); }
 __device__ __forceinline__ __half upper(__half2 x) { return __high2half(x); }

@@ -196,12 +196,11 @@ struct ReadTile {
 };
 
 // Four neighbouring elements of a result.
+template <typename T>
 __device__ __forceinline__ void read_store4(const ReadArgs &a, long long at, const float (&x)[4])
 {
     unsigned short *out = (unsigned short *)a.out + at;
-    uint2 y;
-    if (a.bf16) y = make_uint2(pack2<__nv_bfloat16>(x[0], x[1]), pack2<__nv_bfloat16>(x[2], x[3]));
-    else y = make_uint2(pack2<__half>(x[0], x[1]), pack2<__half>(x[2], x[3]));
+    const uint2 y = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
     if (a.o_vec >= 8) *(uint2 *)out = y;
     else {
         out[0] = (unsigned short)y.x; out[1] = (unsigned short)(y.x >> 16);
@@ -212,11 +211,13 @@ __device__ __forceinline__ void read_store4(const ReadArgs &a, long long at, con
 // Blocks of an SM.
 constexpr int read_blocks(bool kv4, int dc, int nt) { return nt == 1 && dc <= 4 ? 3 : 2; }
 
-// T: the operands' type, f16 in 4 bits.
+// T: the type of queries and results; that of the products is f16 in 4 bits.
 template <typename T, bool KV4, int DC, int NT, int STAGES>
 __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_kernel(const ReadArgs a)
 {
     using Tile = ReadTile<KV4, DC>;
+    using M = std::conditional_t<KV4, __half, T>;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     // Binary orders by which weights are held larger.  In 4 bits they are also
     // multiplied with the groups' scales, below 2^(se + 3): 4 - se, so that 2^8 times
     // both is what f16 holds, and se moves up only when a scale is too large.  (Values
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const uint32_t x = raw[nt][g * 4 + e];
-                            const float2 y = a.bf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u))
+                            const float2 y = kBf16 ? make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u))
                                                     : __half22float2(*(const __half2 *)&x);
                             f[g][2 * e] = y.x * sign;
                             f[g][2 * e + 1] = y.y * sign;
@@ -548,7 +549,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        mma16816_first<T>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
+                        mma16816_first<M>(s[mt][nt], low, qs[nt][0], qs[nt][1]);
 #pragma unroll
                         for (int j = 0; j < 4; j++) s[mt][nt][j] *= 0x1p-24f;
                     }
@@ -563,8 +564,8 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             float acc[4];
-                            mma16816_first<T>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
-                            mma16816<T>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
+                            mma16816_first<M>(acc, {x0.p[0], x1.p[0], x0.p[1], x1.p[1]}, qb[nt][2 * g][0], qb[nt][2 * g][1]);
+                            mma16816<M>(acc, {x0.p[2], x1.p[2], x0.p[3], x1.p[3]}, qb[nt][2 * g + 1][0], qb[nt][2 * g + 1][1]);
 #pragma unroll
                             for (int j = 0; j < 2; j++) {
                                 s[mt][nt][j] = fmaf(f0, acc[j], s[mt][nt][j]);
@@ -579,8 +580,8 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         ldmatrix4(kt + (mt * 16 + (lane & 15)) * Tile::kRow + (2 * k + (lane >> 4)) * 16, w);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            if (k) mma16816<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
-                            else mma16816_first<T>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                            if (k) mma16816<M>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
+                            else mma16816_first<M>(s[mt][nt], w, qb[nt][k][0], qb[nt][k][1]);
                         }
                     }
                 }
@@ -618,7 +619,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
                         if (x != -INFINITY) {
                             m[nt][j] = x;
-                            off[nt][j] = fmaf(-x, slq[nt][j], KV4 ? (float)(4 - se) : kWeightShift<T>);
+                            off[nt][j] = fmaf(-x, slq[nt][j], KV4 ? (float)(4 - se) : kWeightShift<M>);
                             // as in attn_tc_kernel: steps of up to 8 binary orders leave m
                             most_s[nt][j] = x + __fdividef(8.f, slq[nt][j]);
                         }
@@ -641,8 +642,8 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     for (int j = 0; j < 4; j++) e[j] = ex2(fmaf(s[mt][nt][j], slq[nt][j & 1], off[nt][j & 1]));
                     l[nt][0] += e[0] + e[2];
                     l[nt][1] += e[1] + e[3];
-                    pb[nt][mt][0] = transpose8x8(pack2<T>(e[0], e[1]));
-                    pb[nt][mt][1] = transpose8x8(pack2<T>(e[2], e[3]));
+                    pb[nt][mt][0] = transpose8x8(pack2<M>(e[0], e[1]));
+                    pb[nt][mt][1] = transpose8x8(pack2<M>(e[2], e[3]));
                 }
             // ---- values
 #pragma unroll
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         low[2] = __byte_perm(pv[8 * DC + r], pv[9 * DC + r], 0x7632);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma16816<T>(o_lo[nt], low, pb[nt][mt][0], pb[nt][mt][1]);
+                    for (int nt = 0; nt < NT; nt++) mma16816<M>(o_lo[nt], low, pb[nt][mt][0], pb[nt][mt][1]);
                     uint32_t w[4];
 #pragma unroll
                     for (int g = 0; g < DC; g++) {
@@ -674,12 +675,15 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
                             const uint32_t b0 = mul2(pb[nt][mt][0], s0), b1 = mul2(pb[nt][mt][1], s1);
-                            mma16816<T>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
-                            mma16816<T>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
+                            mma16816<M>(o[2 * g][nt], {x0.p[0], x0.p[1], x1.p[0], x1.p[1]}, b0, b1);
+                            mma16816<M>(o[2 * g + 1][nt], {x0.p[2], x0.p[3], x1.p[2], x1.p[3]}, b0, b1);
                             // what p s lost in f16 (exactly f16 again), times the middle code, to the lo of
-                            // row g: else lo + code s, which cancel, would not lose the same
-                            const uint32_t middle = r == g ? 0x47804780u : 0u;
-                            mma16816<T>(o_lo[nt], {middle, 0u, middle, 0u}, lost2(pb[nt][mt][0], s0, b0), lost2(pb[nt][mt][1], s1, b1));
+                            // row g: else lo + code s, which cancel, would not lose the same (f16 results
+                            // 1.7 times as far off as a 16-bit cache's; 1.3 with it).  bf16 cannot tell.
+                            if constexpr (!kBf16) {
+                                const uint32_t middle = r == g ? 0x47804780u : 0u;
+                                mma16816<M>(o_lo[nt], {middle, 0u, middle, 0u}, lost2(pb[nt][mt][0], s0, b0), lost2(pb[nt][mt][1], s1, b1));
+                            }
                         }
                     }
                 } else {
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         uint32_t w[4];
                         ldmatrix4_t(vt + (mt * 16 + (lane & 7) + (lane >> 4) * 8) * Tile::kRow + (2 * t + (lane >> 3 & 1)) * 16, w);
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma16816<T>(o[t][nt], w, pb[nt][mt][0], pb[nt][mt][1]);
+                        for (int nt = 0; nt < NT; nt++) mma16816<M>(o[t][nt], w, pb[nt][mt][0], pb[nt][mt][1]);
                     }
                 }
             }
@@ -734,7 +738,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                             }
                             const int d = g * 32 + r * 4;
                             if (!whole) *(float4 *)(a.part_o + pat + d) = make_float4(x[0], x[1], x[2], x[3]);
-                            else read_store4(a, oat + d, x);
+                            else read_store4<T>(a, oat + d, x);
                         }
                     } else {
 #pragma unroll
@@ -745,8 +749,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                                 if (d >= a.d) continue;
                                 const float x = o[t][nt][2 * e + j] * f;
                                 if (!whole) a.part_o[pat + d] = x;
-                                else if (a.bf16) ((__nv_bfloat16 *)a.out)[oat + d] = __float2bfloat16_rn(x);
-                                else ((__half *)a.out)[oat + d] = __float2half_rn(x);
+                                else ((T *)a.out)[oat + d] = from_f32<T>(x);
                             }
                     }
                 }
@@ -905,6 +908,11 @@ static ReadPlan read_plan(bool kv4, uint32_t seqs, uint64_t most, uint32_t kv_he
     return w;
 }
 
+// The kernels' launches, each compiled apart (aie_read16.cu, aie_read4_f16.cu, aie_read4_bf16.cu).
+cudaError_t read16_run(const ReadArgs &a, int nt, cudaStream_t s);
+cudaError_t read4_run_f16(const ReadArgs &a, int nt, cudaStream_t s);
+cudaError_t read4_run_bf16(const ReadArgs &a, int nt, cudaStream_t s);
+
 template <typename T, bool KV4, int DC, int NT>
 static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
 {
@@ -945,12 +953,19 @@ static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const 
     a.part_o = (float *)(ws + w.o_at);
 }
 
-template <int DC>
+template <typename T>
 static cudaError_t read4_launch(const ReadArgs &a, int nt, cudaStream_t s)
 {
-    if constexpr (DC <= 4)
-        if (nt == 2) return read_launch<__half, true, DC, 2>(a, s);
-    return read_launch<__half, true, DC, 1>(a, s);
+    switch (a.d / 32) {
+    case 1: return nt == 2 ? read_launch<T, true, 1, 2>(a, s) : read_launch<T, true, 1, 1>(a, s);
+    case 2: return nt == 2 ? read_launch<T, true, 2, 2>(a, s) : read_launch<T, true, 2, 1>(a, s);
+    case 3: return nt == 2 ? read_launch<T, true, 3, 2>(a, s) : read_launch<T, true, 3, 1>(a, s);
+    case 4: return nt == 2 ? read_launch<T, true, 4, 2>(a, s) : read_launch<T, true, 4, 1>(a, s);
+    case 5: return read_launch<T, true, 5, 1>(a, s);
+    case 6: return read_launch<T, true, 6, 1>(a, s);
+    case 7: return read_launch<T, true, 7, 1>(a, s);
+    default: return read_launch<T, true, 8, 1>(a, s);
+    }
 }
 
 template <typename T>

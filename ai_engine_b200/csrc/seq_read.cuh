@@ -18,14 +18,35 @@
 // tiles end up in several warps, each leaves a partial result (O / l and log2 of
 // the weights' sum), and a second launch joins them:
 //   out = sum 2^(lse_i - lse) O_i.
-// Partial result number `warp + sequence` is its own for every pair that meet,
-// since both only grow along the list.  Fixed order throughout: results repeat
-// bit for bit.
+// Partial result number `warp + (head, sequence)` is its own for every pair that
+// meet, since both only grow along the list.  Fixed order throughout: results
+// repeat bit for bit.
 //
 // Rounding to fewer bits: the weights to 16 bits for the product with V (l sums
 // them unrounded; f16 weights 2^7 times as large, as in attn_tc_kernel), the
 // result, and over the 4-bit cache the weights times the scales to f16 for the
-// product with the codes.
+// product with the codes.  What that last rounding loses is put back, times the
+// middle code, where results are f16 (1.75 times a 32-bit computation's error
+// without, 1.3 with); a bf16 result's own rounding is 8 times as large, and the
+// kernel takes 153 us with it for 140 without in the second case below.
+//
+// Over the 4-bit cache the work is on the codes: 32 elements of a place and head
+// are 20 bytes, which come in 0.9 cycles of an SM at the memory's rate; one
+// instruction a pair of codes takes the logic pipe 0.25 of them.  So codes are not
+// made into numbers at all: masked in place they are subnormal f16 (n 2^-24; the
+// odd ones 16 times as large), which the products multiply exactly and at full
+// rate; scales go into the weights, lowest values into a product of their own.
+//
+// Measured (states larger than L2): 96 streams of up to 2855 states of 8 heads of
+// 128, bf16: 109 us a call, 561 MB at 5.1 TB/s; its issue slots are used 26%.  4
+// bits, 64 streams of up to 16384 places of 8 heads of 128, 4 query heads each:
+// 138 us a call (666 MB at 4.8 TB/s) in runs of some milliseconds, 157 in long
+// ones, where the power limit takes the clock from 1.95 to 1.72 GHz; issue slots
+// 52%, logic pipe about 50%; 5.6 TB/s once all warps run, after 9 us to a
+// warp's first tile, and blocks of an SM end unevenly (with the f16 results'
+// correction between 102 and 153 us).  Parts taken from a counter end together but
+// cost 165-178 us (each part begins with its own queries); 4 blocks an SM of 128
+// registers 146-148; 16 places a tile 154.
 #pragma once
 #include "seq_kv4.cuh"
 #include "seq_step.cuh"
@@ -49,6 +70,7 @@ struct ReadArgs {
     const int32_t *table, *lens;
     int max_len, table_stride;
     int seqs, hq, group, d;
+    unsigned most;           // tiles of all sequences, at most
     int zs, heads;           // blocks of a group's query heads; key heads times those
     int rows;                // query heads of a block that are kept
     int bf16;
@@ -232,26 +254,29 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 
     // ---- tiles before each thread's sequences, and in all
     const int per = (a.seqs + kRdThreads - 1) / kRdThreads, s_from = tid * per, s_to = min(s_from + per, a.seqs);
+    // (sums stop at 2^31 - 1 instead of wrapping: a cu that decreases can have any number)
+    auto sum = [](unsigned x, unsigned y) { return min(x + y, 0x7fffffffu); };
     unsigned mine = 0;
-    for (int s = s_from; s < s_to; s++) mine += (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys;
+    for (int s = s_from; s < s_to; s++) mine = sum(mine, (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys);
     unsigned upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += y;
+        if (lane >= o) upto = sum(upto, y);
     }
     if (lane == 31) warp_sums[warp] = upto;
     __syncthreads();
     unsigned tiles = 0, base = upto - mine;
 #pragma unroll
     for (int i = 0; i < kRdWarps; i++) {
-        if (i < warp) base += warp_sums[i];
-        tiles += warp_sums[i];
+        if (i < warp) base = sum(base, warp_sums[i]);
+        tiles = sum(tiles, warp_sums[i]);
     }
+    if (tiles > a.most) tiles = 0;  // no list of starts: zeros
     scan[tid] = base;
     if (blockIdx.x == 0) {  // for the joining launch
         for (int s = s_from; s < s_to; s++) {
-            a.before[s] = base;
+            a.before[s] = tiles ? base : 0u;
             base += (read_len(a, s) + Tile::kKeys - 1) / Tile::kKeys;
         }
         if (tid == 0) a.before[a.seqs] = tiles;
@@ -884,7 +909,7 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
 // the workspace.
 struct ReadPlan {
     int nt, zs, heads, rows, workers;
-    uint64_t tiles, lse_at, o_at, bytes;  // tiles: at most
+    uint64_t tiles, lse_at, o_at, bytes;  // tiles: of all key heads, at most
 };
 
 // DC as the kernels are instantiated for it
@@ -940,6 +965,7 @@ static void read_args(ReadArgs &a, const ReadPlan &w, const aie_heads &q, const 
 {
     a.q = q.data; a.q_ts = q.token_stride; a.q_hs = q.head_stride;
     a.out = out.data; a.o_ts = out.token_stride; a.o_hs = out.head_stride;
+    a.most = (unsigned)(w.tiles / w.heads);
     a.zs = w.zs; a.heads = w.heads; a.rows = w.rows; a.workers = w.workers;
     a.parts_each = (unsigned)(std::min<uint64_t>(w.workers, w.tiles) / ((uint64_t)w.heads * a.seqs)) + 1;
     char *ws = (char *)(((uintptr_t)workspace + 31) / 32 * 32);

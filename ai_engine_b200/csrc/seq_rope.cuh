@@ -212,8 +212,9 @@ __device__ __forceinline__ void load_floats(const float *p, float *f)
 
 // Heads in whole 16-element pieces, everything 16-byte aligned: LPR lanes per
 // head (a power of two, at least d / 2 N), each with two pieces of N = 8 elements
-// (4 for heads that allow no more) that the rotation pairs with each other, so that it needs no exchange: with
-// halves, elements i and i + rot / 2; interleaved or not rotated, neighbours.
+// (4 for heads that allow no more) that the rotation pairs with each other, so
+// that it needs no exchange: with halves, elements i and i + rot / 2; interleaved
+// or not rotated, neighbours.
 // A lane keeps its pieces' weights and its token's angles in registers for
 // HPT heads of the token, whose loads are all in flight at once.
 //
@@ -223,6 +224,12 @@ __device__ __forceinline__ void load_floats(const float *p, float *f)
 // threads 99.  At 5 blocks the four-heads form spills 20 to 36 bytes a thread in
 // 16 bits.  In f32, where the heads alone take 64 registers, it spills 108 to
 // 164: the same tokens take 187 us, 881 MB at 4.7 TB/s.
+//
+// By several axes (AXES) a pair's angle is that of its token's position on the
+// pair's axis.  A lane whose pairs all have one axis reads its angles as before,
+// from that axis' row; others read theirs one by one (1297 tokens of 20 + 5 heads
+// of 96, axes taking turns: 6.7 us a call).  16350 tokens of 32 + 8 heads of 128,
+// three axes, filed: 86 us, 5.2 TB/s.
 constexpr int kRopeThreads = 128, kRopeBlocks = 5;
 struct RopeVec {
     unsigned q_units, k_units;  // groups of HPT heads of a token

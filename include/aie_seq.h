@@ -104,7 +104,8 @@ AIE_API int aie_prompt_attn(const aie_prompt *p, void *stream);
  * sequence s: tokens cu_q[s] .. cu_q[s + 1] of q see states cu_k[s] .. cu_k[s + 1]
  * of k and v.  cu_q NULL: token s is sequence s's one token (tokens == seqs).
  * Both lists (device, [seqs + 1], not decreasing, within 0 .. tokens and 0 ..
- * keys) are read on the device.  A sequence without states gives zeros; tokens
+ * keys) are read on the device; with others nothing is read out of range, and
+ * the results are unspecified.  A sequence without states gives zeros; tokens
  * of no sequence are left unwritten.  Values of other sequences, infinities and
  * NaN among them, never reach a result.  out overlaps no input.
  * workspace: aie_cross_attn_workspace(p) bytes (p as in the call, apart from

@@ -169,3 +169,20 @@ def test_refusals(cuda_ok):
     ]:
         with pytest.raises(error):
             attention.cross_attention(*args, **kw)
+
+
+@pytest.mark.parametrize("dt, d", [(F16, 64), (BF16, 128), (F32, 64)])
+@pytest.mark.parametrize("each", [False, True])
+def test_lists_that_are_no_starts(cuda_ok, dt, d, each):
+    """Starts that decrease or lie outside: results are unspecified, but nothing
+    outside out is written, and the next call is as ever."""
+    bad = torch.tensor([0, 160, 0, 160, -7, 1 << 30, 0, 160, 90], dtype=torch.int32, device="cuda")
+    q, k, v = _inputs([1] * 8 if each else [160], [160], 8, 2, d, dt)
+    around = torch.full((q.shape[0] + 8, 8, d), 7.0, dtype=dt, device="cuda")
+    cu_q = None if each else bad
+    attention.cross_attention(q, k, v, bad, cu_q=cu_q, out=around[4:-4])
+    assert bool((around[:4] == 7.0).all()) and bool((around[-4:] == 7.0).all())
+    k_lens = [20] * 8
+    cu, t = _read.starts(k_lens), q.shape[0] // 8
+    got = attention.cross_attention(q, k, v, cu, cu_q=None if each else _read.starts([t] * 8))
+    _seq.check(got, *_read.cross(q, k, v, [t] * 8, k_lens))

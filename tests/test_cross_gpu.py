@@ -186,3 +186,18 @@ def test_lists_that_are_no_starts(cuda_ok, dt, d, each):
     cu, t = _read.starts(k_lens), q.shape[0] // 8
     got = attention.cross_attention(q, k, v, cu, cu_q=None if each else _read.starts([t] * 8))
     _seq.check(got, *_read.cross(q, k, v, [t] * 8, k_lens))
+
+
+@pytest.mark.parametrize("q_lens", [[1, 1], [40, 3], None])
+def test_states_beyond_32_bits(cuda_ok, q_lens):
+    """States more than 2^31 elements into k and v, and the same ones alone."""
+    n, k_lens = 2_200_000, [1000, 77]
+    kv = torch.zeros(n, 2, 8, 128, dtype=BF16, device="cuda")
+    few = _rand((sum(k_lens), 2, 8, 128), BF16, 1)
+    kv[-few.shape[0] - 1:-1] = few
+    cu = _read.starts(k_lens)
+    far = cu + (n - few.shape[0] - 1)
+    q = _rand((sum(q_lens or [1, 1]), 32, 128), BF16, 2)
+    cu_q = None if q_lens is None else _read.starts(q_lens)
+    assert torch.equal(attention.cross_attention(q, kv[:, 0], kv[:, 1], far, cu_q=cu_q),
+                       attention.cross_attention(q, few[:, 0], few[:, 1], cu, cu_q=cu_q))

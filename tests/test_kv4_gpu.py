@@ -290,3 +290,23 @@ def test_refusals(cuda_ok):
         pages.new_cache4(1, 4, 12, 2, 64)
     with pytest.raises(ValueError):
         pages.new_cache4(1, 4, 16, 2, 80)
+
+
+def test_offsets_beyond_32_bits(cuda_ok):
+    """The same pages far into a cache of 4.5 GB a half: filed, read and attended to as near its start."""
+    lens, size, hk, d = [700, 64, 1], 64, 8, 128
+    kp, vp, table = _cache(lens, hk, d, size)
+    n = kp.shape[0]
+    kv = pages.new_cache4(1, 110000, size, hk, d)
+    far = 110000 - 1 - 3571 * torch.arange(n, device="cuda")  # on both sides of 2^31 and of 2^32 bytes
+    assert int(far.min()) * kv.stride(2) > 2 ** 31 and int(far.max()) * kv.stride(2) > 2 ** 32
+    kv[0, 0][far], kv[0, 1][far] = kp, vp
+    moved = torch.where(table >= 0, far[table.long().clamp(min=0)].int(), table)
+    q, cu = _rand((3, 32, d), BF16, 9), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    assert torch.equal(attention.kv4_attention(q, kv[0, 0], kv[0, 1], moved, cu), attention.kv4_attention(q, kp, vp, table, cu))
+    near = torch.arange(n * size, device="cuda")
+    slots = far[near // size] * size + near % size
+    k, v = _rand((n * size, hk, d), F16, 3), _rand((n * size, hk, d), F16, 4)
+    attention.kv4_file(k, v, kv[0, 0], kv[0, 1], slots)
+    for got, x in zip(attention.kv4_load(kv[0, 0], kv[0, 1], slots, dtype=F32), (k, v)):
+        _same(got, x)

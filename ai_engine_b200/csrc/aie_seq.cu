@@ -553,6 +553,12 @@ static int cross_read(const aie_cross &p, cudaStream_t s)
     return launched(read16_run(a, w.nt, s), "cross attention");
 }
 
+// Rows a sequence from which tiles are worth it with heads of more than 128, where
+// few blocks fit an SM (64 sequences over 2000 states, 8 heads of 256: a warp per row
+// 2.1, 2.9 and 4.5 ms with 1, 2 and 4 rows, tiles 3.3); others always are (8 heads
+// of 128, 1 row: 1.65 ms and 1.33; one sequence over 20000: 16.4 and 4.5).
+constexpr int kTileLeast = 3;
+
 template <typename T>
 static int cross_rows(const aie_cross &p, cudaStream_t s)
 {
@@ -563,6 +569,15 @@ static int cross_rows(const aie_cross &p, cudaStream_t s)
     a.hq = (int)p.q_heads; a.group = (int)(p.q_heads / p.kv_heads); a.d = (int)p.head_dim;
     a.scale = p.scale;
     const long long rows = (long long)p.tokens * p.q_heads;
+    // tiles of rows, no more than whole ones and one that is not per sequence
+    const uint64_t units = ((uint64_t)p.tokens * a.group / kTileRows + std::min(p.seqs, p.tokens)) * p.kv_heads;
+    if ((p.head_dim <= 128 || (uint64_t)p.tokens * a.group >= (uint64_t)kTileLeast * p.seqs) && units <= 0x7fffffffull) {
+        auto *fn = a.d <= 64 ? &cross_tile_kernel<T, 1> : a.d <= 128 ? &cross_tile_kernel<T, 2> : &cross_tile_kernel<T, 4>;
+        const uint32_t smem = cross_tile_smem(a.d);
+        cudaError_t e = ensure_smem_attr((const void *)fn, cross_tile_smem(a.d <= 64 ? 64 : a.d <= 128 ? 128 : 256));
+        if (e == cudaSuccess) e = launch_behind(fn, (unsigned)units, kTileThreads, smem, s, a, (int)p.kv_heads);
+        return launched(e, "cross attention");
+    }
     return launched(launch_behind(cross_rows_kernel<T>, (unsigned)((rows + 3) / 4), 128, 0, s, a), "cross attention");
 }
 

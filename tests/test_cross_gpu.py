@@ -201,3 +201,17 @@ def test_states_beyond_32_bits(cuda_ok, q_lens):
     cu_q = None if q_lens is None else _read.starts(q_lens)
     assert torch.equal(attention.cross_attention(q, kv[:, 0], kv[:, 1], far, cu_q=cu_q),
                        attention.cross_attention(q, few[:, 0], few[:, 1], cu, cu_q=cu_q))
+
+
+@pytest.mark.parametrize("rows", [1, 5, 70])
+@pytest.mark.parametrize("dt, d", [(F32, 64), (F32, 100), (BF16, 256)])
+def test_scores_of_minus_infinity_in_f32(cuda_ok, rows, dt, d):
+    """The same where the tensor cores take no part, with a last tile that is not whole."""
+    n = 333
+    q = torch.ones(rows, 4, d, device="cuda", dtype=dt)
+    k, v = _rand((n, 2, d), dt, 2, 0.1), _rand((n, 2, d), dt, 3)
+    k[:100] = k[200:250] = -float("inf")
+    seen = torch.cat([torch.arange(100, 200), torch.arange(250, n)]).cuda()
+    for cu_q in (_read.starts([rows]),) if rows > 1 else (None, _read.starts([1])):
+        got = attention.cross_attention(q, k, v, _read.starts([n]), cu_q=cu_q)
+        _seq.check(got, *_read.cross(q, k[seen], v[seen], [rows], [len(seen)]))

@@ -530,6 +530,11 @@ int pack_kv(PyObject *o, aie_pages &p)
     if ((!bytes && dtype_id(kv) < 0) || !kv.is_cuda() || kv.dim() != 6 || kv.size(1) != 2 || !kv.is_contiguous())
         refuse(PyExc_TypeError, "kv must be a contiguous float16, bfloat16 or float32 CUDA tensor "
                                "[layers, 2, pages, page_size, kv_heads, head_dim], or a uint8 one of pages.new_cache4");
+    // what aie_kv4 takes: heads of a multiple of 32 up to 256 elements, pages of a multiple of 8
+    // places.  Bytes in another order would go by the wrong page size.
+    if (bytes && (kv.size(5) == 0 || kv.size(5) % 20 || kv.size(5) > 160 || kv.size(4) == 0 || kv.size(4) % 8))
+        refuse(PyExc_TypeError, "kv's pages of [%lld, %lld, %lld] bytes are not pages.new_cache4's: [kv_heads, page_size (a multiple "
+                               "of 8), head_dim * 5 / 8]", (long long)kv.size(3), (long long)kv.size(4), (long long)kv.size(5));
     p.kv = kv.data_ptr();
     p.layers = u32(kv.size(0), "layers");
     p.pages = u32(kv.size(2), "pages");

@@ -129,10 +129,12 @@ def grid(frames: int, height: int, width: int, device="cuda") -> torch.Tensor:
 class FrameDecoder:
     """Layers of x += attention(x) wo over a 4-bit cache, then x += attention of
     x to the frames' states.  A stream a row, all of them in every call; heads of
-    a multiple of 32."""
+    a multiple of 32, float16 or bfloat16 (what the 4-bit attention takes)."""
 
     def __init__(self, layers: int, dim: int, q_heads: int, kv_heads: int, head_dim: int, *, streams: int, pages_: int,
                  page_size: int = 16, max_len: int = 4096, dtype=torch.bfloat16, device="cuda", seed: int = 0):
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"{dtype}: float16 or bfloat16")
         self.dim, self.hq, self.hk, self.d, self.streams = dim, q_heads, kv_heads, head_dim, streams
         width = -(-max_len // page_size)
         self.page_size, self.max_len, self.dtype, self.device = page_size, width * page_size, dtype, torch.device(device)

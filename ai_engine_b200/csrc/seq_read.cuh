@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     const float sl = fabsf(a.scale) * 1.4426950408889634f, sign = a.scale < 0.f ? -1.f : a.scale > 0.f ? 1.f : 0.f;
     uint32_t qb[NT][KV4 ? 2 * DC : DC][2], qs[NT][2];  // queries; 4 bits: each group's sum of them, in two f16
     float slq[NT][2];                                  // scale of a column's scores, in binary orders
-    float off[NT][2], most_s[NT][2];                   // weights are 2^(slq s + off); scores above that move m
+    float ref[NT][2], most_s[NT][2];                   // weights are 2^(slq (s - ref) + shift), ref = m; scores above most_s move m
     float o[OT][NT][4], m[NT][2], l[NT][2];
     float o_lo[KV4 ? NT : 1][4];  // 4 bits: the weighted sums of the groups' lo
     int se = kLeastScale;         // their scales are below 2^(se + 3)
@@ -490,8 +490,11 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     }
                     if (DC <= 4) qs[nt][1] = 0u;
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        slq[nt][j] = fmaxf(sl * 0x1p24f * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f);
+                    for (int j = 0; j < 2; j++) {
+                        // 2^127 at most: larger (queries beyond 2^115), and scores that differ at all
+                        // have weights 1 and 0 either way
+                        slq[nt][j] = fminf(fmaxf(sl * 0x1p24f * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f), 0x1p127f);
+                    }
                     o_lo[nt][0] = o_lo[nt][1] = o_lo[nt][2] = o_lo[nt][3] = 0.f;
                     se = kLeastScale;
                 } else {
@@ -505,7 +508,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     m[nt][j] = most_s[nt][j] = -INFINITY;
-                    l[nt][j] = off[nt][j] = 0.f;
+                    l[nt][j] = ref[nt][j] = 0.f;
                 }
 #pragma unroll
                 for (int x = 0; x < OT; x++) o[x][nt][0] = o[x][nt][1] = o[x][nt][2] = o[x][nt][3] = 0.f;
@@ -536,11 +539,6 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             if (__any_sync(0xffffffffu, most >= (uint32_t)(se + 3 + 15) << 26)) {
                 const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 26) - 15, 14);
                 const float f = __uint_as_float((uint32_t)(127 + se - e) << 23);
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    off[nt][0] += (float)(se - e);
-                    off[nt][1] += (float)(se - e);
-                }
                 se = e;
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -643,10 +641,10 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         for (int e = 4; e < 32; e <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, e));
                         const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
                         if (x != -INFINITY) {
-                            m[nt][j] = x;
-                            off[nt][j] = fmaf(-x, slq[nt][j], KV4 ? (float)(4 - se) : kWeightShift<M>);
-                            // as in attn_tc_kernel: steps of up to 8 binary orders leave m
-                            most_s[nt][j] = x + __fdividef(8.f, slq[nt][j]);
+                            m[nt][j] = ref[nt][j] = x;
+                            // as in attn_tc_kernel: steps of up to 8 binary orders leave m (rounded down:
+                            // what f16 holds allows no more, however large the scores are)
+                            most_s[nt][j] = __fadd_rd(x, __fdividef(8.f, slq[nt][j]));
                         }
                         l[nt][j] *= f;
                         if constexpr (KV4) o_lo[nt][j] *= f;
@@ -657,6 +655,9 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         }
                     }
             }
+            // (the difference first: slq s - slq ref would be as far off as slq ref is rounded,
+            // more than f16 holds from scores of 2^27 on)
+            const float shift = KV4 ? (float)(4 - se) : kWeightShift<M>;
             uint32_t pb[NT][MT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -664,7 +665,12 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                 for (int mt = 0; mt < MT; mt++) {
                     float e[4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) e[j] = ex2(fmaf(s[mt][nt][j], slq[nt][j & 1], off[nt][j & 1]));
+                    for (int j = 0; j < 4; j += 2) {
+                        const float2 x = __ffma2_rn(__fadd2_rn(make_float2(s[mt][nt][j], s[mt][nt][j + 1]), make_float2(-ref[nt][0], -ref[nt][1])),
+                                                    make_float2(slq[nt][0], slq[nt][1]), make_float2(shift, shift));
+                        e[j] = ex2(x.x);
+                        e[j + 1] = ex2(x.y);
+                    }
                     l[nt][0] += e[0] + e[2];
                     l[nt][1] += e[1] + e[3];
                     pb[nt][mt][0] = transpose8x8(pack2<M>(e[0], e[1]));
@@ -750,7 +756,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
-                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : log2f(sum) - off[nt][j];
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(ref[nt][j], slq[nt][j], log2f(sum) - (KV4 ? (float)(4 - se) : kWeightShift<M>));
                     if constexpr (KV4) {
                         // four neighbouring elements of each group
 #pragma unroll

@@ -520,7 +520,17 @@ attn_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     }
                 }
             }
-            const float off = m == -INFINITY ? 0.f : fmaf(-m, sl, kWeightShift<T>);
+            float off = m == -INFINITY ? 0.f : fmaf(-m, sl, kWeightShift<T>);
+            if constexpr (CROSS) {
+                // Scores so large that the rounding of m sl counts (beyond 2^27 it is more than
+                // f16 holds): the difference first.  Too dear for every step.
+                if (__any_sync(0xffffffffu, m != -INFINITY && fabsf(m) * sl >= 65536.f)) {
+                    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                    for (int i = 0; i < kAtTile; i++) s[i] -= base;
+                    off = m == -INFINITY ? 0.f : kWeightShift<T>;
+                }
+            }
             const float2 sl2 = make_float2(sl, sl), off2 = make_float2(off, off);
 #pragma unroll
             for (int c = 0; c < kAtTile / 64; c++) {

@@ -1,5 +1,5 @@
-"""One token over states and over the 4-bit cache where scores are far larger than
-a norm leaves: as long as they are finite in f32, the largest one's value results."""
+"""Tokens over states and one token over the 4-bit cache where scores are far larger
+than a norm leaves: as long as they are finite in f32, the largest one's value results."""
 import pytest
 import torch
 
@@ -8,7 +8,7 @@ from tests import _kv4, _read, _seq
 
 pytestmark = pytest.mark.gpu
 
-F16, BF16 = torch.float16, torch.bfloat16
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 
 
 def _keys(n, d, seed):
@@ -75,3 +75,25 @@ def test_one_hot_over_states(cuda_ok, dt, size, n, hq, d):
         return
     for h in range(hq):
         assert torch.equal(got[h], v[least if h % 2 else top, 0])
+
+
+@pytest.mark.parametrize("dt, size", [(F16, 1.0), (F16, 1e3), (F16, 65504.0), (BF16, 1e5), (BF16, 1e8), (BF16, 3e9), (BF16, 1e20), (BF16, 1e30),
+                                      (F32, 1e9), (F32, 1e30)])
+@pytest.mark.parametrize("n", [5, 300, 20000])
+@pytest.mark.parametrize("rows", [1, 3, 70, 300])
+@pytest.mark.parametrize("hq, d", [(2, 64), (8, 128), (2, 200)])
+def test_one_hot_of_packed_tokens(cuda_ok, dt, size, n, rows, hq, d):
+    """Beside them tokens of another sequence, whose scores are ordinary."""
+    k, top, least = _keys(min(n, 300), d, n)
+    k = torch.cat([k, torch.zeros(n - k.shape[0], 1, d, device="cuda", dtype=k.dtype)])
+    k = (k * (60000.0 if dt == F16 else 1.0)).to(dt)
+    g = torch.Generator("cuda").manual_seed(1)
+    v = torch.randn(n, 1, d, generator=g, device="cuda").to(dt)
+    q = torch.full((rows, hq, d), size, device="cuda", dtype=dt)
+    q[:, 1::2] *= -1
+    q1, k1, v1 = (torch.randn(m, h, d, generator=g, device="cuda").to(dt) for m, h in ((9, hq), (50, 1), (50, 1)))
+    got = attention.cross_attention(torch.cat([q, q1]), torch.cat([k, k1]), torch.cat([v, v1]), _read.starts([n, 50]),
+                                    cu_q=_read.starts([rows, 9]))
+    want = v[[least if h % 2 else top for h in range(hq)], 0]
+    assert torch.equal(got[:rows], want.expand(rows, -1, -1))
+    _seq.check(got[rows:], *_read.cross(q1, k1, v1, [9], [50]))

@@ -240,12 +240,16 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     using Tile = ReadTile<KV4, DC>;
     using M = std::conditional_t<KV4, __half, T>;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-    // Binary orders by which weights are held larger.  In 4 bits they are also
-    // multiplied with the groups' scales, below 2^(se + 3): 4 - se, so that 2^8 times
-    // both is what f16 holds, and se moves up only when a scale is too large.  (Values
-    // of a few units need no move; where they reach thousands, weights below 2^-5 of
-    // the largest begin to lose bits as subnormals.)
-    constexpr int kLeastScale = -3;
+    // Binary orders by which m may lag behind the scores.  In 4 bits weights are also
+    // multiplied with the groups' scales: weights of 2^7 2^4 times scales below 2^4 are
+    // what f16 holds.  In a tile with a larger scale, or with none of 2^-8, each group's
+    // are multiplied by a power of two before they are used, and its sums follow (both
+    // exactly, but for scales that become subnormal beside a larger one in their tile);
+    // weights stay as they are, so that no group or place coarsens what others add.  (64
+    // streams of up to 16384 places, bf16, in short runs: 145 us a call, 167 where every
+    // tile has scales above 2^4, that is values that span 240; 155 where none has 2^-8.)
+    constexpr float kLag = KV4 ? 4.f : 8.f;
+    constexpr uint32_t kLeastScale = 0x1C00u << 16, kMostScale = 0x4C00u << 16;  // 2^-8, 2^4
     constexpr int MT = Tile::kKeys / 16, OT = KV4 ? 2 * DC : DC;  // tiles of 16 keys; of 16 elements of V
     extern __shared__ __align__(16) char smem[];
     __shared__ unsigned scan[kRdThreads], warp_sums[kRdWarps];
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
     float ref[NT][2], most_s[NT][2];                   // weights are 2^(slq (s - ref) + shift), ref = m; scores above most_s move m
     float o[OT][NT][4], m[NT][2], l[NT][2];
     float o_lo[KV4 ? NT : 1][4];  // 4 bits: the weighted sums of the groups' lo
-    int se = kLeastScale;         // their scales are below 2^(se + 3)
+    int lift = 0;                 // the lane's group's (lane / 4) scales, and its sums in o, are 2^-lift of what they stand for
     bool fresh = true;
     int first_tile = 0, stage = 0;  // of the sequence's tiles; of the ring
     for (int i = 0; i < count; i++) {
@@ -496,7 +500,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         slq[nt][j] = fminf(fmaxf(sl * 0x1p24f * __shfl_sync(0xffffffffu, down, (c2 + j) * 4), 1e-37f), 0x1p127f);
                     }
                     o_lo[nt][0] = o_lo[nt][1] = o_lo[nt][2] = o_lo[nt][3] = 0.f;
-                    se = kLeastScale;
+                    lift = 0;
                 } else {
 #pragma unroll
                     for (int k = 0; k < 2 * DC; k++) {
@@ -531,24 +535,44 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         stage = stage + 1 == STAGES ? 0 : stage + 1;
         const uint32_t kt = smem_u32(st), vt = kt + Tile::kSide;
         if constexpr (KV4) {
+            // a lane has a place's (s, lo) of V
+            uint32_t *const pairs = (uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC;
             uint32_t pv[DC], most = 0;
-            shared_words<DC>((const uint32_t *)(st + 2 * Tile::kSide + Tile::kPairs) + lane * DC, pv);
+            shared_words<DC>(pairs, pv);
 #pragma unroll
             for (int g = 0; g < DC; g++) most = max2(most, pv[g]);  // of the lower halves
             most <<= 16;
-            if (__any_sync(0xffffffffu, most >= (uint32_t)(se + 3 + 15) << 26)) {
-                const int e = min((int)(__reduce_max_sync(0xffffffffu, most) >> 26) - 15, 14);
-                const float f = __uint_as_float((uint32_t)(127 + se - e) << 23);
-                se = e;
+            const bool tiny = !__any_sync(0xffffffffu, most >= kLeastScale);
+            if (tiny || __any_sync(0xffffffffu, most >= kMostScale || lift)) {
+                int next = tiny && r < DC ? -8 : 0;
+                if (__any_sync(0xffffffffu, most >= kMostScale)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if (j < 2) l[nt][j] *= f;
-                        o_lo[nt][j] *= f;
-#pragma unroll
-                        for (int t = 0; t < OT; t++) o[t][nt][j] *= f;
+                    for (int g = 0; g < DC; g++) {
+                        // s < 2^(need + 4); lift is left alone where it is one too many
+                        const int need = (int)(__reduce_max_sync(0xffffffffu, pv[g] & 0xffffu) >> 10) - 18;
+                        if (r == g) next = lift > 0 && lift == need + 1 ? lift : min(max(need, 0), 12);
                     }
+                }
+                if (__any_sync(0xffffffffu, next != lift)) {
+                    const float f = __uint_as_float((uint32_t)(127 + lift - next) << 23);
+                    lift = next;
+#pragma unroll
+                    for (int t = 0; t < OT; t++) {
+                        const float x = __shfl_sync(0xffffffffu, f, (t >> 1) * 4);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[t][nt][j] *= x;
+                    }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int g = 0; g < DC; g++) {
+                    const int k = __shfl_sync(0xffffffffu, lift, g * 4);
+                    const __half y = __hmul(__ushort_as_half((unsigned short)pv[g]), __ushort_as_half((unsigned short)(15 - k << 10)));
+                    pairs[g] = __byte_perm(pv[g], __half_as_ushort(y), 0x3254);
+                }
+                __syncwarp();
             }
         }
         {
@@ -642,9 +666,9 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                         const float f = x == m[nt][j] ? 1.f : ex2((m[nt][j] - x) * slq[nt][j]);
                         if (x != -INFINITY) {
                             m[nt][j] = ref[nt][j] = x;
-                            // as in attn_tc_kernel: steps of up to 8 binary orders leave m (rounded down:
+                            // as in attn_tc_kernel: steps of a few binary orders leave m (rounded down:
                             // what f16 holds allows no more, however large the scores are)
-                            most_s[nt][j] = __fadd_rd(x, __fdividef(8.f, slq[nt][j]));
+                            most_s[nt][j] = __fadd_rd(x, __fdividef(kLag, slq[nt][j]));
                         }
                         l[nt][j] *= f;
                         if constexpr (KV4) o_lo[nt][j] *= f;
@@ -657,7 +681,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
             }
             // (the difference first: slq s - slq ref would be as far off as slq ref is rounded,
             // more than f16 holds from scores of 2^27 on)
-            const float shift = KV4 ? (float)(4 - se) : kWeightShift<M>;
+            const float shift = kWeightShift<M>;
             uint32_t pb[NT][MT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -712,7 +736,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                             // row g: else lo + code s, which cancel, would not lose the same (f16 results
                             // 1.7 times as far off as a 16-bit cache's; 1.3 with it).  bf16 cannot tell.
                             if constexpr (!kBf16) {
-                                const uint32_t middle = r == g ? 0x47804780u : 0u;
+                                const uint32_t middle = r == g ? (0x4780u + (lift << 10)) * 0x10001u : 0u;  // 7.5 2^lift
                                 mma16816<M>(o_lo[nt], {middle, 0u, middle, 0u}, lost2(pb[nt][mt][0], s0, b0), lost2(pb[nt][mt][1], s1, b1));
                             }
                         }
@@ -744,10 +768,13 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     float sum = l[nt][j];
 #pragma unroll
                     for (int e = 4; e < 32; e <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, e);
-                    float low[KV4 ? DC : 1];
+                    float low[KV4 ? DC : 1], code[KV4 ? DC : 1];
                     if constexpr (KV4) {
 #pragma unroll
-                        for (int g = 0; g < DC; g++) low[g] = __shfl_sync(0xffffffffu, o_lo[nt][j], g * 4 + (lane & 3));
+                        for (int g = 0; g < DC; g++) {
+                            low[g] = __shfl_sync(0xffffffffu, o_lo[nt][j], g * 4 + (lane & 3));
+                            code[g] = __uint_as_float((uint32_t)(127 + 24 + __shfl_sync(0xffffffffu, lift, g * 4)) << 23);
+                        }
                     }
                     const int n = nt * 8 + c2 + j;
                     if (n >= heads) continue;
@@ -756,7 +783,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                     const long long oat = (long long)at.s * a.o_ts + (long long)(kvh * a.group + row0 + n) * a.o_hs;
                     const long long pat = (part * a.rows + n) * a.d;
                     if (!whole && r == 0)
-                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(ref[nt][j], slq[nt][j], log2f(sum) - (KV4 ? (float)(4 - se) : kWeightShift<M>));
+                        a.part_lse[part * a.rows + n] = sum == 0.f ? -INFINITY : fmaf(ref[nt][j], slq[nt][j], log2f(sum) - kWeightShift<M>);
                     if constexpr (KV4) {
                         // four neighbouring elements of each group
 #pragma unroll
@@ -765,7 +792,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 const float *t = o[2 * g + (e >> 1)][nt];
-                                x[e] = f * fmaf(e & 1 ? t[2 + j] - t[j] : t[j], e & 1 ? 0x1p20f : 0x1p24f, low[g]);
+                                x[e] = f * fmaf(e & 1 ? t[2 + j] - t[j] : t[j], e & 1 ? code[g] * 0.0625f : code[g], low[g]);
                             }
                             const int d = g * 32 + r * 4;
                             if (!whole) *(float4 *)(a.part_o + pat + d) = make_float4(x[0], x[1], x[2], x[3]);

@@ -26,8 +26,13 @@ def one_stream(q, k, v, ks, kl, vs, vl, scale, dt):
       weights     exponent (s - m) scale and its power of two in f32: 2^-23 of the
                   exponent and 2^-20; then to f16: 2^-11, or 2^-25 where subnormal
       p s         to f16: 2^-11 of code s, or 2^-25 where subnormal (times 2^-8
-                  where all scales are below 2^-8: they are held larger then).
-                  f16 results have what it lost put back times 7.5, the middle code:
+                  where all scales are below 2^-8: they are held larger then).  Where
+                  a tile's 32 places have a scale of 16 or more in a group, all of it
+                  are held 2^lift times smaller, and the largest is 2^(lift + 2) or
+                  more: 32 places of 15 2^(lift - 25), of a sum of 2^7 or more, are no
+                  more than 2^-29 of 15 times that scale; and scales that are subnormal
+                  then are off by 2^(lift - 25), 2^-27 of the largest, which counts by
+                  the tile's weight.  f16 results have what it lost put back times 7.5, the middle code:
                   code times the loss becomes code - 7.5 times it
       sums        in f32: 2^-23 for each 16 places
     """
@@ -43,7 +48,10 @@ def one_stream(q, k, v, ks, kl, vs, vl, scale, dt):
     size, whole = w @ v.abs(), w @ (15 * vs + vl.abs())
     codes = v - vl - (7.5 * vs if dt == torch.float16 else 0)  # times s
     limit = _seq.UNIT[dt] * out.abs() + _seq.TINY[dt] + wd @ v.abs() + 2.0 ** -11 * (size + w @ codes.abs())
-    limit = limit + (8 + n / 16) * 2.0 ** -23 * whole + 2.0 ** -32 * (15 * vs + vl.abs()).sum(0)
+    limit = limit + (8 + n / 16) * 2.0 ** -23 * whole + (2.0 ** -32 + 2.0 ** -29) * (15 * vs + vl.abs()).sum(0)
+    tile = torch.nn.functional.pad(vs, (0, 0, 0, -n % 32)).view(-1, 32, vs.shape[1]).amax(1)
+    share = torch.nn.functional.pad(w, (0, -n % 32)).view(w.shape[0], -1, 32).sum(-1)
+    limit = limit + 2.0 ** -27 * share @ (15 * tile * (tile >= 16))
     return out, limit + n * 15 * 2.0 ** -32 * (2.0 ** -8 if float(vs.max()) < 2.0 ** -8 else 1.0)
 
 

@@ -18,8 +18,8 @@
 // tiles end up in several warps, each leaves a partial result (O / l and log2 of
 // the weights' sum), and a second launch joins them:
 //   out = sum 2^(lse_i - lse) O_i.
-// Partial result number `warp + (head, sequence)` is its own for every pair that
-// meet, since both only grow along the list.  Fixed order throughout: results
+// A warp leaves two at most: number `warp` of the sequence that its part begins
+// within, `warps + warp` of the one that it ends within.  Fixed order throughout: results
 // repeat bit for bit.
 //
 // Rounding to fewer bits: the weights to 16 bits for the product with V (l sums
@@ -760,7 +760,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
         if (ends || i + 1 == count) {
             const bool whole = ends && first_tile == 0;
             const int kvh = at.head / a.zs, row0 = at.head % a.zs * (8 * NT), heads = min(a.group - row0, 8 * NT);
-            const long long part = (long long)worker + (long long)at.head * a.seqs + at.s;
+            const long long part = worker + (first_tile ? 0 : a.workers);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -850,7 +850,9 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
     const unsigned share = read_share(tiles * a.heads, a.workers), at = head * tiles + from, first = at / share;
     const int parts = (int)((at + n - 1) / share - first + 1);
     if (parts == 1) return;
-    const long long id = (long long)first + (long long)head * a.seqs + s, next = (long long)a.rows * a.d;
+    // of the first warp the part that it ends within, of the others those that they begin within
+    auto part = [&](int i) { return (long long)(i ? i : a.workers); };
+    const long long id = first, next = (long long)a.rows * a.d;
     const float *lse = a.part_lse + id * a.rows + row, *po = a.part_o + (id * a.rows + row) * a.d + lane * 4;
     // a warp every WARPS-th part, a lane four neighbouring elements (of 128 at a time);
     // the first on their way before the weights are known
@@ -861,7 +863,7 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
 #pragma unroll
         for (int k = 0; k < 2; k++)
             if (warp + i * WARPS < parts && k * 128 + lane * 4 < a.d)
-                y[i][k] = *(const float4 *)(po + (warp + i * WARPS) * next + k * 128);
+                y[i][k] = *(const float4 *)(po + part(warp + i * WARPS) * next + k * 128);
     float top = -INFINITY, sum = 0.f;
     float4 x[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
     auto weigh = [&](float w) { return w == -INFINITY ? 0.f : ex2(w - top); };
@@ -873,12 +875,12 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
     auto load = [&](int i, float4 (&z)[2]) {
 #pragma unroll
         for (int k = 0; k < 2; k++)
-            if (k * 128 + lane * 4 < a.d) z[k] = *(const float4 *)(po + i * next + k * 128);
+            if (k * 128 + lane * 4 < a.d) z[k] = *(const float4 *)(po + part(i) * next + k * 128);
     };
     if constexpr (MANY) {
         // the weights first, by all threads
         for (int i = threadIdx.x; i < parts; i += 32 * WARPS) {
-            const float w = lse[(long long)i * a.rows];
+            const float w = lse[part(i) * a.rows];
             weight[i] = w;
             top = fmaxf(top, w);
         }
@@ -903,12 +905,12 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
             add(weight[i], z);
         }
     } else {
-        for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[(long long)i * a.rows]);
+        for (int i = lane; i < parts; i += 32) top = fmaxf(top, lse[part(i) * a.rows]);
         top = warp_max(top);
 #pragma unroll
         for (int i = 0; i < kFirst; i++)
             if (warp + i * WARPS < parts) {
-                const float f = weigh(lse[(long long)(warp + i * WARPS) * a.rows]);
+                const float f = weigh(lse[part(warp + i * WARPS) * a.rows]);
                 sum += f;
                 add(f, y[i]);
             }
@@ -916,7 +918,7 @@ __global__ void __launch_bounds__(32 * WARPS) read_join_kernel(const JoinArgs a)
         for (int i = warp + kFirst * WARPS; i < parts; i += WARPS) {
             float4 z[2];
             load(i, z);
-            const float f = weigh(lse[(long long)i * a.rows]);
+            const float f = weigh(lse[part(i) * a.rows]);
             sum += f;
             add(f, z);
         }
@@ -958,7 +960,7 @@ static ReadPlan read_plan(bool kv4, uint32_t seqs, uint64_t most, uint32_t kv_he
     w.rows = (int)std::min<uint32_t>(group, 8 * w.nt);
     w.workers = read_blocks(kv4, read_dc(kv4, d), w.nt) * tc_sm_count() * kRdWarps;
     w.tiles = (most / (kv4 ? 32 : 16) + seqs) * w.heads;
-    const uint64_t parts = (uint64_t)w.workers + (uint64_t)w.heads * seqs;
+    const uint64_t parts = 2ull * w.workers;
     auto up = [](uint64_t x) { return (x + 31) / 32 * 32; };
     w.lse_at = up((seqs + 1ull) * 4);
     w.o_at = up(w.lse_at + parts * w.rows * 4);

@@ -230,8 +230,22 @@ __device__ __forceinline__ void read_store4(const ReadArgs &a, long long at, con
     }
 }
 
-// Blocks of an SM.
-constexpr int read_blocks(bool kv4, int dc, int nt) { return nt == 1 && dc <= 4 ? 3 : 2; }
+// Blocks of an SM.  With 16-bit heads of more than 128 the rings of two would hold one
+// tile a warp.  (One block of three stages, all at once: 64 sequences of 2000 states, 8/2
+// heads of 256, 57 us, one after the other of two stages 64.5; 500 of 1-999, 8/4 heads of
+// 160, 152 and 158; 300 of 500, 8 heads of 200, 214 and 199.)
+constexpr int read_blocks(bool kv4, int dc, int nt) { return nt == 1 && dc <= 4 ? 3 : !kv4 && dc > 8 ? 1 : 2; }
+
+// A ring's stages: as many, up to six, as let all blocks of an SM fit it with their
+// static shared memory and what the system keeps (1 KB a block).
+constexpr uint32_t kReadOther = 1024 + 1280;
+template <bool KV4, int DC, int NT>
+struct ReadRing {
+    static constexpr uint32_t kOne = kRdWarps * ReadTile<KV4, DC>::kStage;
+    static constexpr uint32_t kRoom = 228 * 1024 / read_blocks(KV4, DC, NT) - kReadOther;
+    static constexpr int kStages = kRoom / kOne > 6 ? 6 : kRoom / kOne;
+    static_assert(kStages >= 2 && kStages * kOne <= 227 * 1024, "two tiles a warp, all blocks of an SM at once");
+};
 
 // T: the type of queries and results; that of the products is f16 in 4 bits.
 template <typename T, bool KV4, int DC, int NT, int STAGES>
@@ -976,9 +990,8 @@ cudaError_t read4_run_bf16(const ReadArgs &a, int nt, cudaStream_t s);
 template <typename T, bool KV4, int DC, int NT>
 static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
 {
-    // the deepest ring with which all blocks of an SM fit it
-    constexpr uint32_t one = kRdWarps * ReadTile<KV4, DC>::kStage, room = (228 * 1024 / read_blocks(KV4, DC, NT) - 1024 - 1280) / one;
-    constexpr int stages = room > 6 ? 6 : room < 2 ? 2 : (int)room;
+    constexpr int stages = ReadRing<KV4, DC, NT>::kStages;
+    constexpr uint32_t one = ReadRing<KV4, DC, NT>::kOne;
     auto *fn = &read_kernel<T, KV4, DC, NT, stages>;
     cudaError_t e = ensure_smem_attr((const void *)fn, stages * one);
     if (e != cudaSuccess) return e;

@@ -188,13 +188,26 @@ __global__ void __launch_bounds__(kTileThreads, J == 4 ? 1 : 2) cross_tile_kerne
     const long long unit = blockIdx.x / heads;
 
     // ---- whose rows these are
-    if (warp == 0) {
+    if (!a.cu_q) {
+        // a token each: as many tiles for every sequence
+        if (tid == 0) {
+            const int tiles = (a.group + kTileRows - 1) / kTileRows;
+            const long long s = unit / tiles;
+            work[0] = s < a.seqs ? (int)s + 1 : 0;
+            if (s < a.seqs) {
+                work[1] = (int)s; work[2] = 1;
+                work[3] = min(max(a.cu_k[s], 0), a.keys);
+                work[4] = max(min(a.cu_k[s + 1], a.keys) - work[3], 0);
+                *(long long *)tile_smem = (unit - s * tiles) * kTileRows;
+            }
+        }
+    } else if (warp == 0) {
         if (lane == 0) work[0] = 0;
         __syncwarp();
         long long before = 0;
         for (int s0 = 0; s0 < a.seqs; s0 += 32) {
             const int s = min(s0 + lane, a.seqs), next = min(s + 1, a.seqs);
-            const int from = min(a.cu_q ? max(a.cu_q[s], 0) : s, a.tokens), n = max(min(a.cu_q ? a.cu_q[next] : next, a.tokens) - from, 0);
+            const int from = min(max(a.cu_q[s], 0), a.tokens), n = max(min(a.cu_q[next], a.tokens) - from, 0);
             const long long mine = ((long long)n * a.group + kTileRows - 1) / kTileRows;
             long long upto = mine;
 #pragma unroll

@@ -85,7 +85,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_k: tor
     sequence s's one token, as in a step of a batch.  cu_q and cu_k are int32
     CUDA tensors [sequences + 1]; they are not copied to the host.  scale
     defaults to head_dim ** -0.5.  A sequence without states gives zeros; tokens
-    of no sequence are left as they are in out, undefined without it."""
+    of no sequence are left as they are in out, undefined without it.  out
+    overlaps no input."""
     return _lib.seqcall().cross_attention(q, k, v, cu_k, cu_q, scale, out, stream)
 
 
@@ -103,8 +104,9 @@ def kv4_file(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: t
 def kv4_load(k_pages: torch.Tensor, v_pages: torch.Tensor, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16,
              stream=None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values at slots of a 4-bit cache (aie_kv4_load) as k and v [tokens,
-    kv_heads, head_dim], for instance to attend a prompt's next part to its
-    first; a slot outside the cache (-1) gives zeros."""
+    kv_heads, head_dim]; a slot outside the cache (-1) gives zeros.  A prompt's
+    next part attends to its first by prompt_attention over both, the first
+    part's keys and values read back and its queries handed in again."""
     return _lib.seqcall().kv4_load(k_pages, v_pages, slots, dtype, stream)
 
 
@@ -116,5 +118,5 @@ def kv4_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     first lens[b] places (int32 CUDA tensor), in pages table[b, place //
     page_size].  A stream without places gives zeros; what stands behind a
     stream's places never reaches its result.  max_len bounds lens (default: what
-    a table row holds); longer streams are cut off there."""
+    a table row holds); longer streams are cut off there.  out overlaps no input."""
     return _lib.seqcall().kv4_attention(q, k_pages, v_pages, table, lens, max_len, scale, out, stream)

@@ -48,6 +48,9 @@
 // first copies and the exchange are the rest.  Long texts over states (5095 tokens,
 // 32/8 heads of 128) run at the prompts' rate, 1.02 PFLOP/s.
 //
+// At 168 registers a thread the prompts' form spills 8 bytes, the paged one 12,
+// that of states 8, FEW 72 (32 with heads of up to 64).
+//
 // Every wait is bounded (1 s); on expiry the block records an error code,
 // waits for its copies in flight, frees its tensor memory and returns.
 #pragma once

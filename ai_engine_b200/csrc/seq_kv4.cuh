@@ -14,6 +14,7 @@
 // A group is read once and written once: memory-bound.  16384 tokens of 8 heads
 // of 128 in bf16, k and v: 67 MB read, 21 MB written in 30 us (2.9 TB/s; issue slots
 // 67%: the arithmetic of two roundings an element); read back in 20 us (4.4 TB/s).
+// Filing with 64 registers (8 blocks an SM) spills 28 bytes a thread, 60 in f32.
 #pragma once
 #include "seq_rope.cuh"
 

@@ -27,8 +27,8 @@
 // result, and over the 4-bit cache the weights times the scales to f16 for the
 // product with the codes.  What that last rounding loses is put back, times the
 // middle code, where results are f16 (1.75 times a 32-bit computation's error
-// without, 1.3 with); a bf16 result's own rounding is 8 times as large, and the
-// kernel takes 153 us with it for 140 without in the second case below.
+// without, 1.3 with); a bf16 result's own rounding is 8 times as large, and in
+// the second case below the kernel takes 139 us without it, 151 with it.
 //
 // Over the 4-bit cache the work is on the codes: 32 elements of a place and head
 // are 20 bytes, which come in 0.9 cycles of an SM at the memory's rate; one
@@ -38,13 +38,13 @@
 // rate; scales go into the weights, lowest values into a product of their own.
 //
 // Measured (states larger than L2): 96 streams of up to 2855 states of 8 heads of
-// 128, bf16: 109 us a call, 561 MB at 5.1 TB/s; its issue slots are used 26%.  4
+// 128, bf16: 109 us a call, 561 MB at 5.1 TB/s; its issue slots are used 25%.  4
 // bits, 64 streams of up to 16384 places of 8 heads of 128, 4 query heads each:
-// 138 us a call (666 MB at 4.8 TB/s) in runs of some milliseconds, 157 in long
-// ones, where the power limit takes the clock from 1.95 to 1.72 GHz; issue slots
-// 52%, logic pipe about 50%; 5.6 TB/s once all warps run, after 9 us to a
-// warp's first tile, and blocks of an SM end unevenly (with the f16 results'
-// correction between 102 and 153 us).  Parts taken from a counter end together but
+// 137 us a call (666 MB at 4.9 TB/s) in runs of some milliseconds, 155 in long
+// ones, where the power limit takes the clock from 1.95 to 1.72 GHz (f16 results
+// 149 and 166); issue slots 52%, logic pipe about 50%; 5.6 TB/s once all warps
+// run, after 9 us to a warp's first tile, and blocks of an SM end unevenly (with
+// the f16 results' correction between 102 and 153 us).  Parts taken from a counter end together but
 // cost 165-178 us (each part begins with its own queries); 4 blocks an SM of 128
 // registers 146-148; 16 places a tile 154.
 #pragma once
@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(kRdThreads, read_blocks(KV4, DC, NT)) read_ker
                             // row g: else lo + code s, which cancel, would not lose the same (f16 results
                             // 1.7 times as far off as a 16-bit cache's; 1.3 with it).  bf16 cannot tell.
                             if constexpr (!kBf16) {
-                                const uint32_t middle = r == g ? (0x4780u + (lift << 10)) * 0x10001u : 0u;  // 7.5 2^lift
+                                const uint32_t middle = r == g ? (uint32_t)(0x4780 + lift * 1024) * 0x10001u : 0u;  // 7.5 2^lift
                                 mma16816<M>(o_lo[nt], {middle, 0u, middle, 0u}, lost2(pb[nt][mt][0], s0, b0), lost2(pb[nt][mt][1], s1, b1));
                             }
                         }
@@ -1004,7 +1004,9 @@ static cudaError_t read_launch(const ReadArgs &a, cudaStream_t s)
     if (e != cudaSuccess) return e;
     const JoinArgs j{a.out, a.o_ts, a.o_hs, a.before, a.part_lse, a.part_o, a.seqs, a.hq, a.group, a.d, a.zs, a.heads, a.rows, a.bf16,
                      a.workers};
-    // warps a row, by its parts: with two each (256 streams of up to 1900 places in 4 bits)
+    // warps a row, by its parts, as many as there were if all sequences had the same length
+    // (the host does not know them; a long one among many short ones is joined by few warps
+    // for its parts: 50000 states among 95 sequences of 100, 73 us a call): with two each (256 streams of up to 1900 places in 4 bits)
     // 87.4 us a call of two warps, 91.3 of four; with three (96 of 5000) 83.4 and 81.5; with
     // 600 (one of 9682 states) 14.8 of sixteen, 21 of eight, 31 of four; with 15, 14.4 of
     // four and 15.5 of sixteen

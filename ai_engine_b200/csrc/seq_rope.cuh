@@ -229,7 +229,8 @@ __device__ __forceinline__ void load_floats(const float *p, float *f)
 // pair's axis.  A lane whose pairs all have one axis reads its angles as before,
 // from that axis' row; others read theirs one by one (1297 tokens of 20 + 5 heads
 // of 96, axes taking turns: 6.7 us a call).  16350 tokens of 32 + 8 heads of 128,
-// three axes, filed: 86 us, 5.2 TB/s.
+// three axes, filed: 87 us, 436 MB at 5.0 TB/s; with the axes taking turns 89; pairs
+// of neighbours 92, and 95 with turns.
 constexpr int kRopeThreads = 128, kRopeBlocks = 5;
 struct RopeVec {
     unsigned q_units, k_units;  // groups of HPT heads of a token

@@ -23,6 +23,11 @@
  * and the detail in aie_last_error.  Arguments come in one struct, all of
  * whose unused bytes are zero.  Strides are in elements.  Query head h reads
  * key/value head h / (q_heads / kv_heads).
+ *
+ * Attention's scores are held in f32: q . k and scale log2(e) q . k have to be
+ * finite there.  aie_prompt_attn and aie_prefix_attn on the tensor cores (16 bits,
+ * heads of up to 128) take |scale log2(e) q . k| up to 2^24; beyond that, f16
+ * weights can overflow and give NaN.
  */
 #ifndef AIE_SEQ_H
 #define AIE_SEQ_H
@@ -110,7 +115,9 @@ AIE_API int aie_prompt_attn(const aie_prompt *p, void *stream);
  * NaN among them, never reach a result.  out overlaps no input.
  * workspace: aie_cross_attn_workspace(p) bytes (p as in the call, apart from
  * these two), 16-byte aligned, its contents unspecified before and after; calls
- * that may overlap need one each. */
+ * that may overlap need one each.
+ * With cu_q every block looks for its tokens from the first sequence on: the cost
+ * of that grows with the square of the sequences (thousands, not millions, of them). */
 typedef struct aie_cross {
     aie_heads q, k, v, out;
     const int32_t *cu_q, *cu_k;
@@ -152,9 +159,9 @@ AIE_API int aie_prefix_attn(const aie_prefix *p, void *stream);
 
 /* A paged cache of keys and values in 4 bits.  Elements 32 g .. 32 g + 31 of a
  * head are a group with a scale s and a lowest value lo, both f16: its elements
- * are lo + code * s, codes 0 to 15, s finite and not negative.  The block of page p and head h is the
- * page_size * head_dim * 5 / 8 bytes at k + p * page_stride + h * (block bytes)
- * (v alike): first the codes, head_dim / 2 bytes a place, two to a byte, the even
+ * are lo + code * s, codes 0 to 15, s finite and not negative.  The block of
+ * page p and head h is the page_size * head_dim * 5 / 8 bytes at
+ * k + p * page_stride + h * (block bytes) (v alike): first the codes, head_dim / 2 bytes a place, two to a byte, the even
  * element in the low half; then the groups' (s, lo) pairs, head_dim / 8 bytes a
  * place.  head_dim is a multiple of 32 up to 256, page_size of 8; k, v and
  * page_stride (in bytes) are 16-byte aligned. */
@@ -192,6 +199,8 @@ AIE_API int aie_kv4_load(const aie_kv4_rows *p, void *stream);
  * outside the cache are never read from; the stream's result is then
  * unspecified.  Places from lens[b] on, whatever they hold, never reach stream
  * b's result.  out overlaps no input.
+ * A place of V whose group spans far more than the others' adds at most 2^-26 of
+ * that span to the error of the group's 32 elements, whatever its weight is.
  * workspace: aie_kv4_attn_workspace(p) bytes, 16-byte aligned, its contents
  * unspecified before and after; calls that may overlap need one each. */
 typedef struct aie_kv4_step {
